@@ -35,7 +35,7 @@
 extern "C" {
 #endif
 
-#define W8A8_ABI_VERSION 7
+#define W8A8_ABI_VERSION 8
 
 typedef enum w8a8_dtype {
   W8A8_F32 = 0,
@@ -92,6 +92,13 @@ typedef enum w8a8_row_layout {
    * (_pack_gateup_tensors layout "interleave", lightweight_runner.py:81-92) */
   W8A8_ROWS_INTERLEAVE_HALVES = 1
 } w8a8_row_layout;
+
+typedef enum w8a8_rotary_layout {
+  /* pairs of elements (i, i + rotary_dim / 2) of a head */
+  W8A8_ROTARY_HALF = 0,
+  /* pairs of neighbours (2i, 2i + 1) */
+  W8A8_ROTARY_INTERLEAVED = 1
+} w8a8_rotary_layout;
 
 /* Library ABI version (W8A8_ABI_VERSION). */
 int w8a8_abi_version(void);
@@ -470,6 +477,106 @@ int w8a8_dequant_i32_bf16(const int32_t* acc, int64_t ld_acc, const uint16_t* sa
 int w8a8_dense_gemv(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
                     void* y, int64_t ldy, int dtype, int64_t m, int64_t n, int64_t k,
                     hipStream_t stream);
+
+/*
+ * The attention core of a decoder layer: rotary positions, the store into a
+ * paged key-value cache, and attention over it (the precomputed branch of
+ * PagedLlamaAttention.forward, paged_attention.py:1284-1307, 1354-1440).
+ *
+ * Rows are 16-bit [tokens, heads, head_dim] with any token and head stride in
+ * elements (not negative) and contiguous heads: the views of a packed QKV
+ * product are taken as they are.  head_dim is a multiple of 8, at most 256.
+ * A cache is two tensors of equal shape [pages, kv_heads, page_size, head_dim]
+ * and equal strides (elements; head_dim contiguous, the other axes in any
+ * order); page_size is a power of two up to 2^20.  Offsets are 64-bit.
+ */
+
+/*
+ * Rotary positions: y = x with each pair i < rotary_dim / 2 of a head turned
+ * by positions[t] * inv_freq[i] (radians, formed in binary64), (a, b) ->
+ * (a c - b s, b c + a s) with c = factor * cos, s = factor * sin, computed in
+ * binary32 and rounded once to `dtype` (W8A8_F16 or W8A8_BF16); elements from
+ * rotary_dim (even, may be 0) on are copied.  y may be x itself (same pointer
+ * and strides); any other overlap returns W8A8_ERR_OVERLAP.  positions:
+ * [tokens], any int64 values; inv_freq: [rotary_dim / 2].  factor: the
+ * amplitude of scaled long-context frequencies, 1 otherwise.
+ */
+int w8a8_rotary(const void* x, int64_t x_stride_t, int64_t x_stride_h, int dtype,
+                const int64_t* positions, const double* inv_freq, int64_t rotary_dim, int layout,
+                float factor, void* y, int64_t y_stride_t, int64_t y_stride_h, int64_t tokens,
+                int64_t heads, int64_t head_dim, hipStream_t stream);
+
+/*
+ * w8a8_rotary of q into q_out, and in the same launch the rotated k and the
+ * unchanged v into the cache (_store_kvcache_kernel, paged_attention.py:332-385):
+ * token t goes to row slots[t] % page_size of page slots[t] / page_size.  A
+ * slot outside [0, pages * page_size) is not written (padded rows: -1); the
+ * others must differ from each other.  q_out may be q itself; k, v and q_out
+ * overlap nothing else, though q, k and v may be column ranges of one matrix.
+ */
+int w8a8_rotary_store(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
+                      int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
+                      int64_t v_stride_h, int dtype, const int64_t* positions,
+                      const int64_t* slots, const double* inv_freq, int64_t rotary_dim, int layout,
+                      float factor, void* q_out, int64_t q_out_stride_t, int64_t q_out_stride_h,
+                      void* k_cache, void* v_cache, int64_t cache_stride_page,
+                      int64_t cache_stride_head, int64_t cache_stride_token, int64_t pages,
+                      int64_t page_size, int64_t tokens, int64_t q_heads, int64_t kv_heads,
+                      int64_t head_dim, hipStream_t stream);
+
+/*
+ * Attention of one new token per sequence over the paged cache
+ * (_paged_decode_attention_*_kernel, paged_attention.py:408-845):
+ *   out[b, h] = sum_j p_j v_j,  p = softmax_j(scale * q[b, h] . k_j),  j < lengths[b]
+ * where key j of sequence b is row j % page_size of page
+ * page_table[b * ld_table + j / page_size], head h / (q_heads / kv_heads).
+ * Scores, softmax and sums are binary32, out is rounded once.
+ * lengths[b] <= 0 gives zeros; a length past table_pages * page_size is cut
+ * to it.  Entries of the table past a sequence's pages are not used.  A page
+ * outside [0, pages) is never read: its keys are masked.
+ * q and out: 16-byte aligned, strides multiples of 8, as the cache's; out
+ * overlaps no input.  Workspace: w8a8_paged_decode_workspace_bytes(batch,
+ * q_heads, kv_heads, head_dim, table_pages * page_size) bytes (0 where the
+ * cache is not split over its length), 16-byte aligned; no state survives the
+ * call.
+ */
+int w8a8_paged_decode(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_cache,
+                      const void* v_cache, int64_t cache_stride_page, int64_t cache_stride_head,
+                      int64_t cache_stride_token, int64_t pages, int64_t page_size,
+                      const int32_t* page_table, int64_t ld_table, int64_t table_pages,
+                      const int32_t* lengths, int dtype, float scale, void* out,
+                      int64_t out_stride_t, int64_t out_stride_h, int64_t batch, int64_t q_heads,
+                      int64_t kv_heads, int64_t head_dim, void* workspace,
+                      int64_t workspace_bytes, hipStream_t stream);
+
+/* Workspace bytes of w8a8_paged_decode; -1 for sizes it does not take. */
+int64_t w8a8_paged_decode_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                          int64_t head_dim, int64_t max_keys);
+
+/*
+ * Causal attention of prompts, or of chunks of them behind a cached part, over
+ * the paged cache (_paged_varlen_attention_kernel, paged_attention.py:1037-1141).
+ * Rows q_starts[b] .. q_starts[b + 1] - 1 of q (n of them; q_starts: [batch + 1],
+ * not decreasing) are sequence b's newest tokens, whose keys the cache already
+ * holds: row i of them sees keys j <= lengths[b] - n + i, and with none the
+ * output row is zeros.  Rows of no sequence are left as they were.  Scores and
+ * sums are binary32; the probabilities are rounded to `dtype` for their
+ * product with v, and the same rounded values are summed.  Otherwise as
+ * w8a8_paged_decode; workspace w8a8_paged_prefill_workspace_bytes(tokens,
+ * batch, q_heads, kv_heads, head_dim, table_pages * page_size).
+ */
+int w8a8_paged_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_cache,
+                       const void* v_cache, int64_t cache_stride_page, int64_t cache_stride_head,
+                       int64_t cache_stride_token, int64_t pages, int64_t page_size,
+                       const int32_t* page_table, int64_t ld_table, int64_t table_pages,
+                       const int32_t* lengths, const int32_t* q_starts, int dtype, float scale,
+                       void* out, int64_t out_stride_t, int64_t out_stride_h, int64_t tokens,
+                       int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                       void* workspace, int64_t workspace_bytes, hipStream_t stream);
+
+/* Workspace bytes of w8a8_paged_prefill; -1 for sizes it does not take. */
+int64_t w8a8_paged_prefill_workspace_bytes(int64_t tokens, int64_t batch, int64_t q_heads,
+                                           int64_t kv_heads, int64_t head_dim, int64_t max_keys);
 
 #ifdef __cplusplus
 }

@@ -1,7 +1,8 @@
 // extern "C" entry points of libw8a8_gfx950.so (declared in
 // include/w8a8_gfx950.h).  Validation and dispatch only: shapes, dtypes,
 // alignment and workspace are checked here and reported as status codes; the
-// kernels live in quant.hip, gemv.hip and gemm.hip.
+// kernels live in quant.hip, gemv.hip and gemm.hip.  The attention core's entry
+// points are in capi_attention.hip.
 #include <mutex>
 #include <utility>
 
@@ -36,12 +37,6 @@ constexpr int64_t kMaxK = ((int64_t{1} << 31) - 1) / (127 * 127);
 // launch one workgroup per row in the quantizers; the margin keeps a count
 // rounded up to whole 256-row tiles inside int as well.
 constexpr int64_t kMaxRows = INT32_MAX - 256;
-
-inline int status_of(hipError_t e) {
-  if (e == hipSuccess) return W8A8_OK;
-  g_last_hip_error = static_cast<int>(e);
-  return W8A8_ERR_HIP;
-}
 
 inline bool aligned(const void* p, uintptr_t a) {
   return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0;
@@ -439,6 +434,12 @@ int scratch_address(void** out) {
 }
 
 }  // namespace
+
+int w8a8::status_of(hipError_t e) {
+  if (e == hipSuccess) return W8A8_OK;
+  g_last_hip_error = static_cast<int>(e);
+  return W8A8_ERR_HIP;
+}
 
 extern "C" {
 

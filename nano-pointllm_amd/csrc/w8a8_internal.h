@@ -227,4 +227,73 @@ hipError_t launch_gemv_dense(const void* x, int64_t ldx, const void* w, int64_t 
                              const void* bias, void* y, int64_t ldy, int dtype, int64_t M,
                              int64_t N, int64_t K, hipStream_t st);
 
+// Rotary positions (rotary.hip) over 16-bit rows [tokens, heads, head_dim]
+// with token and head strides in elements: q into q_out (which may be q
+// itself), and with k (nullable) the rotated k and v into the paged cache's
+// slots; a slot outside [0, pages << page_shift) is skipped.  Elements of a
+// head are contiguous.
+constexpr int kRotaryMaxDim = 256;
+struct RotaryRows {
+  const void* q;
+  int64_t q_st, q_sh;
+  const void* k;
+  int64_t k_st, k_sh;
+  const void* v;
+  int64_t v_st, v_sh;
+  const int64_t* positions;  // [tokens]
+  const int64_t* slots;      // [tokens], with k
+  const double* inv_freq;    // [rotary_dim / 2], radians per position
+  void* q_out;
+  int64_t qo_st, qo_sh;
+  void* k_cache;
+  void* v_cache;
+  int64_t c_page, c_head, c_tok;  // cache strides in elements
+  int64_t pages;
+  int64_t tokens;
+  int page_shift;
+  int q_heads, kv_heads, head_dim;  // kv_heads 0 without k
+  int rotary_dim;
+  bool half;  // pairs (i, i + rotary_dim / 2), else (2i, 2i + 1)
+  float factor;
+};
+hipError_t launch_rotary(const RotaryRows& r, int dtype, hipStream_t st);
+
+// Attention of 16-bit query rows over a paged cache: one row per sequence
+// (q_starts null, tokens == batch: it sees all lengths[b] keys), or rows
+// q_starts[b] .. q_starts[b + 1] - 1 of sequence b, the last of which sees all
+// lengths[b] keys and each other one key fewer than the next.  Key j of
+// sequence b is row j % page of page table[b * ld_table + j / page]; lengths
+// past max_keys are cut to it, and keys of a page outside [0, pages) are
+// masked, never read.  A row without keys is written as zeros; rows of no
+// sequence are not written.
+struct PagedAttention {
+  const void* q;
+  int64_t q_st, q_sh;
+  const void* k;
+  const void* v;
+  int64_t c_page, c_head, c_tok;
+  int64_t pages;
+  const int32_t* table;
+  int64_t ld_table;
+  const int32_t* lengths;
+  const int32_t* q_starts;
+  void* out;
+  int64_t o_st, o_sh;
+  void* workspace;
+  int page_shift;
+  int max_keys;
+  int batch, tokens, q_heads, kv_heads, head_dim;
+  float scale;
+};
+constexpr int kAttentionMaxDim = 256;
+int64_t paged_decode_workspace(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                               int64_t max_keys);
+int64_t paged_prefill_workspace(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                int64_t head_dim, int64_t max_keys);
+hipError_t launch_paged_decode(const PagedAttention& p, int dtype, hipStream_t st);
+hipError_t launch_paged_prefill(const PagedAttention& p, int dtype, hipStream_t st);
+
+// The w8a8_status of a launch; a failure is kept for w8a8_last_hip_error.
+int status_of(hipError_t e);
+
 }  // namespace w8a8

@@ -16,6 +16,9 @@ Public surface:
   model for the W8A8 modules, plus the packed call-site helpers.
 * :mod:`nanopointllm_amd.runner` - a decoder stack in the shape of
   ``LightweightLlamaRunner`` on the W8A8 modules, capturable in a HIP graph.
+* :mod:`nanopointllm_amd.attention` - the runner's attention core: rotary
+  positions, a paged key-value cache and attention over it, for prompts and
+  for single tokens.
 * :mod:`nanopointllm_amd.calibration` - activation range collection, QDQ
   hooks, weight fake-quant and SmoothQuant smoothing.
 * :mod:`nanopointllm_amd.integer_epilogues` - the int32 -> int8

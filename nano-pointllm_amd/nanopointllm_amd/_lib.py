@@ -13,12 +13,13 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "libw8a8_gfx950.so"
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 F32, F16, BF16, I32, I8 = 0, 1, 2, 3, 4
 EPI_I32, EPI_DEQUANT, EPI_SILU_MUL, EPI_SILU_MUL_Q8 = 0, 1, 2, 3
 EPI_REQUANT, EPI_DEQUANT_BF16_EXACT = 4, 5
 ROWS_AS_IS, ROWS_INTERLEAVE_HALVES = 0, 1
+ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1
 
 OK = 0
 ERR_NULL, ERR_SHAPE, ERR_DTYPE, ERR_ALIGN, ERR_WORKSPACE, ERR_HIP = -1, -2, -3, -4, -5, -6
@@ -70,6 +71,12 @@ EXPORTED_SYMBOLS = (
     "w8a8_requantize_i32",
     "w8a8_dequant_i32_bf16",
     "w8a8_dense_gemv",
+    "w8a8_rotary",
+    "w8a8_rotary_store",
+    "w8a8_paged_decode",
+    "w8a8_paged_decode_workspace_bytes",
+    "w8a8_paged_prefill",
+    "w8a8_paged_prefill_workspace_bytes",
 )
 
 _lock = threading.Lock()
@@ -123,6 +130,19 @@ _SIGNATURES = {
     "w8a8_dequant_i32_bf16": (_int, [_vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
     "w8a8_dense_gemv": (_int, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _int, _i64, _i64, _i64,
                                _vp]),
+    "w8a8_rotary": (_int, [_vp, _i64, _i64, _int, _vp, _vp, _i64, _int, _f32, _vp, _i64, _i64,
+                           _i64, _i64, _i64, _vp]),
+    "w8a8_rotary_store": (_int, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _int, _vp,
+                                 _vp, _vp, _i64, _int, _f32, _vp, _i64, _i64, _vp, _vp, _i64,
+                                 _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp]),
+    "w8a8_paged_decode": (_int, [_vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp,
+                                 _i64, _i64, _vp, _int, _f32, _vp, _i64, _i64, _i64, _i64, _i64,
+                                 _i64, _vp, _i64, _vp]),
+    "w8a8_paged_decode_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64]),
+    "w8a8_paged_prefill": (_int, [_vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp,
+                                  _i64, _i64, _vp, _vp, _int, _f32, _vp, _i64, _i64, _i64, _i64,
+                                  _i64, _i64, _i64, _vp, _i64, _vp]),
+    "w8a8_paged_prefill_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64]),
 }
 
 
