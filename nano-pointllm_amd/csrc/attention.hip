@@ -108,14 +108,10 @@ hipError_t launch_rows(const PagedAttention& p, int dtype, hipStream_t st) {
 
 }  // namespace
 
-int64_t paged_decode_workspace(int64_t, int64_t, int64_t, int64_t, int64_t) { return 0; }
 int64_t paged_prefill_workspace(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t) {
   return 0;
 }
 
-hipError_t launch_paged_decode(const PagedAttention& p, int dtype, hipStream_t st) {
-  return launch_rows(p, dtype, st);
-}
 hipError_t launch_paged_prefill(const PagedAttention& p, int dtype, hipStream_t st) {
   return launch_rows(p, dtype, st);
 }

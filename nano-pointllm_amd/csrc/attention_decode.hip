@@ -1,0 +1,485 @@
+// Attention of one new token per sequence over a paged key-value cache
+// (gfx950).
+//
+// Mathematics.  Per sequence and key head, with the queries q_0 .. q_{G-1}
+// that share the head as columns: S^T = K Q^T, P = 2^(S^T c - r) with c = scale
+// log2(e) and a running reference r per query, O^T = V^T P, l = sum P; the
+// result is O / l.  The reference follows the running maximum lazily: scores
+// may exceed the maximum it was set from by 2^8 before it is raised, and it
+// lies 7 below that maximum, so a probability is at most 2^15 and one of
+// 2^-31 of the largest still counts in binary16.
+//
+// Bound by memory: every key and value is read once, 4 head_dim bytes per key
+// and key head against 4 head_dim G operations.
+//
+// Design:
+//   * A wavefront takes tiles of 32 keys through v_mfma_f32_16x16x32 with the
+//     queries as the 16 columns, for any G up to 16: with one query 15/16 of
+//     the product is unused, and it still costs a tenth of the tile's bytes.
+//   * Nothing goes through LDS in the loop.  A lane's 8 scores of a tile are
+//     those of the 8 keys whose values it loads, so the probabilities are the
+//     second product's operand as they are: the matrix instruction's inner
+//     index is summed over, so any order of keys will do that both operands
+//     share.  A lane loads 1/16 of the head of each of its 8 values, 16 lanes
+//     whole rows, and interleaves them two keys at a time (v_perm_b32) into
+//     rows of V^T.
+//   * The probabilities enter as two 16-bit parts each (split2): the second
+//     product is as exact as binary32 scores are, for a doubled product that
+//     the memory time covers.
+//   * While a tile is computed the next one's 16 KiB are in flight, in
+//     registers; table entries are read a tile further ahead.
+//   * Work is cut by the keys there are, on the device: the tiles of all
+//     sequences are counted, and a sequence gets as many workgroups as its
+//     share of kDecodeSlots asks for, so uneven batches and tables wider than
+//     the lengths cost nothing.  A sequence of more than one workgroup leaves
+//     (O, r, l) per workgroup in the workspace, which join_kernel adds up.
+#include <algorithm>
+
+#include "attention_common.h"
+
+namespace w8a8 {
+
+namespace {
+
+constexpr int kTile = 32;            // keys of a wavefront's step
+constexpr int kWaves = 4;            // wavefronts of a workgroup
+constexpr int kMinTiles = 4;         // least tiles of a workgroup of several
+constexpr int kDecodeSlots = 1024;   // workgroups aimed at
+constexpr int kJoinWaves = 8;
+constexpr float kBelowMax = 7.0f;    // the reference below the maximum it was set from
+constexpr float kSlack = 15.0f;      // scores above the reference that raise it
+
+struct DecodeParams {
+  PagedAttention a;
+  int units;       // workgroups of one piece of a sequence: kv_heads x blocks of 16 queries
+  int blocks;      // blocks of 16 queries per key head
+  int group;       // queries per key head
+  int rows;        // query rows of a workgroup: min(group, 16)
+  float* part_o;   // [pieces x units, rows, head_dim]
+  f32x2* part_rl;  // [pieces x units, rows]
+};
+
+// Pieces that all sequences are cut into at most: each gets one, and the cut
+// itself adds at most slots / units.
+inline int64_t max_pieces(int64_t batch, int64_t units, int64_t max_keys) {
+  const int64_t whole = ceil_div(ceil_div(max_keys, kTile), kMinTiles);
+  const int64_t cut = batch + kDecodeSlots / units;
+  return whole <= 1 ? batch : std::min(cut, batch * whole);
+}
+
+struct Piece {
+  int seq;     // the sequence, or -1
+  int first;   // its first piece
+  int count;   // its pieces
+  int tiles;   // its tiles
+  int keys;    // its keys
+};
+
+// The sequence of piece `slot`, or the pieces of sequence `seq` (slot < 0).
+// Every lane of the wavefront takes part and gets the same answer.
+__device__ inline Piece find_piece(const DecodeParams& p, int slot, int seq) {
+  const int lane = threadIdx.x & 63;
+  const int batch = p.a.batch;
+  auto keys_of = [&](int b) { return b < batch ? max(0, min(p.a.lengths[b], p.a.max_keys)) : 0; };
+  auto sum = [](int64_t v) {
+#pragma unroll
+    for (int w = 1; w < 64; w <<= 1) v += __shfl_xor(v, w);
+    return v;
+  };
+  int keys = keys_of(lane);
+  int64_t total = (keys + kTile - 1) / kTile;
+  for (int b = lane + 64; b < batch; b += 64) total += (keys_of(b) + kTile - 1) / kTile;
+  total = sum(total) * p.units;
+  const int64_t share = min((total + kDecodeSlots - 1) / kDecodeSlots, int64_t{INT32_MAX / 2});
+  const int cut = max(kMinTiles, static_cast<int>(share));
+  int before = 0;
+  for (int b0 = 0; b0 < batch; b0 += 64) {
+    if (b0 > 0) keys = keys_of(b0 + lane);
+    const int tiles = (keys + kTile - 1) / kTile;
+    const int count = b0 + lane < batch ? max(1, (tiles + cut - 1) / cut) : 0;
+    int upto = count;
+#pragma unroll
+    for (int w = 1; w < 64; w <<= 1) {
+      const int v = __shfl_up(upto, w);
+      if (lane >= w) upto += v;
+    }
+    const bool mine = slot >= 0 ? before + upto > slot : b0 + lane == seq;
+    const uint64_t found = __ballot(mine);
+    if (found != 0) {
+      const int at = __ffsll(static_cast<unsigned long long>(found)) - 1;
+      const int n = __shfl(count, at);
+      return Piece{b0 + at, before + __shfl(upto, at) - n, n, __shfl(tiles, at), __shfl(keys, at)};
+    }
+    before += __shfl(upto, 63);
+  }
+  return Piece{-1, 0, 0, 0, 0};
+}
+
+// The result rows of one workgroup's queries: normalised to the output, or
+// (O, r, l) to the workspace.
+template <typename T>
+__device__ inline void write_out(const DecodeParams& p, int seq, int head, int d, float o,
+                                 float l) {
+  const float y = o * (l == 0.0f ? 0.0f : 1.0f / l);
+  static_cast<T*>(p.a.out)[seq * p.a.o_st + head * p.a.o_sh + d] = from_f32<T>(y);
+}
+
+// DP: head_dim rounded up to 64, 128 or 256; FULL: head_dim == DP.  SMALL:
+// pages of fewer than 4 keys, so that each key has a table entry of its own.
+template <typename T, int DP, bool FULL, bool SMALL>
+__global__ __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) void decode_kernel(DecodeParams p) {
+  constexpr int KS = DP / 32;   // first product: steps over the head
+  constexpr int DV = DP / 16;   // elements of a value row per lane
+  constexpr int VW = DV / 2;    // ... dwords
+  constexpr int NV = SMALL ? 8 : 2;  // table entries of a lane's 8 values
+  __shared__ float red_o[kWaves][16][DP];
+  __shared__ float red_r[kWaves][16], red_l[kWaves][16];
+
+  const PagedAttention& a = p.a;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, g = lane >> 4;
+  const int slot = blockIdx.x / p.units, unit = blockIdx.x % p.units;
+  const Piece piece = find_piece(p, slot, -1);
+  const int seq = __builtin_amdgcn_readfirstlane(piece.seq);
+  if (seq < 0) return;
+  const int count = __builtin_amdgcn_readfirstlane(piece.count);
+  const int part = slot - __builtin_amdgcn_readfirstlane(piece.first);
+  const int tiles = __builtin_amdgcn_readfirstlane(piece.tiles);
+  const int keys = __builtin_amdgcn_readfirstlane(piece.keys);
+  const int t0 = static_cast<int>(static_cast<int64_t>(tiles) * part / count);
+  const int t1 = static_cast<int>(static_cast<int64_t>(tiles) * (part + 1) / count);
+  const int kvh = unit / p.blocks;
+  const int head0 = kvh * p.group + (unit % p.blocks) * 16;
+  const int rows = min(16, (kvh + 1) * p.group - head0);
+  const int D = a.head_dim;
+
+  u32x4 qf[KS];
+  bool live[KS];   // whether the head has elements 32 s + 8 g
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    live[s] = FULL || 32 * s + 8 * g < D;
+    qf[s] = u32x4{0, 0, 0, 0};
+    if (live[s] && r < rows)
+      qf[s] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + seq * a.q_st +
+                                              (head0 + r) * a.q_sh + 32 * s + 8 * g);
+  }
+  const int vd = FULL || r * DV < D ? r * DV : 0;   // rows past the head are not written
+  const int32_t* table = a.table + seq * a.ld_table;
+  const uint16_t* kb = static_cast<const uint16_t*>(a.k) + kvh * a.c_head + 8 * g;
+  const uint16_t* vb = static_cast<const uint16_t*>(a.v) + kvh * a.c_head + vd;
+  const int page_mask = (1 << a.page_shift) - 1;
+  const int pages = static_cast<int>(a.pages);
+
+  struct Entries {
+    int k[2];    // of keys 16 t + r
+    int v[NV];   // of keys 4 g and 16 + 4 g (SMALL: 4 g + i, then 16 + 4 g + i)
+  };
+  struct Tile {
+    u32x4 k[2][KS];
+    uint32_t v[8][VW];
+    uint32_t ok;   // bit i: the lane's key i is there
+  };
+  auto entry = [&](int j) {
+    int e = -1;
+    if (j < keys) e = table[j >> a.page_shift];
+    return e;
+  };
+  auto lookup = [&](int t, Entries& e) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) e.k[h] = entry(t * kTile + 16 * h + r);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      e.v[i] = SMALL ? entry(t * kTile + (i < 4 ? 0 : 16) + 4 * g + (i & 3))
+                     : entry(t * kTile + 16 * i + 4 * g);
+  };
+  // A key that is not there reads row 0 of page 0 instead.
+  auto row_of = [&](int e, int j) {
+    return e >= 0 && e < pages ? e * a.c_page + (j & page_mask) * a.c_tok : int64_t{0};
+  };
+  auto issue = [&](int t, const Entries& e, Tile& x) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint16_t* src = kb + row_of(e.k[h], t * kTile + 16 * h + r);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        if constexpr (FULL) {
+          x.k[h][s] = *reinterpret_cast<const u32x4*>(src + 32 * s);
+        } else {
+          x.k[h][s] = u32x4{0, 0, 0, 0};
+          if (live[s]) x.k[h][s] = *reinterpret_cast<const u32x4*>(src + 32 * s);
+        }
+      }
+    }
+    x.ok = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int j = t * kTile + (i < 4 ? 0 : 16) + 4 * g + (i & 3);
+      const int ev = e.v[SMALL ? i : i >> 2];
+      const bool there = j < keys && ev >= 0 && ev < pages;
+      x.ok |= static_cast<uint32_t>(there) << i;
+      const uint16_t* src = vb + row_of(there ? ev : -1, j);
+      if constexpr (VW == 2) {
+        const u32x2 w = *reinterpret_cast<const u32x2*>(src);
+        x.v[i][0] = w[0];
+        x.v[i][1] = w[1];
+      } else {
+#pragma unroll
+        for (int c = 0; c < VW; c += 4) {
+          // head_dim is a multiple of 8: a lane's second half may lie past it.
+          const int more = FULL || c == 0 || vd + 2 * c < D ? 2 * c : 0;
+          const u32x4 w = *reinterpret_cast<const u32x4*>(src + more);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) x.v[i][c + k] = w[k];
+        }
+      }
+    }
+  };
+
+  f32x4 o[DV];
+#pragma unroll
+  for (int i = 0; i < DV; ++i) o[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  float ref = -INFINITY, l = 0.0f;
+  const float sc = a.scale * kLog2e;
+
+  auto compute = [&](Tile& x) {
+    f32x4 s0{0.0f, 0.0f, 0.0f, 0.0f}, s1 = s0;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      s0 = mfma_16x16x32<T>(x.k[0][s], qf[s], s0);
+      s1 = mfma_16x16x32<T>(x.k[1][s], qf[s], s1);
+    }
+    float w[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = s0[i] * sc;
+      w[4 + i] = s1[i] * sc;
+    }
+    if (!__all(x.ok == 0xffu)) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool there = (x.ok >> i) & 1;
+        w[i] = there ? w[i] : -INFINITY;
+#pragma unroll
+        for (int c = 0; c < VW; ++c) x.v[i][c] = there ? x.v[i][c] : 0u;
+      }
+    }
+    float top = w[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) top = fmaxf(top, w[i]);
+    if (__any(top > ref + kSlack)) {
+      // Raise the reference of the columns that need it; all four lanes of a
+      // column agree.
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      if (top > ref + kSlack) {
+        const float next = top - kBelowMax;
+        const float f = ref == -INFINITY ? 1.0f : exp2_hw(ref - next);
+        ref = next;
+        l *= f;
+#pragma unroll
+        for (int i = 0; i < DV; ++i) o[i] *= f;
+      }
+    }
+    // Without a score above -inf so far the reference is 0: -inf gives 0, NaN
+    // stays.
+    const float base = ref == -INFINITY ? 0.0f : ref;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = exp2_hw(w[i] - base);
+    l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+    u32x4 hi, lo;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t h, m;
+      split2<T>(w[2 * i], w[2 * i + 1], h, m);
+      hi[i] = h;
+      lo[i] = m;
+    }
+#pragma unroll
+    for (int i = 0; i < DV; ++i) {
+      u32x4 vt;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        vt[k] = __builtin_amdgcn_perm(x.v[2 * k + 1][i >> 1], x.v[2 * k][i >> 1],
+                                      (i & 1) ? 0x07060302u : 0x05040100u);
+      o[i] = mfma_16x16x32<T>(vt, hi, o[i]);
+      o[i] = mfma_16x16x32<T>(vt, lo, o[i]);
+    }
+  };
+
+  {
+    int t = t0 + wave;
+    Entries e;
+    Tile x0, x1;
+    if (t < t1) {
+      lookup(t, e);
+      issue(t, e, x0);
+      lookup(min(t + kWaves, t1 - 1), e);
+    }
+    while (t < t1) {
+      const int tn = t + kWaves;
+      if (tn < t1) {
+        issue(tn, e, x1);
+        lookup(min(tn + kWaves, t1 - 1), e);
+      }
+      compute(x0);
+      if (tn >= t1) break;
+      const int tm = tn + kWaves;
+      if (tm < t1) {
+        issue(tm, e, x0);
+        lookup(min(tm + kWaves, t1 - 1), e);
+      }
+      compute(x1);
+      t = tm;
+    }
+  }
+
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  if (r < rows) {
+    if (g == 0) {
+      red_r[wave][r] = ref;
+      red_l[wave][r] = l;
+    }
+    // o[i][k]: element DV (4 g + k) + i of the head.
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int i = 0; i < DV; ++i) red_o[wave][r][DV * (4 * g + k) + i] = o[i][k];
+  }
+  __syncthreads();
+  const int64_t item = blockIdx.x;
+  for (int n = threadIdx.x; n < rows * DP; n += 64 * kWaves) {
+    const int q = n / DP, d = n % DP;
+    if (!FULL && d >= D) continue;
+    float top = red_r[0][q];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) top = fmaxf(top, red_r[w][q]);
+    const float base = top == -INFINITY ? 0.0f : top;
+    float ov = 0.0f, lv = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float f = exp2_hw(red_r[w][q] - base);
+      ov += red_o[w][q][d] * f;
+      lv += red_l[w][q] * f;
+    }
+    if (count == 1) {
+      write_out<T>(p, seq, head0 + q, d, ov, lv);
+    } else {
+      p.part_o[(item * p.rows + q) * D + d] = ov;
+      if (d == 0) p.part_rl[item * p.rows + q] = f32x2{top, lv};
+    }
+  }
+}
+
+// One workgroup per query row: adds up what the pieces of its sequence left.
+template <typename T, int DP>
+__global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(DecodeParams p) {
+  constexpr int N = DP / 64;
+  __shared__ float red_o[kJoinWaves][DP];
+  __shared__ float red_r[kJoinWaves], red_l[kJoinWaves];
+  const int seq = blockIdx.x, head = blockIdx.y;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int D = p.a.head_dim;
+  const Piece piece = find_piece(p, -1, seq);
+  if (piece.count <= 1) return;
+  const int kvh = head / p.group, q = head % p.group;
+  const int unit = kvh * p.blocks + q / 16;
+  float ref = -INFINITY, l = 0.0f, o[N] = {};
+  for (int c = wave; c < piece.count; c += kJoinWaves) {
+    const int64_t at = (static_cast<int64_t>(piece.first + c) * p.units + unit) * p.rows + q % 16;
+    const f32x2 rl = p.part_rl[at];
+    const float next = fmaxf(ref, rl[0]);
+    const float base = next == -INFINITY ? 0.0f : next;
+    const float f0 = exp2_hw(ref - base), f1 = exp2_hw(rl[0] - base);
+    ref = next;
+    l = l * f0 + rl[1] * f1;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int d = lane + 64 * i;
+      const float v = d < D ? p.part_o[at * D + d] : 0.0f;
+      o[i] = o[i] * f0 + v * f1;
+    }
+  }
+  if (lane == 0) {
+    red_r[wave] = ref;
+    red_l[wave] = l;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) red_o[wave][lane + 64 * i] = o[i];
+  __syncthreads();
+  for (int d = threadIdx.x; d < D; d += 64 * kJoinWaves) {
+    float top = red_r[0];
+#pragma unroll
+    for (int w = 1; w < kJoinWaves; ++w) top = fmaxf(top, red_r[w]);
+    const float base = top == -INFINITY ? 0.0f : top;
+    float ov = 0.0f, lv = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kJoinWaves; ++w) {
+      const float f = exp2_hw(red_r[w] - base);
+      ov += red_o[w][d] * f;
+      lv += red_l[w] * f;
+    }
+    write_out<T>(p, seq, head, d, ov, lv);
+  }
+}
+
+template <typename T, int DP, bool FULL>
+hipError_t launch_d(const DecodeParams& p, int64_t pieces, hipStream_t st) {
+  const dim3 grid(static_cast<uint32_t>(pieces * p.units)), block(64 * kWaves);
+  if (p.a.page_shift < 2)
+    hipLaunchKernelGGL((decode_kernel<T, DP, FULL, true>), grid, block, 0, st, p);
+  else
+    hipLaunchKernelGGL((decode_kernel<T, DP, FULL, false>), grid, block, 0, st, p);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || pieces == p.a.batch) return e;
+  hipLaunchKernelGGL((join_kernel<T, DP>), dim3(p.a.batch, p.a.q_heads), dim3(64 * kJoinWaves), 0,
+                     st, p);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_t(const DecodeParams& p, int64_t pieces, hipStream_t st) {
+  const int d = p.a.head_dim;
+  if (d == 64) return launch_d<T, 64, true>(p, pieces, st);
+  if (d < 64) return launch_d<T, 64, false>(p, pieces, st);
+  if (d == 128) return launch_d<T, 128, true>(p, pieces, st);
+  if (d < 128) return launch_d<T, 128, false>(p, pieces, st);
+  if (d == 256) return launch_d<T, 256, true>(p, pieces, st);
+  return launch_d<T, 256, false>(p, pieces, st);
+}
+
+int64_t units_of(int64_t q_heads, int64_t kv_heads) {
+  return kv_heads * ceil_div(q_heads / kv_heads, 16);
+}
+
+// Bytes of the (r, l) pairs in front of the O rows.
+int64_t pairs_bytes(int64_t items, int64_t rows) { return ceil_div(items * rows * 8, 256) * 256; }
+
+}  // namespace
+
+int64_t paged_decode_workspace(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                               int64_t max_keys) {
+  const int64_t units = units_of(q_heads, kv_heads);
+  const int64_t pieces = max_pieces(batch, units, max_keys);
+  if (pieces <= batch) return 0;
+  const int64_t rows = std::min<int64_t>(q_heads / kv_heads, 16), items = pieces * units;
+  return pairs_bytes(items, rows) + items * rows * head_dim * 4;
+}
+
+hipError_t launch_paged_decode(const PagedAttention& a, int dtype, hipStream_t st) {
+  DecodeParams p;
+  p.a = a;
+  p.group = a.q_heads / a.kv_heads;
+  p.blocks = static_cast<int>(ceil_div(p.group, 16));
+  p.units = a.kv_heads * p.blocks;
+  p.rows = std::min(p.group, 16);
+  const int64_t pieces = max_pieces(a.batch, p.units, a.max_keys);
+  if (pieces * p.units > INT32_MAX) return hipErrorInvalidConfiguration;
+  char* ws = static_cast<char*>(a.workspace);
+  p.part_rl = reinterpret_cast<f32x2*>(ws);
+  p.part_o = reinterpret_cast<float*>(ws + pairs_bytes(pieces * p.units, p.rows));
+  return dtype == kF16 ? launch_t<__half>(p, pieces, st) : launch_t<__hip_bfloat16>(p, pieces, st);
+}
+
+}  // namespace w8a8

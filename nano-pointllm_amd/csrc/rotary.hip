@@ -17,6 +17,8 @@
 // one 16-byte chunk, or the two chunks of a half pair), so cos and sin are
 // formed once per workgroup by R/2 threads, in LDS, while the row loads are in
 // flight.
+#include <algorithm>
+
 #include "w8a8_internal.h"
 
 namespace w8a8 {
@@ -208,14 +210,14 @@ template <typename T>
 hipError_t launch_t(const RotaryRows& r, hipStream_t st) {
   // The widest chunk that every address and the rotated part divide into.
   int w = r.half ? width_of(r.rotary_dim / 2) : width_of(r.rotary_dim);
-  for (const int64_t v : {r.q_st, r.q_sh, r.qo_st, r.qo_sh}) w = min(w, width_of(v));
-  w = min(w, min(width_of(r.q), width_of(r.q_out)));
+  for (const int64_t v : {r.q_st, r.q_sh, r.qo_st, r.qo_sh}) w = std::min(w, width_of(v));
+  w = std::min(w, std::min(width_of(r.q), width_of(r.q_out)));
   if (r.k != nullptr) {
     for (const int64_t v : {r.k_st, r.k_sh, r.v_st, r.v_sh, r.c_page, r.c_head, r.c_tok})
-      w = min(w, width_of(v));
+      w = std::min(w, width_of(v));
     for (const void* v : {r.k, r.v, static_cast<const void*>(r.k_cache),
                           static_cast<const void*>(r.v_cache)})
-      w = min(w, width_of(v));
+      w = std::min(w, width_of(v));
   }
   if (r.half) {
     if (w == 8) return launch_w<T, true, 8>(r, st);
