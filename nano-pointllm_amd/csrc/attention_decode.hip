@@ -34,6 +34,7 @@
 //     the lengths cost nothing.  A sequence of more than one workgroup leaves
 //     (O, r, l) per workgroup in the workspace, which join_kernel adds up.
 #include <algorithm>
+#include <type_traits>
 
 #include "attention_common.h"
 
@@ -44,8 +45,9 @@ namespace {
 constexpr int kTile = 32;            // keys of a wavefront's step
 constexpr int kWaves = 4;            // wavefronts of a workgroup
 constexpr int kMinTiles = 4;         // least tiles of a workgroup of several
-constexpr int kDecodeSlots = 1024;   // workgroups aimed at
-constexpr int kJoinWaves = 8;
+constexpr int kDecodeSlots = 768;    // workgroups aimed at
+constexpr int kJoinThreads = 256;
+constexpr int kJoinAhead = 4;        // rows a thread loads before the weights are known
 constexpr float kBelowMax = 7.0f;    // the reference below the maximum it was set from
 constexpr float kSlack = 15.0f;      // scores above the reference that raise it
 
@@ -75,48 +77,61 @@ struct Piece {
   int keys;    // its keys
 };
 
+// Inclusive sum over the wavefront's lanes (each step a DPP move: shifts by 1,
+// 2, 4 and 8 in rows of 16 lanes, then the rows' last lanes to the next ones).
+__device__ inline uint32_t scan64(uint32_t v) {
+  auto moved = [](uint32_t x, auto ctrl, auto rows) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(
+        0, static_cast<int>(x), decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
+  };
+  using std::integral_constant;
+  const integral_constant<int, 0xf> all;
+  v += moved(v, integral_constant<int, 0x111>{}, all);
+  v += moved(v, integral_constant<int, 0x112>{}, all);
+  v += moved(v, integral_constant<int, 0x114>{}, all);
+  v += moved(v, integral_constant<int, 0x118>{}, all);
+  v += moved(v, integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});
+  v += moved(v, integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});
+  return v;
+}
+__device__ inline int lane_value(uint32_t v, int lane) {
+  return __builtin_amdgcn_readlane(static_cast<int>(v), lane);
+}
+
 // The sequence of piece `slot`, or the pieces of sequence `seq` (slot < 0).
-// Every lane of the wavefront takes part and gets the same answer.
+// Every lane of the wavefront takes part and gets the same answer, in scalar
+// registers.  A lane's tiles stay below 2^26, so 64 of them fit 32 bits.
 __device__ inline Piece find_piece(const DecodeParams& p, int slot, int seq) {
   const int lane = threadIdx.x & 63;
   const int batch = p.a.batch;
   auto keys_of = [&](int b) { return b < batch ? max(0, min(p.a.lengths[b], p.a.max_keys)) : 0; };
-  auto sum = [](int64_t v) {
-#pragma unroll
-    for (int w = 1; w < 64; w <<= 1) v += __shfl_xor(v, w);
-    return v;
-  };
-  int keys = keys_of(lane);
-  int64_t total = (keys + kTile - 1) / kTile;
-  for (int b = lane + 64; b < batch; b += 64) total += (keys_of(b) + kTile - 1) / kTile;
-  total = sum(total) * p.units;
+  auto tiles_of = [](int keys) { return static_cast<uint32_t>(keys + kTile - 1) / kTile; };
+  const int keys0 = keys_of(lane);
+  int64_t total = static_cast<uint32_t>(lane_value(scan64(tiles_of(keys0)), 63));
+  for (int b0 = 64; b0 < batch; b0 += 64)
+    total += static_cast<uint32_t>(lane_value(scan64(tiles_of(keys_of(b0 + lane))), 63));
+  total *= p.units;
   const int64_t share = min((total + kDecodeSlots - 1) / kDecodeSlots, int64_t{INT32_MAX / 2});
-  const int cut = max(kMinTiles, static_cast<int>(share));
+  const uint32_t cut = max(static_cast<uint32_t>(kMinTiles), static_cast<uint32_t>(share));
   int before = 0;
   for (int b0 = 0; b0 < batch; b0 += 64) {
-    if (b0 > 0) keys = keys_of(b0 + lane);
-    const int tiles = (keys + kTile - 1) / kTile;
-    const int count = b0 + lane < batch ? max(1, (tiles + cut - 1) / cut) : 0;
-    int upto = count;
-#pragma unroll
-    for (int w = 1; w < 64; w <<= 1) {
-      const int v = __shfl_up(upto, w);
-      if (lane >= w) upto += v;
-    }
-    const bool mine = slot >= 0 ? before + upto > slot : b0 + lane == seq;
+    const int keys = b0 == 0 ? keys0 : keys_of(b0 + lane);
+    const uint32_t tiles = tiles_of(keys);
+    const uint32_t count = b0 + lane < batch ? max(1u, (tiles + cut - 1) / cut) : 0u;
+    const uint32_t upto = scan64(count);
+    const bool mine = slot >= 0 ? before + static_cast<int>(upto) > slot : b0 + lane == seq;
     const uint64_t found = __ballot(mine);
     if (found != 0) {
       const int at = __ffsll(static_cast<unsigned long long>(found)) - 1;
-      const int n = __shfl(count, at);
-      return Piece{b0 + at, before + __shfl(upto, at) - n, n, __shfl(tiles, at), __shfl(keys, at)};
+      const int n = lane_value(count, at);
+      return Piece{b0 + at, before + lane_value(upto, at) - n, n, lane_value(tiles, at),
+                   lane_value(static_cast<uint32_t>(keys), at)};
     }
-    before += __shfl(upto, 63);
+    before += lane_value(upto, 63);
   }
   return Piece{-1, 0, 0, 0, 0};
 }
 
-// The result rows of one workgroup's queries: normalised to the output, or
-// (O, r, l) to the workspace.
 template <typename T>
 __device__ inline void write_out(const DecodeParams& p, int seq, int head, int d, float o,
                                  float l) {
@@ -141,12 +156,9 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) void decode_kernel(
   const int r = lane & 15, g = lane >> 4;
   const int slot = blockIdx.x / p.units, unit = blockIdx.x % p.units;
   const Piece piece = find_piece(p, slot, -1);
-  const int seq = __builtin_amdgcn_readfirstlane(piece.seq);
+  const int seq = piece.seq, count = piece.count, tiles = piece.tiles, keys = piece.keys;
   if (seq < 0) return;
-  const int count = __builtin_amdgcn_readfirstlane(piece.count);
-  const int part = slot - __builtin_amdgcn_readfirstlane(piece.first);
-  const int tiles = __builtin_amdgcn_readfirstlane(piece.tiles);
-  const int keys = __builtin_amdgcn_readfirstlane(piece.keys);
+  const int part = slot - piece.first;
   const int t0 = static_cast<int>(static_cast<int64_t>(tiles) * part / count);
   const int t1 = static_cast<int>(static_cast<int64_t>(tiles) * (part + 1) / count);
   const int kvh = unit / p.blocks;
@@ -373,54 +385,75 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) void decode_kernel(
 }
 
 // One workgroup per query row: adds up what the pieces of its sequence left.
+// A thread takes four elements of every eighth (D = 128) piece, the first
+// kJoinAhead of them in flight while the weights are formed.
 template <typename T, int DP>
-__global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(DecodeParams p) {
-  constexpr int N = DP / 64;
-  __shared__ float red_o[kJoinWaves][DP];
-  __shared__ float red_r[kJoinWaves], red_l[kJoinWaves];
-  const int seq = blockIdx.x, head = blockIdx.y;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+__global__ __launch_bounds__(kJoinThreads) void join_kernel(DecodeParams p) {
+  constexpr int C = DP / 4;              // threads of a row
+  constexpr int R = kJoinThreads / C;    // rows at a time
+  constexpr int W = kJoinThreads / 64;
+  __shared__ float weight[kDecodeSlots + 1];   // one sequence's pieces at most
+  __shared__ f32x4 red_o[R][C];
+  __shared__ float red[2][W];
+  const int seq = blockIdx.x, head = blockIdx.y, tid = threadIdx.x;
   const int D = p.a.head_dim;
   const Piece piece = find_piece(p, -1, seq);
-  if (piece.count <= 1) return;
-  const int kvh = head / p.group, q = head % p.group;
-  const int unit = kvh * p.blocks + q / 16;
-  float ref = -INFINITY, l = 0.0f, o[N] = {};
-  for (int c = wave; c < piece.count; c += kJoinWaves) {
-    const int64_t at = (static_cast<int64_t>(piece.first + c) * p.units + unit) * p.rows + q % 16;
-    const f32x2 rl = p.part_rl[at];
-    const float next = fmaxf(ref, rl[0]);
-    const float base = next == -INFINITY ? 0.0f : next;
-    const float f0 = exp2_hw(ref - base), f1 = exp2_hw(rl[0] - base);
-    ref = next;
-    l = l * f0 + rl[1] * f1;
+  const int n = piece.count;
+  if (n <= 1) return;
+  const int q = head % p.group;
+  const int unit = head / p.group * p.blocks + q / 16;
+  const int64_t step = static_cast<int64_t>(p.units) * p.rows;
+  const int64_t at = (static_cast<int64_t>(piece.first) * p.units + unit) * p.rows + q % 16;
+  const int c = tid % C, row = tid / C;
+  const float* src = p.part_o + at * D + 4 * c;
+  f32x4 ahead[kJoinAhead];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int d = lane + 64 * i;
-      const float v = d < D ? p.part_o[at * D + d] : 0.0f;
-      o[i] = o[i] * f0 + v * f1;
-    }
+  for (int i = 0; i < kJoinAhead; ++i) {
+    ahead[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (row + i * R < n && 4 * c < D)
+      ahead[i] = *reinterpret_cast<const f32x4*>(src + (row + i * R) * step * D);
   }
-  if (lane == 0) {
-    red_r[wave] = ref;
-    red_l[wave] = l;
+  float top = -INFINITY;
+  for (int i = tid; i < n; i += kJoinThreads) {
+    weight[i] = p.part_rl[at + i * step][0];
+    top = fmaxf(top, weight[i]);
   }
 #pragma unroll
-  for (int i = 0; i < N; ++i) red_o[wave][lane + 64 * i] = o[i];
+  for (int w = 1; w < 64; w <<= 1) top = fmaxf(top, __shfl_xor(top, w));
+  if ((tid & 63) == 0) red[0][tid >> 6] = top;
   __syncthreads();
-  for (int d = threadIdx.x; d < D; d += 64 * kJoinWaves) {
-    float top = red_r[0];
+  top = red[0][0];
 #pragma unroll
-    for (int w = 1; w < kJoinWaves; ++w) top = fmaxf(top, red_r[w]);
-    const float base = top == -INFINITY ? 0.0f : top;
-    float ov = 0.0f, lv = 0.0f;
+  for (int w = 1; w < W; ++w) top = fmaxf(top, red[0][w]);
+  const float base = top == -INFINITY ? 0.0f : top;
+  float l = 0.0f;
+  for (int i = tid; i < n; i += kJoinThreads) {
+    weight[i] = exp2_hw(weight[i] - base);
+    l += weight[i] * p.part_rl[at + i * step][1];
+  }
 #pragma unroll
-    for (int w = 0; w < kJoinWaves; ++w) {
-      const float f = exp2_hw(red_r[w] - base);
-      ov += red_o[w][d] * f;
-      lv += red_l[w] * f;
-    }
-    write_out<T>(p, seq, head, d, ov, lv);
+  for (int w = 1; w < 64; w <<= 1) l += __shfl_xor(l, w);
+  if ((tid & 63) == 0) red[1][tid >> 6] = l;
+  __syncthreads();
+  f32x4 o{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < kJoinAhead; ++i)
+    if (row + i * R < n) o += ahead[i] * weight[row + i * R];
+  if (4 * c < D) {
+#pragma unroll 4
+    for (int i = row + kJoinAhead * R; i < n; i += R)
+      o += *reinterpret_cast<const f32x4*>(src + i * step * D) * weight[i];
+  }
+  red_o[row][c] = o;
+  __syncthreads();
+  if (row == 0 && 4 * c < D) {
+    l = red[1][0];
+#pragma unroll
+    for (int w = 1; w < W; ++w) l += red[1][w];
+#pragma unroll
+    for (int w = 1; w < R; ++w) o += red_o[w][c];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) write_out<T>(p, seq, head, 4 * c + i, o[i], l);
   }
 }
 
@@ -433,8 +466,8 @@ hipError_t launch_d(const DecodeParams& p, int64_t pieces, hipStream_t st) {
     hipLaunchKernelGGL((decode_kernel<T, DP, FULL, false>), grid, block, 0, st, p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || pieces == p.a.batch) return e;
-  hipLaunchKernelGGL((join_kernel<T, DP>), dim3(p.a.batch, p.a.q_heads), dim3(64 * kJoinWaves), 0,
-                     st, p);
+  hipLaunchKernelGGL((join_kernel<T, DP>), dim3(p.a.batch, p.a.q_heads), dim3(kJoinThreads), 0, st,
+                     p);
   return hipGetLastError();
 }
 
