@@ -31,6 +31,18 @@ __device__ inline f32x4 mfma_16x16x32(u32x4 a, u32x4 b, f32x4 c) {
 // normal value are 0).
 __device__ inline float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// The reference that scores are taken against (in powers of two) follows the
+// running maximum lazily: set kBelow below a maximum, raised once a score is
+// kSlack above it.  Binary16 probabilities: up to 2^15, so that one of 2^-31 of
+// the largest still counts, and the running sums are rarely rescaled; bfloat16
+// ones, whose range is binary32's: up to 1, so that no product with a value
+// near the type's largest overflows.
+template <typename T> struct Reference {
+  static constexpr bool kHalf = std::is_same<T, __half>::value;
+  static constexpr float kBelow = kHalf ? 7.0f : -8.0f;
+  static constexpr float kSlack = kHalf ? 15.0f : 0.0f;
+};
+
 // p0 and p1 as the sum of two 16-bit values each, packed: p = hi + lo to 22
 // bits (binary16) or 16 (bfloat16), both parts cut off, not rounded.
 template <typename T>
@@ -48,6 +60,27 @@ __device__ inline void split2(float p0, float p1, uint32_t& hi, uint32_t& lo) {
     const float r1 = p1 - __uint_as_float(u1 & 0xffff0000u);
     lo = __builtin_amdgcn_perm(__float_as_uint(r1), __float_as_uint(r0), 0x07060302u);
   }
+}
+
+// Inclusive sum over the wavefront's lanes (each step a DPP move: shifts by 1,
+// 2, 4 and 8 in rows of 16 lanes, then the rows' last lanes to the next ones).
+__device__ inline uint32_t scan64(uint32_t v) {
+  auto moved = [](uint32_t x, auto ctrl, auto rows) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(
+        0, static_cast<int>(x), decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
+  };
+  using std::integral_constant;
+  const integral_constant<int, 0xf> all;
+  v += moved(v, integral_constant<int, 0x111>{}, all);
+  v += moved(v, integral_constant<int, 0x112>{}, all);
+  v += moved(v, integral_constant<int, 0x114>{}, all);
+  v += moved(v, integral_constant<int, 0x118>{}, all);
+  v += moved(v, integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});
+  v += moved(v, integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});
+  return v;
+}
+__device__ inline int lane_value(uint32_t v, int lane) {
+  return __builtin_amdgcn_readlane(static_cast<int>(v), lane);
 }
 
 }  // namespace w8a8

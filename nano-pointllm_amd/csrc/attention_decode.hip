@@ -3,11 +3,8 @@
 //
 // Mathematics.  Per sequence and key head, with the queries q_0 .. q_{G-1}
 // that share the head as columns: S^T = K Q^T, P = 2^(S^T c - r) with c = scale
-// log2(e) and a running reference r per query, O^T = V^T P, l = sum P; the
-// result is O / l.  The reference follows the running maximum lazily: scores
-// may exceed the maximum it was set from by 2^8 before it is raised, and it
-// lies 7 below that maximum, so a probability is at most 2^15 and one of
-// 2^-31 of the largest still counts in binary16.
+// log2(e) and a running reference r per query (Reference in
+// attention_common.h), O^T = V^T P, l = sum P; the result is O / l.
 //
 // Bound by memory: every key and value is read once, 4 head_dim bytes per key
 // and key head against 4 head_dim G operations.
@@ -48,8 +45,6 @@ constexpr int kMinTiles = 4;         // least tiles of a workgroup of several
 constexpr int kDecodeSlots = 768;    // workgroups aimed at
 constexpr int kJoinThreads = 256;
 constexpr int kJoinAhead = 4;        // rows a thread loads before the weights are known
-constexpr float kBelowMax = 7.0f;    // the reference below the maximum it was set from
-constexpr float kSlack = 15.0f;      // scores above the reference that raise it
 
 struct DecodeParams {
   PagedAttention a;
@@ -76,27 +71,6 @@ struct Piece {
   int tiles;   // its tiles
   int keys;    // its keys
 };
-
-// Inclusive sum over the wavefront's lanes (each step a DPP move: shifts by 1,
-// 2, 4 and 8 in rows of 16 lanes, then the rows' last lanes to the next ones).
-__device__ inline uint32_t scan64(uint32_t v) {
-  auto moved = [](uint32_t x, auto ctrl, auto rows) {
-    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(
-        0, static_cast<int>(x), decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
-  };
-  using std::integral_constant;
-  const integral_constant<int, 0xf> all;
-  v += moved(v, integral_constant<int, 0x111>{}, all);
-  v += moved(v, integral_constant<int, 0x112>{}, all);
-  v += moved(v, integral_constant<int, 0x114>{}, all);
-  v += moved(v, integral_constant<int, 0x118>{}, all);
-  v += moved(v, integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});
-  v += moved(v, integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});
-  return v;
-}
-__device__ inline int lane_value(uint32_t v, int lane) {
-  return __builtin_amdgcn_readlane(static_cast<int>(v), lane);
-}
 
 // The sequence of piece `slot`, or the pieces of sequence `seq` (slot < 0).
 // Every lane of the wavefront takes part and gets the same answer, in scalar
@@ -279,13 +253,13 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) void decode_kernel(
     float top = w[0];
 #pragma unroll
     for (int i = 1; i < 8; ++i) top = fmaxf(top, w[i]);
-    if (__any(top > ref + kSlack)) {
+    if (__any(top > ref + Reference<T>::kSlack)) {
       // Raise the reference of the columns that need it; all four lanes of a
       // column agree.
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
-      if (top > ref + kSlack) {
-        const float next = top - kBelowMax;
+      if (top > ref + Reference<T>::kSlack) {
+        const float next = top - Reference<T>::kBelow;
         const float f = ref == -INFINITY ? 1.0f : exp2_hw(ref - next);
         ref = next;
         l *= f;

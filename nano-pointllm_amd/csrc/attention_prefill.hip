@@ -1,0 +1,661 @@
+// Causal attention of prompts and prompt chunks over a paged key-value cache
+// (gfx950).
+//
+// Mathematics.  Rows (token, query head of one key head) are the columns of
+// S^T = K Q^T; P = 2^(S^T c - r) with c = scale log2(e) and a running reference
+// r per row (Reference in attention_common.h), rounded to 16 bits; O^T = V^T P
+// and l = sum P over the rounded values; the result is O / l.
+//
+// Bound by the matrix units and the exponentials together: per 64 keys and 32
+// rows of 128 elements a wavefront issues 32 matrix instructions of 32 cycles
+// and about as many cycles of vector work.
+//
+// Design:
+//   * A workgroup takes 128 rows of one key head, 32 per wavefront, held in
+//     registers; the queries that share a key head are packed as rows, so a
+//     short chunk fills its tiles and every key is read once per 128 rows.
+//   * Keys and values pass through a double-buffered LDS tile of 64 keys,
+//     filled by LDS-DMA buffer loads straight from the pages: one descriptor
+//     per load, whose range ends at the sequence's last key, so what lies
+//     behind it arrives as zeros.  16-byte chunks are permuted by key (in the
+//     source address), which leaves the reads of both operands without bank
+//     conflicts.
+//   * The score tile's registers are the second product's operand as they
+//     are: its inner index is summed over, so the values are read (transposing
+//     ds_read_b64_tr_b16) in the key order that the scores have.
+//   * Masks are formed for the tiles that a row of the wavefront sees in part,
+//     the last ones; the others have none.
+//   * Few rows far into a long cache are cut over its length: each piece
+//     leaves (O, r, l) in the workspace and join_kernel adds them up.
+//   * A masked key's probability is 0, but 0 times an infinite or NaN value is
+//     NaN.  Such values are not searched for: a row whose sums are not finite
+//     is computed again by careful_rows, key by key.
+#include <algorithm>
+#include <type_traits>
+
+#include "attention_common.h"
+
+namespace w8a8 {
+
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef const int32_t __attribute__((address_space(4))) const_i32;   // scalar loads
+
+constexpr int kKeys = 64;            // keys of a tile
+constexpr int kWaves = 4;
+constexpr int kRows = 32 * kWaves;   // rows of a workgroup
+constexpr int kSlots = 512;          // workgroups below which the keys are cut
+constexpr int kMinTiles = 4;         // least tiles of a piece
+constexpr int kMaxCut = 32;
+constexpr int kOutside = 0x7ffffff0;   // a buffer offset past every range
+constexpr int kBufferWord3 = 0x00020000;
+constexpr int kJoinThreads = 256;
+
+struct PrefillParams {
+  PagedAttention a;
+  int group;           // query heads per key head
+  int cut;             // most pieces of a row tile
+  float* part_o;       // [row tiles x kv_heads x cut, kRows, head_dim]
+  f32x2* part_rl;      // [row tiles x kv_heads x cut, kRows]
+};
+
+// r / group for 0 <= r < 2^31, by a binary32 estimate that is put right.
+__device__ inline int divide_rows(int r, int group) {
+  if (group == 1) return r;
+  int q = static_cast<int>(static_cast<float>(r) / static_cast<float>(group));
+  int rest = r - q * group;
+  while (rest < 0) {
+    --q;
+    rest += group;
+  }
+  while (rest >= group) {
+    ++q;
+    rest -= group;
+  }
+  return q;
+}
+
+// One row tile: which rows of which sequence, and the keys that they see.
+struct Place {
+  int seq;      // or -1
+  int start;    // the sequence's first row of q
+  int count;    // its tokens
+  int row0;     // the tile's first row of count x group
+  int keys;     // the sequence's keys
+};
+
+__device__ inline Place find_tile(const PrefillParams& p, int tile) {
+  const int lane = threadIdx.x & 63;
+  const PagedAttention& a = p.a;
+  int before = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    const int b = b0 + lane;
+    int s0 = 0, n = 0;
+    if (b < a.batch) {
+      s0 = max(a.q_starts[b], 0);
+      n = max(min(a.q_starts[b + 1], a.tokens) - s0, 0);
+    }
+    const uint32_t tiles = (static_cast<uint32_t>(n) * p.group + kRows - 1) / kRows;
+    const uint32_t upto = scan64(tiles);
+    const uint64_t found = __ballot(before + static_cast<int>(upto) > tile);
+    if (found != 0) {
+      const int at = __ffsll(static_cast<unsigned long long>(found)) - 1;
+      const int first = before + lane_value(upto, at) - lane_value(tiles, at);
+      const int seq = b0 + at;
+      return Place{seq, lane_value(s0, at), lane_value(n, at), (tile - first) * kRows,
+                   max(0, min(a.lengths[seq], a.max_keys))};
+    }
+    before += lane_value(upto, 63);
+  }
+  return Place{-1, 0, 0, 0, 0};
+}
+
+// Key tiles that the rows of a tile see, and how many pieces they are cut into.
+__device__ inline int key_tiles(const PrefillParams& p, const Place& at) {
+  const int last = min(at.row0 + kRows, at.count * p.group) - 1;
+  const int seen = at.keys - at.count + divide_rows(last, p.group) + 1;
+  return (max(seen, 0) + kKeys - 1) / kKeys;
+}
+__device__ inline int pieces_of(const PrefillParams& p, int tiles) {
+  return max(1, min(p.cut, tiles / kMinTiles));
+}
+
+template <typename T>
+__device__ inline f32x16 mfma_32x32x16(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (std::is_same<T, __half>::value) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a),
+                                                  __builtin_bit_cast(h8, b), c, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a),
+                                                   __builtin_bit_cast(b8, b), c, 0, 0, 0);
+  }
+}
+
+// Two probabilities rounded to the 16-bit type, packed, and l plus the two
+// rounded values.
+template <typename T>
+__device__ inline uint32_t round2(float p0, float p1, float& l) {
+  if constexpr (std::is_same<T, __half>::value) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    const h2 v = __builtin_convertvector(f32x2{p0, p1}, h2);
+    l = __builtin_amdgcn_fdot2(v, h2{1, 1}, l, false);
+    return __builtin_bit_cast(uint32_t, v);
+  } else {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    const b2 v = __builtin_convertvector(f32x2{p0, p1}, b2);
+    l = __builtin_amdgcn_fdot2_f32_bf16(v, b2{1.0f, 1.0f}, l, false);
+    return __builtin_bit_cast(uint32_t, v);
+  }
+}
+
+// 16 bytes per lane from the buffer into LDS at lds + 16 * lane; zeros from
+// past its range.
+__device__ inline void dma16(__amdgpu_buffer_rsrc_t r, char* lds, int offset) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)lds, 16, offset, 0, 0, 0);
+}
+
+// The upper 32 lanes of x and the lower 32 of y change places.
+__device__ inline void swap_halves(uint32_t& x, uint32_t& y) {
+  const auto z = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+  x = z[0];
+  y = z[1];
+}
+
+// Each 16 lanes read 16 x 8 bytes, four rows of 16 elements (lane i: element
+// 4 (i % 4) of row i / 4), and lane i gets element i of the four rows.
+__device__ inline u32x2 read_transposed(const char* lds) {
+  return __builtin_bit_cast(u32x2,
+                            __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds)));
+}
+
+// Chunk permutations of a key's row of DP / 8 chunks of 16 bytes: position =
+// chunk ^ swizzle.  Keys: the 32 keys that a matrix operand reads at one chunk
+// spread over all banks.  Values: the four keys that a transposing read takes
+// at 64 bytes spread over all banks.
+template <int DP> __device__ inline int swizzle_k(int key) {
+  return DP == 64 ? (key >> 1) & 7 : key & 15;
+}
+template <int DP> __device__ inline int swizzle_v(int key) {
+  return DP == 64 ? ((key >> 1) & 1) << 2 | ((key >> 2) & 3) : (key & 3) << 2 | ((key >> 2) & 3);
+}
+
+// Where a row's result goes.
+template <typename T>
+__device__ inline T* out_row(const PagedAttention& a, int start, int token, int head) {
+  return static_cast<T*>(a.out) + (start + token) * a.o_st + head * a.o_sh;
+}
+
+// The rows of `bad` (bit c: row c of the wavefront's 32), key by key: lane i
+// holds elements i, i + 64, ... of the head.  Masked and unknown keys are not
+// read.
+template <typename T, int DP>
+__device__ inline void careful_rows(const PrefillParams& p, const Place& at, int kvh,
+                                          int wave_row, uint32_t bad, int k0, int k1,
+                                          int64_t item, bool whole) {
+  constexpr int N = DP / 64;
+  const PagedAttention& a = p.a;
+  const int lane = threadIdx.x & 63;
+  const int D = a.head_dim;
+  const float sc = a.scale * kLog2e;
+  const int32_t* table = a.table + at.seq * a.ld_table;
+  while (bad != 0) {
+    const int c = __ffs(bad) - 1;
+    bad &= bad - 1;
+    const int row = wave_row + c;
+    const int token = divide_rows(row, p.group);
+    const int head = kvh * p.group + row - token * p.group;
+    const T* q = static_cast<const T*>(a.q) + (at.start + token) * a.q_st + head * a.q_sh;
+    float qv[N], o[N] = {}, ref = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) qv[i] = lane + 64 * i < D ? to_f32(q[lane + 64 * i]) : 0.0f;
+    const int end = min(k1, at.keys - at.count + token + 1);
+    for (int j = k0; j < end; ++j) {
+      const int page = table[j >> a.page_shift];
+      if (page < 0 || page >= a.pages) continue;
+      const int64_t off = page * a.c_page + kvh * a.c_head +
+                          (j & ((1 << a.page_shift) - 1)) * a.c_tok;
+      float s = 0.0f, v[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int d = lane + 64 * i;
+        v[i] = d < D ? to_f32(static_cast<const T*>(a.v)[off + d]) : 0.0f;
+        if (d < D) s += qv[i] * to_f32(static_cast<const T*>(a.k)[off + d]);
+      }
+#pragma unroll
+      for (int w = 1; w < 64; w <<= 1) s += __shfl_xor(s, w);
+      s *= sc;
+      const float next = fmaxf(ref, s);
+      const float base = next == -INFINITY ? 0.0f : next;
+      const float f = exp2_hw(ref - base), w = exp2_hw(s - base);
+      ref = next;
+      l = l * f + w;
+#pragma unroll
+      for (int i = 0; i < N; ++i) o[i] = o[i] * f + w * v[i];
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int64_t r = item * kRows + row % kRows;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int d = lane + 64 * i;
+      if (d >= D) continue;
+      if (whole)
+        out_row<T>(a, at.start, token, head)[d] = from_f32<T>(o[i] * inv);
+      else
+        p.part_o[r * D + d] = o[i];
+    }
+    if (!whole && lane == 0) p.part_rl[r] = f32x2{ref, l};
+  }
+}
+
+// DP: head_dim rounded up to 64, 128 or 256.  DMA: the pages hold whole loads
+// of 1 KiB (512 / DP keys), else each chunk is copied through registers.
+template <typename T, int DP, bool DMA>
+__global__ __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) void prefill_kernel(PrefillParams p) {
+  constexpr int KS = DP / 16;                 // first product: steps over the head
+  constexpr int DT = DP / 32;                 // second product: row tiles of O^T
+  constexpr int RB = DP * 2;                  // bytes of a key's row
+  constexpr int RL = 1024 / RB;               // keys of a load
+  constexpr int NL = kKeys / RL / kWaves;     // loads per wavefront and operand
+  constexpr int TB = kKeys * RB;              // bytes of a tile
+  __shared__ __align__(16) char lds[4 * TB];  // K, V of one tile, then of the other
+  __shared__ int unknown[2][kWaves];          // loads of unknown pages, per wavefront
+
+  const PagedAttention& a = p.a;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 31, h = lane >> 5;
+  const int kvh = blockIdx.x % a.kv_heads;
+  // Later tiles, which see more keys, first.
+  const int tile = static_cast<int>(gridDim.x / a.kv_heads) - 1 - blockIdx.x / a.kv_heads;
+  const Place at = find_tile(p, tile);
+  if (at.seq < 0) return;
+  const int all_tiles = key_tiles(p, at);
+  const int pieces = pieces_of(p, all_tiles);
+  const int piece = blockIdx.y;
+  if (piece >= pieces) return;
+  const int t0 = all_tiles * piece / pieces, t1 = all_tiles * (piece + 1) / pieces;
+  const int D = a.head_dim;
+  const int total_rows = at.count * p.group;
+  const int wave_row = at.row0 + 32 * wave;
+  const int row = wave_row + c;
+  const bool live = row < total_rows;
+  const int token = divide_rows(min(row, total_rows - 1), p.group);
+  const int head = kvh * p.group + min(row, total_rows - 1) - token * p.group;
+  const int seen = live ? at.keys - at.count + token : -1;   // the row's last key
+  // The wavefront's least and greatest last key.
+  const int seen_first =
+      wave_row < total_rows ? at.keys - at.count + divide_rows(wave_row, p.group) : -1;
+  const int seen_last = wave_row < total_rows
+                            ? at.keys - at.count +
+                                  divide_rows(min(wave_row + 31, total_rows - 1), p.group)
+                            : -1;
+
+  // Queries, negated for a negative scale so that the scale below is not.
+  u32x4 qf[KS];
+  {
+    const uint16_t* q =
+        static_cast<const uint16_t*>(a.q) + (at.start + token) * a.q_st + head * a.q_sh + 8 * h;
+    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      qf[s] = u32x4{0, 0, 0, 0};
+      if (live && 16 * s + 8 * h < D) qf[s] = *reinterpret_cast<const u32x4*>(q + 16 * s);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) qf[s][i] ^= flip;
+    }
+  }
+  const float sc = fabsf(a.scale) * kLog2e;
+
+  // Loading: lane's key within a load and its chunk's position there.
+  const int lk = lane / (RB / 16), lp = lane % (RB / 16);
+  const_i32* table = (const_i32*)(a.table + at.seq * a.ld_table);
+  const int page_mask = (1 << a.page_shift) - 1;
+  const int ctok = static_cast<int>(a.c_tok);   // DMA: RL rows stay below 2^31 bytes
+  int off_k[NL], off_v[NL];
+#pragma unroll
+  for (int m = 0; m < NL; ++m) {
+    const int key = (wave * NL + m) * RL + lk;
+    const int ck = (lp ^ swizzle_k<DP>(key)) * 8, cv = (lp ^ swizzle_v<DP>(key)) * 8;
+    off_k[m] = ck < D ? (lk * ctok + ck) * 2 : kOutside;
+    off_v[m] = cv < D ? (lk * ctok + cv) * 2 : kOutside;
+  }
+  auto stage = [&](int t, auto buffer) __attribute__((always_inline)) {
+    constexpr int buf = decltype(buffer)::value;
+    char* dst = lds + buf * 2 * TB + wave * NL * 1024;
+    int bad = 0;
+    if constexpr (DMA) {
+#pragma unroll
+      for (int m = 0; m < NL; ++m) {
+        const int key = t * kKeys + (wave * NL + m) * RL;
+        int page = -1;
+        if (key < at.keys) page = table[key >> a.page_shift];
+        const bool known = page >= 0 && page < a.pages;
+        if (key < at.keys && !known) bad |= 1 << m;
+        const int64_t off =
+            known ? page * a.c_page + kvh * a.c_head + (key & page_mask) * a.c_tok : int64_t{0};
+        const int range = known ? min(RL, at.keys - key) * ctok * 2 : 0;
+        const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint16_t*>(static_cast<const uint16_t*>(a.k) + off), 0, range,
+            kBufferWord3);
+        const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint16_t*>(static_cast<const uint16_t*>(a.v) + off), 0, range,
+            kBufferWord3);
+        dma16(rk, dst + m * 1024, off_k[m]);
+        dma16(rv, dst + TB + m * 1024, off_v[m]);
+      }
+    } else {
+#pragma unroll
+      for (int m = 0; m < NL; ++m) {
+        const int in_tile = (wave * NL + m) * RL + lk;
+        const int key = t * kKeys + in_tile;
+        int page = -1;
+        if (key < at.keys) page = a.table[at.seq * a.ld_table + (key >> a.page_shift)];
+        const bool known = page >= 0 && page < a.pages;
+        if (__any(key < at.keys && !known)) bad = 1;
+        const int64_t off = page * a.c_page + kvh * a.c_head + (key & page_mask) * a.c_tok;
+        const int ck = (lp ^ swizzle_k<DP>(in_tile)) * 8, cv = (lp ^ swizzle_v<DP>(in_tile)) * 8;
+        u32x4 kv{0, 0, 0, 0}, vv{0, 0, 0, 0};
+        if (known && ck < D)
+          kv = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.k) + off + ck);
+        if (known && cv < D)
+          vv = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.v) + off + cv);
+        *reinterpret_cast<u32x4*>(dst + m * 1024 + lane * 16) = kv;
+        *reinterpret_cast<u32x4*>(dst + TB + m * 1024 + lane * 16) = vv;
+      }
+    }
+    if (lane == 0) unknown[buf][wave] = bad;
+  };
+
+  // Reading: byte offsets of the operands in a tile.
+  int read_k[KS], read_v[DT][2];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) read_k[s] = c * RB + (((2 * s + h) ^ swizzle_k<DP>(c)) * 16);
+  {
+    const int i = lane & 15, g = (lane >> 4) & 1;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int key = 8 * b + 4 * h + (i >> 2);
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+        read_v[d][b] = key * RB +
+                       (((4 * d + 2 * g + ((i & 3) >> 1)) ^ swizzle_v<DP>(key)) * 16) + 8 * (i & 1);
+    }
+  }
+
+  f32x16 o[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+  float ref = -INFINITY, l = 0.0f;
+
+  auto compute = [&](int t, auto buffer) __attribute__((always_inline)) {
+    constexpr int buf = decltype(buffer)::value;
+    const char* kt = lds + buf * 2 * TB;
+    const char* vt = kt + TB;
+    const int key0 = t * kKeys;
+    if (key0 > seen_last) return;   // no row of the wavefront sees it
+    f32x16 s[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+        s[b] = mfma_32x32x16<T>(
+            *reinterpret_cast<const u32x4*>(kt + b * 32 * RB + read_k[k]), qf[k], s[b]);
+    }
+    int bad = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) bad |= unknown[buf][w];
+    bad = __builtin_amdgcn_readfirstlane(bad);
+    const bool part = key0 + kKeys - 1 > seen_first || bad != 0;
+    uint32_t shown = 0xffffffffu;   // bit 16 b + i: s[b][i]'s key is seen
+    if (part) {
+      if (bad != 0) {
+#pragma unroll 1
+        for (int n = 0; n < 32; ++n) {
+          const int key = key0 + 32 * (n >> 4) + 8 * ((n >> 2) & 3) + 4 * h + (n & 3);
+          int page = 0;
+          if (key < at.keys) page = a.table[at.seq * a.ld_table + (key >> a.page_shift)];
+          if (page < 0 || page >= a.pages) shown &= ~(1u << n);
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const uint32_t bit = 1u << (16 * b + i);
+          if (key0 + 32 * b + 8 * (i >> 2) + 4 * h + (i & 3) > seen) shown &= ~bit;
+          s[b][i] = shown & bit ? s[b][i] : -INFINITY;
+        }
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
+    top *= sc;
+    if (__any(top > ref + Reference<T>::kSlack)) {
+      // Raise the reference of the rows that need it; both lanes of a row agree.
+      top = fmaxf(top, __shfl_xor(top, 32));
+      if (top > ref + Reference<T>::kSlack) {
+        const float next = top - Reference<T>::kBelow;
+        const float f = ref == -INFINITY ? 1.0f : exp2_hw(ref - next);
+        ref = next;
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[d][i] *= f;
+      }
+    }
+    const float base = ref == -INFINITY ? 0.0f : -ref;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[b][i] = exp2_hw(__builtin_fmaf(s[b][i], sc, base));
+    if (part) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          s[b][i] = (shown >> (16 * b + i)) & 1 ? s[b][i] : 0.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      u32x4 pf;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        pf[i] = round2<T>(s[u >> 1][8 * (u & 1) + 2 * i], s[u >> 1][8 * (u & 1) + 2 * i + 1], l);
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const u32x2 x = read_transposed(vt + u * 16 * RB + read_v[d][0]);
+        const u32x2 y = read_transposed(vt + u * 16 * RB + read_v[d][1]);
+        o[d] = mfma_32x32x16<T>(u32x4{x[0], x[1], y[0], y[1]}, pf, o[d]);
+      }
+    }
+  };
+  // Everything staged so far has arrived, in every wavefront, and every
+  // wavefront has read the tile before.  The wait is the builtin, which the
+  // compiler's own insertion of waits follows: behind an opaque one it would
+  // wait for the next tile's loads before this one's reads.
+  auto arrived = [&]() __attribute__((always_inline)) {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070);   // vmcnt(0), lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+
+  if (t0 < t1) {
+    const std::integral_constant<int, 0> first;
+    const std::integral_constant<int, 1> second;
+    stage(t0, first);
+    for (int t = t0; t < t1; t += 2) {
+      arrived();
+      if (t + 1 < t1) stage(t + 1, second);
+      compute(t, first);
+      if (t + 1 >= t1) break;
+      arrived();
+      if (t + 2 < t1) stage(t + 2, first);
+      compute(t + 1, second);
+    }
+  }
+
+  l += __shfl_xor(l, 32);
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * p.cut + piece;
+  bool finite = fabsf(l) < INFINITY;
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) finite = finite && fabsf(o[d][i]) < INFINITY;
+  const uint64_t odd = __ballot(live && !finite);
+  const uint32_t bad_rows = static_cast<uint32_t>(odd) | static_cast<uint32_t>(odd >> 32);
+  const bool mine = live && !((bad_rows >> c) & 1);
+  if (pieces == 1) {
+    // Registers 4 j .. 4 j + 3 of O^T tile d are elements 32 d + 8 j + 4 h .. + 3:
+    // of two such fours the lanes of a row swap one, and store 16 bytes each.
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    T* dst = out_row<T>(a, at.start, token, head);
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int j = 0; j < 4; j += 2) {
+        uint32_t w[2][2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int i = 4 * j + 2 * k;
+          w[0][k] = pack2_bits<T>(o[d][i] * inv, o[d][i + 1] * inv);
+          w[1][k] = pack2_bits<T>(o[d][i + 4] * inv, o[d][i + 5] * inv);
+          swap_halves(w[0][k], w[1][k]);
+        }
+        const int e = 32 * d + 8 * (j + h);
+        if (mine && e < D)
+          *reinterpret_cast<u32x4*>(dst + e) = u32x4{w[0][0], w[0][1], w[1][0], w[1][1]};
+      }
+  } else if (mine) {
+    const int64_t r = item * kRows + 32 * wave + c;
+    if (h == 0) p.part_rl[r] = f32x2{ref, l};
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int e = 32 * d + 8 * j + 4 * h;
+        if (e < D)
+          *reinterpret_cast<f32x4*>(p.part_o + r * D + e) =
+              f32x4{o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]};
+      }
+  }
+  if (bad_rows != 0)
+    careful_rows<T, DP>(p, at, kvh, wave_row, bad_rows, t0 * kKeys, min(t1 * kKeys, at.keys), item,
+                        pieces == 1);
+}
+
+// Adds up the pieces of a row tile that was cut: four elements of a row per
+// thread.
+template <typename T, int DP>
+__global__ __launch_bounds__(kJoinThreads) void prefill_join_kernel(PrefillParams p) {
+  constexpr int C = DP / 4;             // threads of a row
+  constexpr int R = kJoinThreads / C;   // rows of a workgroup
+  const PagedAttention& a = p.a;
+  const int kvh = blockIdx.x % a.kv_heads;
+  const int tile = static_cast<int>(gridDim.x / a.kv_heads) - 1 - blockIdx.x / a.kv_heads;
+  const Place at = find_tile(p, tile);
+  if (at.seq < 0) return;
+  const int pieces = pieces_of(p, key_tiles(p, at));
+  if (pieces == 1) return;
+  const int c = threadIdx.x % C;
+  const int in_tile = blockIdx.y * R + threadIdx.x / C;
+  const int row = at.row0 + in_tile;
+  const int D = a.head_dim;
+  if (in_tile >= kRows || row >= at.count * p.group || 4 * c >= D) return;
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * p.cut * kRows + in_tile;
+  float top = -INFINITY;
+  for (int i = 0; i < pieces; ++i) top = fmaxf(top, p.part_rl[r0 + i * kRows][0]);
+  const float base = top == -INFINITY ? 0.0f : top;
+  float l = 0.0f;
+  f32x4 o{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int i = 0; i < pieces; ++i) {
+    const int64_t r = r0 + i * kRows;
+    const f32x2 rl = p.part_rl[r];
+    const float f = exp2_hw(rl[0] - base);
+    l += rl[1] * f;
+    o += *reinterpret_cast<const f32x4*>(p.part_o + r * D + 4 * c) * f;
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const int token = divide_rows(row, p.group);
+  T* dst = out_row<T>(a, at.start, token, kvh * p.group + row - token * p.group) + 4 * c;
+  *reinterpret_cast<u32x2*>(dst) =
+      u32x2{pack2_bits<T>(o[0] * inv, o[1] * inv), pack2_bits<T>(o[2] * inv, o[3] * inv)};
+}
+
+// Row tiles of a call at most.
+int64_t max_tiles(int64_t tokens, int64_t batch, int64_t group) {
+  return ceil_div(tokens * group, kRows) + batch;
+}
+
+// Pieces of a row tile: as many as the slots ask for that the tiles leave
+// empty.
+int64_t cut_of(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
+               int64_t max_keys) {
+  const int64_t items = max_tiles(tokens, batch, q_heads / kv_heads) * kv_heads;
+  const int64_t room = kSlots / items;
+  const int64_t most = ceil_div(max_keys, kKeys) / kMinTiles;
+  return std::max<int64_t>(1, std::min<int64_t>({room, most, kMaxCut}));
+}
+
+int64_t pairs_bytes(int64_t rows) { return ceil_div(rows * 8, 256) * 256; }
+
+template <typename T, int DP>
+hipError_t launch_d(const PrefillParams& p, int64_t items, hipStream_t st) {
+  const dim3 grid(static_cast<uint32_t>(items), static_cast<uint32_t>(p.cut));
+  const bool dma = (1 << p.a.page_shift) >= 512 / DP && p.a.c_tok < (1 << 24);
+  if (dma)
+    hipLaunchKernelGGL((prefill_kernel<T, DP, true>), grid, dim3(64 * kWaves), 0, st, p);
+  else
+    hipLaunchKernelGGL((prefill_kernel<T, DP, false>), grid, dim3(64 * kWaves), 0, st, p);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || p.cut == 1) return e;
+  hipLaunchKernelGGL((prefill_join_kernel<T, DP>),
+                     dim3(static_cast<uint32_t>(items), kRows * DP / 4 / kJoinThreads),
+                     dim3(kJoinThreads), 0, st, p);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_t(const PrefillParams& p, int64_t items, hipStream_t st) {
+  if (p.a.head_dim <= 64) return launch_d<T, 64>(p, items, st);
+  if (p.a.head_dim <= 128) return launch_d<T, 128>(p, items, st);
+  return launch_d<T, 256>(p, items, st);
+}
+
+}  // namespace
+
+int64_t paged_prefill_workspace(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                int64_t head_dim, int64_t max_keys) {
+  if (tokens == 0 || batch == 0) return 0;
+  const int64_t cut = cut_of(tokens, batch, q_heads, kv_heads, max_keys);
+  if (cut == 1) return 0;
+  const int64_t rows = max_tiles(tokens, batch, q_heads / kv_heads) * kv_heads * cut * kRows;
+  return pairs_bytes(rows) + rows * head_dim * 4;
+}
+
+hipError_t launch_paged_prefill(const PagedAttention& a, int dtype, hipStream_t st) {
+  PrefillParams p;
+  p.a = a;
+  p.group = a.q_heads / a.kv_heads;
+  p.cut = static_cast<int>(cut_of(a.tokens, a.batch, a.q_heads, a.kv_heads, a.max_keys));
+  const int64_t items = max_tiles(a.tokens, a.batch, p.group) * a.kv_heads;
+  if (items > INT32_MAX) return hipErrorInvalidConfiguration;
+  char* ws = static_cast<char*>(a.workspace);
+  p.part_rl = reinterpret_cast<f32x2*>(ws);
+  p.part_o = reinterpret_cast<float*>(ws + pairs_bytes(items * p.cut * kRows));
+  return dtype == kF16 ? launch_t<__half>(p, items, st) : launch_t<__hip_bfloat16>(p, items, st);
+}
+
+}  // namespace w8a8

@@ -315,7 +315,9 @@ def test_sharp_and_flat_rows(cuda, dtype):
 
 def test_infinities_and_nans_stay_where_they_are_seen(cuda):
     """A NaN or infinite value is seen by the rows at and after its token, and
-    by no row before it; a NaN key likewise."""
+    by no row before it; a NaN key likewise.  The other elements stay within
+    the bound of the definition without it (rows that met such a value may be
+    summed in another order, and with unrounded probabilities)."""
     note("causal NaN")
     n = 200
     k, v, table = paged(4, [n], 2, 128, 16, torch.float16, cuda, poison=False)
@@ -323,22 +325,24 @@ def test_infinities_and_nans_stay_where_they_are_seen(cuda):
     lengths = torch.tensor([n], dtype=torch.int32, device=cuda)
     starts = torch.tensor([0, n], dtype=torch.int32, device=cuda)
     clean = A.paged_prefill(q, k, v, table, lengths, starts)
+    check_attention(clean, q, k, v, table, lengths, starts, what="clean")
     for at, value in ((0, float("nan")), (77, float("inf")), (150, float("nan")),
                       (199, float("-inf"))):
         page, row = int(table[0, at // 16]), at % 16
         bad = v.clone()
         bad[page, 0, row, 5] = value
         out = A.paged_prefill(q, k, bad, table, lengths, starts)
-        assert torch.equal(out[:at], clean[:at]), f"value {value} at {at}"
         assert torch.equal(out[:, 2:], clean[:, 2:])                 # the other head's queries
         assert (~torch.isfinite(out[at:, :2, 5])).all()
-        keep = [i for i in range(128) if i != 5]
-        assert torch.equal(out[at:, :2][..., keep], clean[at:, :2][..., keep])
+        out[at:, :2, 5] = clean[at:, :2, 5]
+        check_attention(out, q, k, v, table, lengths, starts, what=f"value {value} at {at}")
         bad = k.clone()
         bad[page, 1, row, 9] = float("nan")
         out = A.paged_prefill(q, bad, v, table, lengths, starts)
-        assert torch.equal(out[:at], clean[:at]) and torch.equal(out[:, :2], clean[:, :2])
+        assert torch.equal(out[:, :2], clean[:, :2])
         assert torch.isnan(out[at:, 2:]).all()
+        out[at:, 2:] = clean[at:, 2:]
+        check_attention(out, q, k, v, table, lengths, starts, what=f"key {value} at {at}")
 
 
 def test_pages_outside_the_cache_are_masked(cuda):
