@@ -14,16 +14,19 @@
 //   * A workgroup takes 128 rows of one key head, 32 per wavefront, held in
 //     registers; the queries that share a key head are packed as rows, so a
 //     short chunk fills its tiles and every key is read once per 128 rows.
-//   * Keys and values pass through a double-buffered LDS tile of 64 keys,
-//     filled by LDS-DMA buffer loads straight from the pages: one descriptor
-//     per load, whose range ends at the sequence's last key, so what lies
-//     behind it arrives as zeros.  16-byte chunks are permuted by key (in the
-//     source address), which leaves the reads of both operands without bank
-//     conflicts.
+//   * Units of 32 keys and of 32 values pass through double buffers in LDS,
+//     filled by LDS-DMA buffer loads straight from the pages, a unit ahead of
+//     their use: one descriptor per load, whose range ends at the
+//     sequence's last key, so what lies behind it arrives as zeros.  16-byte
+//     chunks are permuted by key (in the source address), which leaves the
+//     reads of both operands without bank conflicts.
+//   * While a unit's scores become probabilities on the vector unit, the
+//     matrix unit forms the next one's scores and the product of the one
+//     before with its values: neither waits for the other.
 //   * The score tile's registers are the second product's operand as they
 //     are: its inner index is summed over, so the values are read (transposing
 //     ds_read_b64_tr_b16) in the key order that the scores have.
-//   * Masks are formed for the tiles that a row of the wavefront sees in part,
+//   * Masks are formed for the units that a row of the wavefront sees in part,
 //     the last ones; the others have none.
 //   * Few rows far into a long cache are cut over its length: each piece
 //     leaves (O, r, l) in the workspace and join_kernel adds them up.
@@ -45,11 +48,11 @@ typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef const int32_t __attribute__((address_space(4))) const_i32;   // scalar loads
 
-constexpr int kKeys = 64;            // keys of a tile
+constexpr int kKeys = 32;            // keys of a unit
 constexpr int kWaves = 4;
 constexpr int kRows = 32 * kWaves;   // rows of a workgroup
 constexpr int kSlots = 512;          // workgroups below which the keys are cut
-constexpr int kMinTiles = 4;         // least tiles of a piece
+constexpr int kMinUnits = 8;         // least units of a piece
 constexpr int kMaxCut = 32;
 constexpr int kOutside = 0x7ffffff0;   // a buffer offset past every range
 constexpr int kBufferWord3 = 0x00020000;
@@ -106,22 +109,24 @@ __device__ inline Place find_tile(const PrefillParams& p, int tile) {
       const int at = __ffsll(static_cast<unsigned long long>(found)) - 1;
       const int first = before + lane_value(upto, at) - lane_value(tiles, at);
       const int seq = b0 + at;
+      const int keys = __builtin_amdgcn_readfirstlane(a.lengths[seq]);
       return Place{seq, lane_value(s0, at), lane_value(n, at), (tile - first) * kRows,
-                   max(0, min(a.lengths[seq], a.max_keys))};
+                   max(0, min(keys, a.max_keys))};
     }
     before += lane_value(upto, 63);
   }
   return Place{-1, 0, 0, 0, 0};
 }
 
-// Key tiles that the rows of a tile see, and how many pieces they are cut into.
-__device__ inline int key_tiles(const PrefillParams& p, const Place& at) {
+// Units of keys that the rows of a tile see, and how many pieces they are cut
+// into.
+__device__ inline int key_units(const PrefillParams& p, const Place& at) {
   const int last = min(at.row0 + kRows, at.count * p.group) - 1;
   const int seen = at.keys - at.count + divide_rows(last, p.group) + 1;
   return (max(seen, 0) + kKeys - 1) / kKeys;
 }
-__device__ inline int pieces_of(const PrefillParams& p, int tiles) {
-  return max(1, min(p.cut, tiles / kMinTiles));
+__device__ inline int pieces_of(const PrefillParams& p, int units) {
+  return max(1, min(p.cut, units / kMinUnits));
 }
 
 template <typename T>
@@ -167,9 +172,8 @@ __device__ inline void swap_halves(uint32_t& x, uint32_t& y) {
 
 // Each 16 lanes read 16 x 8 bytes, four rows of 16 elements (lane i: element
 // 4 (i % 4) of row i / 4), and lane i gets element i of the four rows.
-__device__ inline u32x2 read_transposed(const char* lds) {
-  return __builtin_bit_cast(u32x2,
-                            __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds)));
+__device__ inline u32x2 read_transposed(lds_s16x4* __restrict__ lds) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds));
 }
 
 // Chunk permutations of a key's row of DP / 8 chunks of 16 bytes: position =
@@ -251,18 +255,21 @@ __device__ inline void careful_rows(const PrefillParams& p, const Place& at, int
   }
 }
 
-// DP: head_dim rounded up to 64, 128 or 256.  DMA: the pages hold whole loads
-// of 1 KiB (512 / DP keys), else each chunk is copied through registers.
+// DP: head_dim rounded up to 64, 128 or 256.  DMA: pages of at least 8 keys,
+// the part of a unit that a wavefront copies; else each chunk is copied through
+// registers.
 template <typename T, int DP, bool DMA>
 __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) void prefill_kernel(PrefillParams p) {
-  constexpr int KS = DP / 16;                 // first product: steps over the head
-  constexpr int DT = DP / 32;                 // second product: row tiles of O^T
-  constexpr int RB = DP * 2;                  // bytes of a key's row
-  constexpr int RL = 1024 / RB;               // keys of a load
-  constexpr int NL = kKeys / RL / kWaves;     // loads per wavefront and operand
-  constexpr int TB = kKeys * RB;              // bytes of a tile
-  __shared__ __align__(16) char lds[4 * TB];  // K, V of one tile, then of the other
-  __shared__ int unknown[2][kWaves];          // loads of unknown pages, per wavefront
+  constexpr int KS = DP / 16;               // first product: steps over the head
+  constexpr int DT = DP / 32;               // second product: row tiles of O^T
+  constexpr int RB = DP * 2;                // bytes of a key's row
+  constexpr int RL = 1024 / RB;             // keys of a load
+  constexpr int NL = kKeys / RL / kWaves;   // loads per wavefront, unit and operand
+  constexpr int UB = kKeys * RB;            // bytes of a unit of one operand
+  // Four arrays, so that the compiler sees that one is read while loads into
+  // the others are in flight.
+  __shared__ __align__(16) char k0[UB], k1[UB], v0[UB], v1[UB];
+  __shared__ int odd_pages[kWaves];
 
   const PagedAttention& a = p.a;
   const int lane = threadIdx.x & 63;
@@ -273,118 +280,105 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) void prefill_kernel
   const int tile = static_cast<int>(gridDim.x / a.kv_heads) - 1 - blockIdx.x / a.kv_heads;
   const Place at = find_tile(p, tile);
   if (at.seq < 0) return;
-  const int all_tiles = key_tiles(p, at);
-  const int pieces = pieces_of(p, all_tiles);
+  const int all_units = key_units(p, at);
+  const int pieces = pieces_of(p, all_units);
   const int piece = blockIdx.y;
   if (piece >= pieces) return;
-  const int t0 = all_tiles * piece / pieces, t1 = all_tiles * (piece + 1) / pieces;
+  const int u0 = __builtin_amdgcn_readfirstlane(
+      static_cast<int>(static_cast<int64_t>(all_units) * piece / pieces));
+  const int u1 = __builtin_amdgcn_readfirstlane(
+      static_cast<int>(static_cast<int64_t>(all_units) * (piece + 1) / pieces));
   const int D = a.head_dim;
   const int total_rows = at.count * p.group;
   const int wave_row = at.row0 + 32 * wave;
-  const int row = wave_row + c;
-  const bool live = row < total_rows;
-  const int token = divide_rows(min(row, total_rows - 1), p.group);
-  const int head = kvh * p.group + min(row, total_rows - 1) - token * p.group;
+  const int row = min(wave_row + c, total_rows - 1);
+  const bool live = wave_row + c < total_rows;
+  const int token = divide_rows(row, p.group);
+  const int head = kvh * p.group + row - token * p.group;
   const int seen = live ? at.keys - at.count + token : -1;   // the row's last key
-  // The wavefront's least and greatest last key.
-  const int seen_first =
-      wave_row < total_rows ? at.keys - at.count + divide_rows(wave_row, p.group) : -1;
-  const int seen_last = wave_row < total_rows
-                            ? at.keys - at.count +
-                                  divide_rows(min(wave_row + 31, total_rows - 1), p.group)
-                            : -1;
-
-  // Queries, negated for a negative scale so that the scale below is not.
-  u32x4 qf[KS];
-  {
-    const uint16_t* q =
-        static_cast<const uint16_t*>(a.q) + (at.start + token) * a.q_st + head * a.q_sh + 8 * h;
-    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      qf[s] = u32x4{0, 0, 0, 0};
-      if (live && 16 * s + 8 * h < D) qf[s] = *reinterpret_cast<const u32x4*>(q + 16 * s);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) qf[s][i] ^= flip;
-    }
-  }
-  const float sc = fabsf(a.scale) * kLog2e;
+  // The first row's and the last row's last key of the wavefront.
+  const int seen_first = __builtin_amdgcn_readlane(seen, 0);
+  const int seen_last = __builtin_amdgcn_readlane(
+      seen, max(0, min(31, total_rows - 1 - wave_row)));
+  // The wavefront's units end here; it copies and waits to u1 with the others.
+  const int end =
+      __builtin_amdgcn_readfirstlane(max(u0, seen_last < 0 ? 0 : min(u1, seen_last / kKeys + 1)));
 
   // Loading: lane's key within a load and its chunk's position there.
   const int lk = lane / (RB / 16), lp = lane % (RB / 16);
   const_i32* table = (const_i32*)(a.table + at.seq * a.ld_table);
   const int page_mask = (1 << a.page_shift) - 1;
-  const int ctok = static_cast<int>(a.c_tok);   // DMA: RL rows stay below 2^31 bytes
+  const int ctok = static_cast<int>(a.c_tok);   // DMA: a page stays below 2^31 elements
+  const int pages = static_cast<int>(a.pages);
+  const uint16_t* kb = static_cast<const uint16_t*>(a.k) + kvh * a.c_head;
+  const uint16_t* vb = static_cast<const uint16_t*>(a.v) + kvh * a.c_head;
   int off_k[NL], off_v[NL];
 #pragma unroll
   for (int m = 0; m < NL; ++m) {
     const int key = (wave * NL + m) * RL + lk;
     const int ck = (lp ^ swizzle_k<DP>(key)) * 8, cv = (lp ^ swizzle_v<DP>(key)) * 8;
-    off_k[m] = ck < D ? (lk * ctok + ck) * 2 : kOutside;
-    off_v[m] = cv < D ? (lk * ctok + cv) * 2 : kOutside;
+    off_k[m] = ck < D ? ((m * RL + lk) * ctok + ck) * 2 : kOutside;
+    off_v[m] = cv < D ? ((m * RL + lk) * ctok + cv) * 2 : kOutside;
   }
-  auto stage = [&](int t, auto buffer) __attribute__((always_inline)) {
-    constexpr int buf = decltype(buffer)::value;
-    char* dst = lds + buf * 2 * TB + wave * NL * 1024;
-    int bad = 0;
+  // A wavefront copies eight keys of a unit.  DMA: they lie in one page, whose
+  // place (of keys and of values) is formed once, in scalar registers; rows
+  // past the sequence's last key and of unknown pages arrive as zeros.
+  const int first_key = wave * (kKeys / kWaves);
+  struct Source {
+    int64_t offset;   // elements
+    int range;        // bytes
+  };
+  auto lookup = [&](int u) __attribute__((always_inline)) {
+    return DMA ? table[min(u * kKeys + first_key, at.keys - 1) >> a.page_shift] : 0;
+  };
+  auto locate = [&](int u, int page) __attribute__((always_inline)) {
+    const int key = u * kKeys + first_key;
+    const int left = at.keys - key;
+    const bool known = left > 0 && static_cast<uint32_t>(page) < static_cast<uint32_t>(pages);
+    return Source{known ? page * a.c_page + (key & page_mask) * ctok : int64_t{0},
+                  known ? (left < 8 ? left : 8) * (2 * ctok) : 0};
+  };
+  auto copy = [&](int u, const Source& src, const uint16_t* cache, const int (&off)[NL],
+                  char* dst, auto is_key) __attribute__((always_inline)) {
+    char* to = dst + wave * NL * 1024;
     if constexpr (DMA) {
+      const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<uint16_t*>(cache + src.offset), 0, src.range, kBufferWord3);
 #pragma unroll
-      for (int m = 0; m < NL; ++m) {
-        const int key = t * kKeys + (wave * NL + m) * RL;
-        int page = -1;
-        if (key < at.keys) page = table[key >> a.page_shift];
-        const bool known = page >= 0 && page < a.pages;
-        if (key < at.keys && !known) bad |= 1 << m;
-        const int64_t off =
-            known ? page * a.c_page + kvh * a.c_head + (key & page_mask) * a.c_tok : int64_t{0};
-        const int range = known ? min(RL, at.keys - key) * ctok * 2 : 0;
-        const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<uint16_t*>(static_cast<const uint16_t*>(a.k) + off), 0, range,
-            kBufferWord3);
-        const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<uint16_t*>(static_cast<const uint16_t*>(a.v) + off), 0, range,
-            kBufferWord3);
-        dma16(rk, dst + m * 1024, off_k[m]);
-        dma16(rv, dst + TB + m * 1024, off_v[m]);
-      }
+      for (int m = 0; m < NL; ++m) dma16(r, to + m * 1024, off[m]);
     } else {
 #pragma unroll
       for (int m = 0; m < NL; ++m) {
-        const int in_tile = (wave * NL + m) * RL + lk;
-        const int key = t * kKeys + in_tile;
+        const int in_unit = first_key + m * RL + lk;
+        const int key = u * kKeys + in_unit;
         int page = -1;
         if (key < at.keys) page = a.table[at.seq * a.ld_table + (key >> a.page_shift)];
-        const bool known = page >= 0 && page < a.pages;
-        if (__any(key < at.keys && !known)) bad = 1;
-        const int64_t off = page * a.c_page + kvh * a.c_head + (key & page_mask) * a.c_tok;
-        const int ck = (lp ^ swizzle_k<DP>(in_tile)) * 8, cv = (lp ^ swizzle_v<DP>(in_tile)) * 8;
-        u32x4 kv{0, 0, 0, 0}, vv{0, 0, 0, 0};
-        if (known && ck < D)
-          kv = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.k) + off + ck);
-        if (known && cv < D)
-          vv = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.v) + off + cv);
-        *reinterpret_cast<u32x4*>(dst + m * 1024 + lane * 16) = kv;
-        *reinterpret_cast<u32x4*>(dst + TB + m * 1024 + lane * 16) = vv;
+        const int chunk =
+            (lp ^ (decltype(is_key)::value ? swizzle_k<DP>(in_unit) : swizzle_v<DP>(in_unit))) * 8;
+        u32x4 x{0, 0, 0, 0};
+        if (page >= 0 && page < pages && chunk < D)
+          x = *reinterpret_cast<const u32x4*>(cache + page * a.c_page +
+                                              (key & page_mask) * a.c_tok + chunk);
+        *reinterpret_cast<u32x4*>(to + m * 1024 + lane * 16) = x;
       }
     }
-    if (lane == 0) unknown[buf][wave] = bad;
   };
-
-  // Reading: byte offsets of the operands in a tile.
-  int read_k[KS], read_v[DT][2];
-#pragma unroll
-  for (int s = 0; s < KS; ++s) read_k[s] = c * RB + (((2 * s + h) ^ swizzle_k<DP>(c)) * 16);
-  {
-    const int i = lane & 15, g = (lane >> 4) & 1;
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const int key = 8 * b + 4 * h + (i >> 2);
-#pragma unroll
-      for (int d = 0; d < DT; ++d)
-        read_v[d][b] = key * RB +
-                       (((4 * d + 2 * g + ((i & 3) >> 1)) ^ swizzle_v<DP>(key)) * 16) + 8 * (i & 1);
-    }
-  }
+  auto copy_k = [&](int u, const Source& src, char* dst) __attribute__((always_inline)) {
+    copy(u, src, kb, off_k, dst, std::true_type{});
+  };
+  auto copy_v = [&](int u, const Source& src, char* dst) __attribute__((always_inline)) {
+    copy(u, src, vb, off_v, dst, std::false_type{});
+  };
+  // At most N of this wavefront's loads are in flight, so are the others', and
+  // every wavefront has read what it was reading.  The wait is the builtin,
+  // which the compiler's own insertion of waits follows.
+  auto arrived = [&](auto n) __attribute__((always_inline)) {
+    constexpr int N = decltype(n)::value;
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4));   // lgkmcnt(0) too
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
 
   f32x16 o[DT];
 #pragma unroll
@@ -393,117 +387,216 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) void prefill_kernel
     for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
   float ref = -INFINITY, l = 0.0f;
 
-  auto compute = [&](int t, auto buffer) __attribute__((always_inline)) {
-    constexpr int buf = decltype(buffer)::value;
-    const char* kt = lds + buf * 2 * TB;
-    const char* vt = kt + TB;
-    const int key0 = t * kKeys;
-    if (key0 > seen_last) return;   // no row of the wavefront sees it
-    f32x16 s[2];
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
-#pragma unroll
-      for (int k = 0; k < KS; ++k)
-        s[b] = mfma_32x32x16<T>(
-            *reinterpret_cast<const u32x4*>(kt + b * 32 * RB + read_k[k]), qf[k], s[b]);
-    }
-    int bad = 0;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) bad |= unknown[buf][w];
-    bad = __builtin_amdgcn_readfirstlane(bad);
-    const bool part = key0 + kKeys - 1 > seen_first || bad != 0;
-    uint32_t shown = 0xffffffffu;   // bit 16 b + i: s[b][i]'s key is seen
-    if (part) {
-      if (bad != 0) {
-#pragma unroll 1
-        for (int n = 0; n < 32; ++n) {
-          const int key = key0 + 32 * (n >> 4) + 8 * ((n >> 2) & 3) + 4 * h + (n & 3);
-          int page = 0;
-          if (key < at.keys) page = a.table[at.seq * a.ld_table + (key >> a.page_shift)];
-          if (page < 0 || page >= a.pages) shown &= ~(1u << n);
-        }
+  if (u0 < u1) {
+    // The places of the two units whose values come next; the page of the one
+    // whose keys do.
+    Source source = locate(u0, lookup(u0)), source_1 = locate(u0 + 1, lookup(u0 + 1));
+    int page = lookup(u0 + 2);
+    copy_k(u0, source, k0);
+    copy_k(u0 + 1, source_1, k1);
+    auto copies = [&](int i, char* kfree, char* vn) __attribute__((always_inline)) {
+      const Source source_2 = locate(i + 2, page);
+      copy_k(i + 2, source_2, kfree);
+      copy_v(i, source, vn);
+      source = source_1;
+      source_1 = source_2;
+    };
+
+    // Values of the unit before the first.
+    for (int i = threadIdx.x * 16; i < UB; i += 64 * kWaves * 16)
+      *reinterpret_cast<u32x4*>(v1 + i) = u32x4{0, 0, 0, 0};
+    // Whether a page of these keys is unknown: then every unit looks its keys
+    // up.
+    int odd = 0;
+    {
+      const int n = ((min(u1 * kKeys, at.keys) - 1) >> a.page_shift) + 1;
+      for (int i = (u0 * kKeys >> a.page_shift) + threadIdx.x; i < n; i += 64 * kWaves) {
+        const int page = a.table[at.seq * a.ld_table + i];
+        odd |= page < 0 || page >= a.pages;
       }
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const uint32_t bit = 1u << (16 * b + i);
-          if (key0 + 32 * b + 8 * (i >> 2) + 4 * h + (i & 3) > seen) shown &= ~bit;
-          s[b][i] = shown & bit ? s[b][i] : -INFINITY;
-        }
+      const bool any = __any(odd);
+      if (lane == 0) odd_pages[wave] = any;
     }
-    float top = s[0][0];
+    // Queries, negated for a negative scale so that the one below is not, and
+    // zeros for a scale of zero.
+    u32x4 qf[KS];
+    {
+      const uint16_t* q =
+          static_cast<const uint16_t*>(a.q) + (at.start + token) * a.q_st + head * a.q_sh + 8 * h;
+      const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+      for (int s = 0; s < KS; ++s) {
+        qf[s] = u32x4{0, 0, 0, 0};
+        if (live && a.scale != 0.0f && 16 * s + 8 * h < D)
+          qf[s] = *reinterpret_cast<const u32x4*>(q + 16 * s);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
-    top *= sc;
-    if (__any(top > ref + Reference<T>::kSlack)) {
-      // Raise the reference of the rows that need it; both lanes of a row agree.
-      top = fmaxf(top, __shfl_xor(top, 32));
-      if (top > ref + Reference<T>::kSlack) {
-        const float next = top - Reference<T>::kBelow;
-        const float f = ref == -INFINITY ? 1.0f : exp2_hw(ref - next);
-        ref = next;
-        l *= f;
+        for (int i = 0; i < 4; ++i) qf[s][i] ^= flip;
+      }
+    }
+    const float sc = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * kLog2e;
+
+    // Reading: byte offsets of the operands in a unit.
+    int read_k[KS], read_v[DT][2];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) read_k[s] = c * RB + (((2 * s + h) ^ swizzle_k<DP>(c)) * 16);
+    {
+      const int i = lane & 15, g = (lane >> 4) & 1;
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const int key = 8 * b + 4 * h + (i >> 2);
 #pragma unroll
         for (int d = 0; d < DT; ++d)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[d][i] *= f;
+          read_v[d][b] = key * RB +
+                         (((4 * d + 2 * g + ((i & 3) >> 1)) ^ swizzle_v<DP>(key)) * 16) +
+                         8 * (i & 1);
       }
     }
-    const float base = ref == -INFINITY ? 0.0f : -ref;
+
+    f32x16 even, odd_s;   // scores of this unit and of the next one
+    u32x4 pf[2];   // probabilities of the unit before
+    pf[0] = pf[1] = u32x4{0, 0, 0, 0};
+    auto key_operand = [&](const char* kt, int k) __attribute__((always_inline)) {
+      return *reinterpret_cast<const u32x4*>(kt + read_k[k]);
+    };
+    auto value_operand = [&](char* vt, int u, int d) __attribute__((always_inline)) {
+      const u32x2 x = read_transposed((lds_s16x4*)(vt + u * 16 * RB + read_v[d][0]));
+      const u32x2 y = read_transposed((lds_s16x4*)(vt + u * 16 * RB + read_v[d][1]));
+      return u32x4{x[0], x[1], y[0], y[1]};
+    };
+    auto weight = [&](f32x16& s, int i, float base) __attribute__((always_inline)) {
+      s[i] = exp2_hw(__builtin_fmaf(s[i], sc, base));
+    };
+    auto weights_of = [&](f32x16& s, int i) __attribute__((always_inline)) {
+      pf[i >> 2][i & 3] = round2<T>(s[2 * i], s[2 * i + 1], l);
+    };
+    arrived(std::integral_constant<int, DMA ? NL : 0>{});
+    odd = odd_pages[0] | odd_pages[1] | odd_pages[2] | odd_pages[3];
+    odd = __builtin_amdgcn_readfirstlane(odd);
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int n = 0; n < 16; ++n) even[n] = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[b][i] = exp2_hw(__builtin_fmaf(s[b][i], sc, base));
-    if (part) {
+    for (int k = 0; k < KS; ++k) even = mfma_32x32x16<T>(key_operand(k0, k), qf[k], even);
+
+    // Unit i: the product of the unit before with its values (zeros for the
+    // first), then the scores of the next one while this one's become
+    // probabilities.  The order of the instructions is held (sched_barrier):
+    // operands are read ahead of their matrix instructions, copies are issued
+    // and the vector work is done while those run.
+    auto unit = [&](int i, f32x16& s, f32x16& next, char* kn, char* kfree, char* vp, char* vn)
+        __attribute__((always_inline)) {
+      arrived(std::integral_constant<int, 0>{});
+      u32x4 vf[2][DT], kf[KS];
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          s[b][i] = (shown >> (16 * b + i)) & 1 ? s[b][i] : 0.0f;
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      u32x4 pf;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        pf[i] = round2<T>(s[u >> 1][8 * (u & 1) + 2 * i], s[u >> 1][8 * (u & 1) + 2 * i + 1], l);
+      for (int d = 0; d < DT; ++d) vf[0][d] = value_operand(vp, 0, d);
+      __builtin_amdgcn_sched_barrier(0);
+      copies(i, kfree, vn);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
-        const u32x2 x = read_transposed(vt + u * 16 * RB + read_v[d][0]);
-        const u32x2 y = read_transposed(vt + u * 16 * RB + read_v[d][1]);
-        o[d] = mfma_32x32x16<T>(u32x4{x[0], x[1], y[0], y[1]}, pf, o[d]);
+        vf[1][d] = value_operand(vp, 1, d);
+        o[d] = mfma_32x32x16<T>(vf[0][d], pf[0], o[d]);
+        __builtin_amdgcn_sched_barrier(0);
       }
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        kf[d] = key_operand(kn, d);
+        o[d] = mfma_32x32x16<T>(vf[1][d], pf[1], o[d]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      const int key0 = i * kKeys;
+      if (key0 + kKeys - 1 > seen_first || odd != 0) {
+        uint32_t shown = 0xffffu;
+        if (odd != 0) {
+#pragma unroll 1
+          for (int n = 0; n < 16; ++n) {
+            const int key = key0 + 8 * (n >> 2) + 4 * h + (n & 3);
+            int page = 0;
+            if (key < at.keys) page = a.table[at.seq * a.ld_table + (key >> a.page_shift)];
+            if (page < 0 || page >= pages) shown &= ~(1u << n);
+          }
+        }
+        const int left = seen - key0 - 4 * h;
+#pragma unroll
+        for (int n = 0; n < 16; ++n) {
+          const bool there = 8 * (n >> 2) + (n & 3) <= left && ((shown >> n) & 1);
+          s[n] = there ? s[n] : -INFINITY;
+        }
+      }
+      float top = s[0];
+#pragma unroll
+      for (int n = 1; n < 16; ++n) top = fmaxf(top, s[n]);
+      top *= sc;
+      if (__any(top > ref + Reference<T>::kSlack)) {
+        // Raise the reference of the rows that need it; both lanes of a row
+        // agree.
+        top = fmaxf(top, __shfl_xor(top, 32));
+        if (top > ref + Reference<T>::kSlack) {
+          const float raised = top - Reference<T>::kBelow;
+          const float f = ref == -INFINITY ? 1.0f : exp2_hw(ref - raised);
+          ref = raised;
+          l *= f;
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int n = 0; n < 16; ++n) o[d][n] *= f;
+        }
+      }
+      const float base = ref == -INFINITY ? 0.0f : -ref;
+      constexpr int E = 16 / KS;   // probabilities per matrix instruction
+#pragma unroll
+      for (int n = 0; n < 16; ++n) next[n] = 0.0f;
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        if (k + DT < KS) kf[k + DT] = key_operand(kn, k + DT);
+        next = mfma_32x32x16<T>(kf[k], qf[k], next);
+#pragma unroll
+        for (int e = 0; e < E; ++e) weight(s, k * E + e, base);
+        // The pairs of the step before.
+#pragma unroll
+        for (int n = (k - 1) * E; n < k * E; ++n)
+          if (n > 0 && (n & 1)) weights_of(s, n >> 1);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int n = 16 - E; n < 16; ++n)
+        if (n & 1) weights_of(s, n >> 1);
+      __builtin_amdgcn_sched_barrier(0);
+      page = lookup(i + 3);   // waited for with the next unit's copies
+    };
+    int i = u0;
+    while (i < end) {
+      unit(i, even, odd_s, k1, k0, v1, v0);
+      if (++i >= end) break;
+      unit(i, odd_s, even, k0, k1, v0, v1);
+      ++i;
     }
-  };
-  // Everything staged so far has arrived, in every wavefront, and every
-  // wavefront has read the tile before.  The wait is the builtin, which the
-  // compiler's own insertion of waits follows: behind an opaque one it would
-  // wait for the next tile's loads before this one's reads.
-  auto arrived = [&]() __attribute__((always_inline)) {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0x0070);   // vmcnt(0), lgkmcnt(0)
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-  };
-
-  if (t0 < t1) {
-    const std::integral_constant<int, 0> first;
-    const std::integral_constant<int, 1> second;
-    stage(t0, first);
-    for (int t = t0; t < t1; t += 2) {
-      arrived();
-      if (t + 1 < t1) stage(t + 1, second);
-      compute(t, first);
-      if (t + 1 >= t1) break;
-      arrived();
-      if (t + 2 < t1) stage(t + 2, first);
-      compute(t + 1, second);
+    // The last product; then the wavefront only copies, and waits, for the
+    // others.
+    auto rest = [&](bool last, char* kfree, char* vp, char* vn) __attribute__((always_inline)) {
+      arrived(std::integral_constant<int, 0>{});
+      if (last) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+            o[d] = mfma_32x32x16<T>(value_operand(vp, u, d), pf[u], o[d]);
+      }
+      if (i < u1) {
+        copies(i, kfree, vn);
+        page = lookup(i + 3);
+      }
+      ++i;
+    };
+    const int stop = i;
+    while (i <= u1) {
+      if (((i - u0) & 1) == 0)
+        rest(i == stop && i > u0, k0, v1, v0);
+      else
+        rest(i == stop, k1, v0, v1);
     }
+    // No load into LDS outlives the workgroup.
+    __builtin_amdgcn_s_waitcnt(0x0f70);
   }
 
   l += __shfl_xor(l, 32);
@@ -551,7 +644,7 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) void prefill_kernel
       }
   }
   if (bad_rows != 0)
-    careful_rows<T, DP>(p, at, kvh, wave_row, bad_rows, t0 * kKeys, min(t1 * kKeys, at.keys), item,
+    careful_rows<T, DP>(p, at, kvh, wave_row, bad_rows, u0 * kKeys, min(u1 * kKeys, at.keys), item,
                         pieces == 1);
 }
 
@@ -566,7 +659,7 @@ __global__ __launch_bounds__(kJoinThreads) void prefill_join_kernel(PrefillParam
   const int tile = static_cast<int>(gridDim.x / a.kv_heads) - 1 - blockIdx.x / a.kv_heads;
   const Place at = find_tile(p, tile);
   if (at.seq < 0) return;
-  const int pieces = pieces_of(p, key_tiles(p, at));
+  const int pieces = pieces_of(p, key_units(p, at));
   if (pieces == 1) return;
   const int c = threadIdx.x % C;
   const int in_tile = blockIdx.y * R + threadIdx.x / C;
@@ -605,7 +698,7 @@ int64_t cut_of(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
                int64_t max_keys) {
   const int64_t items = max_tiles(tokens, batch, q_heads / kv_heads) * kv_heads;
   const int64_t room = kSlots / items;
-  const int64_t most = ceil_div(max_keys, kKeys) / kMinTiles;
+  const int64_t most = ceil_div(max_keys, kKeys) / kMinUnits;
   return std::max<int64_t>(1, std::min<int64_t>({room, most, kMaxCut}));
 }
 
@@ -614,7 +707,7 @@ int64_t pairs_bytes(int64_t rows) { return ceil_div(rows * 8, 256) * 256; }
 template <typename T, int DP>
 hipError_t launch_d(const PrefillParams& p, int64_t items, hipStream_t st) {
   const dim3 grid(static_cast<uint32_t>(items), static_cast<uint32_t>(p.cut));
-  const bool dma = (1 << p.a.page_shift) >= 512 / DP && p.a.c_tok < (1 << 24);
+  const bool dma = p.a.page_shift >= 3 && (p.a.c_tok << p.a.page_shift) < (int64_t{1} << 30);
   if (dma)
     hipLaunchKernelGGL((prefill_kernel<T, DP, true>), grid, dim3(64 * kWaves), 0, st, p);
   else
