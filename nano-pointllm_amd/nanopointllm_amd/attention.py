@@ -109,45 +109,56 @@ def rotary_frequencies(rotary_dim: int, *, base: float = 10000.0,
 
 
 # ------------------------------------------------------- checks and launches
-def _launch(name: str, device: torch.device, *args) -> None:
-    """``name(*args, stream)`` on the current stream of the tensors' device,
-    which is made the current device if it is not."""
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return _launch(name, device, *args)
-    _lib.check(getattr(_lib.load(), name)(*args, _lib.stream_handle(device)), name)
+# A decode step runs every call here once per layer, eagerly bounded by the
+# host: each wrapper reads an attribute once and compares devices by number
+# (8 of 15 us of a small call against general helpers).
+_CODES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 
 
-def _heads_rows(x: torch.Tensor, name: str) -> torch.Tensor:
-    """16-bit ``[tokens, heads, head_dim]`` rows with contiguous heads."""
-    if x.dim() != 3 or x.dtype not in (torch.float16, torch.bfloat16):
+def _gpu(*tensors: torch.Tensor | None) -> int:
+    """The number of the one GPU that the tensors are on."""
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != index or index < 0:
+            _lib.require_cuda(*tensors)    # raises, naming the reason
+    return index
+
+
+def _rows(x: torch.Tensor, name: str) -> int:
+    """The dtype code of 16-bit ``[tokens, heads, head_dim]`` rows."""
+    code = _CODES.get(x.dtype)
+    if code is None or x.dim() != 3:
         raise ValueError(f"{name} must be float16 / bfloat16 [tokens, heads, head_dim]")
-    return x if x.stride(2) == 1 or x.shape[2] <= 1 else x.contiguous()
+    return code
 
 
-def _out_rows(out: torch.Tensor | None, like: torch.Tensor) -> torch.Tensor:
+def _out_like(out: torch.Tensor | None, q: torch.Tensor) -> torch.Tensor:
     if out is None:
-        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
-    if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
+        return torch.empty_like(q, memory_format=torch.contiguous_format)
+    if out.shape != q.shape or out.dtype != q.dtype:
         raise ValueError("out must have the queries' shape, dtype and device")
     if out.stride(2) != 1 and out.shape[2] > 1:
         raise ValueError("out must have contiguous heads")
     return out
 
 
-def _check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, q: torch.Tensor) -> None:
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
+def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor, q: torch.Tensor, d: int
+           ) -> tuple[tuple[int, ...], tuple[int, ...]]:
+    """(shape, strides) of the two cache tensors."""
+    shape, strides = k_cache.shape, k_cache.stride()
+    if len(shape) != 4 or shape != v_cache.shape:
         raise ValueError("k_cache and v_cache must be [pages, kv_heads, page_size, head_dim]")
     if k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
         raise ValueError("the cache must have the rows' dtype")
-    if k_cache.shape[3] != q.shape[2]:
+    if shape[3] != d:
         raise ValueError("the cache and the rows must have one head_dim")
-    if k_cache.stride() != v_cache.stride() or k_cache.stride(3) != 1:
+    if strides != v_cache.stride() or strides[3] != 1:
         raise ValueError("k_cache and v_cache must have equal strides and contiguous heads")
+    return shape, strides
 
 
 def _index(t: torch.Tensor, dtype: torch.dtype, count: int, name: str) -> torch.Tensor:
-    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != count:
+    if t.dtype != dtype or t.shape != (count,):
         raise ValueError(f"{name} must be {str(dtype)[6:]} with {count} values")
     return t if t.is_contiguous() else t.contiguous()
 
@@ -177,17 +188,23 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *,
     ``attention_factor``; the rest of each head is copied.  ``layout``:
     ``"half"`` pairs elements ``(i, i + len(inv_freq))``, ``"interleaved"``
     neighbours.  ``out`` may be ``x`` itself."""
-    device = _lib.require_cuda(x, positions, inv_freq, out)
-    x = _heads_rows(x, "x") if out is not x else x
+    index = _gpu(x, positions, inv_freq, out)
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            return rotary(x, positions, inv_freq, layout=layout,
+                          attention_factor=attention_factor, out=out)
+    code = _rows(x, "x")
+    if out is not x and x.stride(2) != 1 and x.shape[2] > 1:
+        x = x.contiguous()
     t, h, d = x.shape
     positions = _index(positions, torch.int64, t, "positions")
     freq = _frequencies(inv_freq, d)
-    out = _out_rows(out, x)
-    _launch(
-        "w8a8_rotary", device,
-        x.data_ptr(), x.stride(0), x.stride(1), _lib.dtype_code(x.dtype),
-        positions.data_ptr(), freq.data_ptr(), 2 * freq.shape[0], _layout(layout),
-        attention_factor, out.data_ptr(), out.stride(0), out.stride(1), t, h, d)
+    out = _out_like(out, x)
+    xs, os = x.stride(), out.stride()
+    _lib.check(_lib.load().w8a8_rotary(
+        x.data_ptr(), xs[0], xs[1], code, positions.data_ptr(), freq.data_ptr(),
+        2 * freq.shape[0], _layout(layout), attention_factor, out.data_ptr(), os[0], os[1], t, h,
+        d, torch._C._cuda_getCurrentRawStream(index)), "w8a8_rotary")
     return out
 
 
@@ -201,30 +218,43 @@ def rotary_store(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: t
     ``slots[t] % page_size`` of page ``slots[t] // page_size`` (int64
     ``[tokens]``, distinct; a slot outside the cache, such as a padded row's
     -1, is not written).  q, k and v may be views of one packed matrix."""
-    device = _lib.require_cuda(q, k, v, positions, slots, inv_freq, k_cache, v_cache, out)
-    q = _heads_rows(q, "q") if out is not q else q
-    k, v = _heads_rows(k, "k"), _heads_rows(v, "v")
-    t, h, d = q.shape
-    g = k.shape[1]
-    if k.shape != v.shape or k.shape[0] != t or k.shape[2] != d:
-        raise ValueError("k and v must be [tokens, kv_heads, head_dim] rows of q's tokens")
-    if k.dtype != q.dtype or v.dtype != q.dtype:
+    index = _gpu(q, k, v, positions, slots, inv_freq, k_cache, v_cache, out)
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            return rotary_store(q, k, v, positions, slots, inv_freq, k_cache, v_cache,
+                                layout=layout, attention_factor=attention_factor, out=out)
+    code = _rows(q, "q")
+    if _rows(k, "k") != code or _rows(v, "v") != code:
         raise ValueError("q, k and v must have one dtype")
-    _check_cache(k_cache, v_cache, q)
-    if k_cache.shape[1] != g:
+    t, h, d = q.shape
+    shape = k.shape
+    if shape != v.shape or shape[0] != t or shape[2] != d:
+        raise ValueError("k and v must be [tokens, kv_heads, head_dim] rows of q's tokens")
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
+    if d > 1:
+        if qs[2] != 1 and out is not q:
+            q = q.contiguous()
+            qs = q.stride()
+        if ks[2] != 1:
+            k = k.contiguous()
+            ks = k.stride()
+        if vs[2] != 1:
+            v = v.contiguous()
+            vs = v.stride()
+    (pages, g, page_size, _), cs = _cache(k_cache, v_cache, q, d)
+    if g != shape[1]:
         raise ValueError("the cache and k must have the same heads")
     positions = _index(positions, torch.int64, t, "positions")
     slots = _index(slots, torch.int64, t, "slots")
     freq = _frequencies(inv_freq, d)
-    out = _out_rows(out, q)
-    cs = k_cache.stride()
-    _launch(
-        "w8a8_rotary_store", device,
-        q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-        v.data_ptr(), v.stride(0), v.stride(1), _lib.dtype_code(q.dtype), positions.data_ptr(),
-        slots.data_ptr(), freq.data_ptr(), 2 * freq.shape[0], _layout(layout), attention_factor,
-        out.data_ptr(), out.stride(0), out.stride(1), k_cache.data_ptr(), v_cache.data_ptr(),
-        cs[0], cs[1], cs[2], k_cache.shape[0], k_cache.shape[2], t, h, g, d)
+    out = _out_like(out, q)
+    os = out.stride()
+    _lib.check(_lib.load().w8a8_rotary_store(
+        q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], code,
+        positions.data_ptr(), slots.data_ptr(), freq.data_ptr(), 2 * freq.shape[0],
+        _layout(layout), attention_factor, out.data_ptr(), os[0], os[1], k_cache.data_ptr(),
+        v_cache.data_ptr(), cs[0], cs[1], cs[2], pages, page_size, t, h, g, d,
+        torch._C._cuda_getCurrentRawStream(index)), "w8a8_rotary_store")
     return out
 
 
@@ -242,21 +272,25 @@ def _prefill_workspace(tokens: int, batch: int, heads: int, kv_heads: int, dim: 
                                                               dim, max_keys))
 
 
-def _attention_rows(q: torch.Tensor) -> torch.Tensor:
+def _queries(q: torch.Tensor) -> tuple[torch.Tensor, tuple[int, ...]]:
     """Query rows whose addresses the kernels' 16-byte loads take."""
-    q = _heads_rows(q, "q")
-    if q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
+    strides = q.stride()
+    if strides[2] != 1 or strides[0] % 8 or strides[1] % 8 or q.data_ptr() % 16:
         q = q.contiguous()
-    return q
+        strides = q.stride()
+    return q, strides
 
 
-def _table(page_table: torch.Tensor, batch: int) -> torch.Tensor:
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != batch:
+def _table(page_table: torch.Tensor, batch: int) -> tuple[torch.Tensor, int, int]:
+    """(table, its row stride, pages per row)."""
+    shape = page_table.shape
+    if page_table.dtype != torch.int32 or len(shape) != 2 or shape[0] != batch:
         raise ValueError("page_table must be int32 [batch, pages of the longest sequence]")
-    if page_table.shape[1] > 1 and page_table.stride(1) != 1 \
-            or page_table.stride(0) < page_table.shape[1]:
+    strides = page_table.stride()
+    if strides[0] < shape[1] or strides[1] != 1 and shape[1] > 1:
         page_table = page_table.contiguous()
-    return page_table
+        strides = page_table.stride()
+    return page_table, max(strides[0], shape[1]), shape[1]
 
 
 def paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -269,24 +303,26 @@ def paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     table entries past a sequence's pages are not used.  ``heads`` is a
     multiple of the cache's heads, which consecutive queries share.  ``scale``
     defaults to ``head_dim ** -0.5``."""
-    device = _lib.require_cuda(q, k_cache, v_cache, page_table, lengths, out)
-    q = _attention_rows(q)
+    index = _gpu(q, k_cache, v_cache, page_table, lengths, out)
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            return paged_decode(q, k_cache, v_cache, page_table, lengths, scale=scale, out=out)
+    code = _rows(q, "q")
+    q, qs = _queries(q)
     b, h, d = q.shape
-    _check_cache(k_cache, v_cache, q)
-    pages, g, page_size, _ = k_cache.shape
-    page_table = _table(page_table, b)
+    (pages, g, page_size, _), cs = _cache(k_cache, v_cache, q, d)
+    page_table, ld, width = _table(page_table, b)
     lengths = _index(lengths, torch.int32, b, "lengths")
-    out = _out_rows(out, q)
-    need = _decode_workspace(b, h, g, d, page_table.shape[1] * page_size)
-    ws = torch.empty((need,), dtype=torch.uint8, device=device) if need > 0 else None
-    cs = k_cache.stride()
-    _launch(
-        "w8a8_paged_decode", device,
-        q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), cs[0],
-        cs[1], cs[2], pages, page_size, page_table.data_ptr(), page_table.stride(0),
-        page_table.shape[1], lengths.data_ptr(), _lib.dtype_code(q.dtype),
-        d ** -0.5 if scale is None else scale, out.data_ptr(), out.stride(0), out.stride(1), b, h,
-        g, d, None if ws is None else ws.data_ptr(), need)
+    out = _out_like(out, q)
+    os = out.stride()
+    need = _decode_workspace(b, h, g, d, width * page_size)
+    ws = q.new_empty(((need + 1) // 2,)) if need > 0 else None
+    _lib.check(_lib.load().w8a8_paged_decode(
+        q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2],
+        pages, page_size, page_table.data_ptr(), ld, width, lengths.data_ptr(), code,
+        d ** -0.5 if scale is None else scale, out.data_ptr(), os[0], os[1], b, h, g, d,
+        None if ws is None else ws.data_ptr(), need, torch._C._cuda_getCurrentRawStream(index)),
+        "w8a8_paged_decode")
     return out
 
 
@@ -300,26 +336,29 @@ def paged_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     last row sees all of them, each row before it one fewer; a row that sees
     none is zeros.  Rows of no sequence are not written (``out``'s keep what
     they hold).  Otherwise as :func:`paged_decode`."""
-    device = _lib.require_cuda(q, k_cache, v_cache, page_table, lengths, q_starts, out)
-    q = _attention_rows(q)
+    index = _gpu(q, k_cache, v_cache, page_table, lengths, q_starts, out)
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            return paged_prefill(q, k_cache, v_cache, page_table, lengths, q_starts, scale=scale,
+                                 out=out)
+    code = _rows(q, "q")
+    q, qs = _queries(q)
     t, h, d = q.shape
-    _check_cache(k_cache, v_cache, q)
-    pages, g, page_size, _ = k_cache.shape
+    (pages, g, page_size, _), cs = _cache(k_cache, v_cache, q, d)
     b = lengths.shape[0] if lengths.dim() == 1 else -1
-    page_table = _table(page_table, b)
+    page_table, ld, width = _table(page_table, b)
     lengths = _index(lengths, torch.int32, b, "lengths")
     q_starts = _index(q_starts, torch.int32, b + 1, "q_starts")
-    out = _out_rows(out, q)
-    need = _prefill_workspace(t, b, h, g, d, page_table.shape[1] * page_size)
-    ws = torch.empty((need,), dtype=torch.uint8, device=device) if need > 0 else None
-    cs = k_cache.stride()
-    _launch(
-        "w8a8_paged_prefill", device,
-        q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), cs[0],
-        cs[1], cs[2], pages, page_size, page_table.data_ptr(), page_table.stride(0),
-        page_table.shape[1], lengths.data_ptr(), q_starts.data_ptr(), _lib.dtype_code(q.dtype),
-        d ** -0.5 if scale is None else scale, out.data_ptr(), out.stride(0), out.stride(1), t, b,
-        h, g, d, None if ws is None else ws.data_ptr(), need)
+    out = _out_like(out, q)
+    os = out.stride()
+    need = _prefill_workspace(t, b, h, g, d, width * page_size)
+    ws = q.new_empty(((need + 1) // 2,)) if need > 0 else None
+    _lib.check(_lib.load().w8a8_paged_prefill(
+        q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2],
+        pages, page_size, page_table.data_ptr(), ld, width, lengths.data_ptr(),
+        q_starts.data_ptr(), code, d ** -0.5 if scale is None else scale, out.data_ptr(), os[0],
+        os[1], t, b, h, g, d, None if ws is None else ws.data_ptr(), need,
+        torch._C._cuda_getCurrentRawStream(index)), "w8a8_paged_prefill")
     return out
 
 
