@@ -42,7 +42,14 @@ namespace {
 constexpr int kTile = 32;            // keys of a wavefront's step
 constexpr int kWaves = 4;            // wavefronts of a workgroup
 constexpr int kMinTiles = 4;         // least tiles of a workgroup of several
+// Sequences up to here are not cut: joining costs a launch (300 keys, 10 tiles,
+// of 32 heads: 8.5 us whole, 5.5 + 4.4 us in pieces; 601 keys: 13 and 9.8 us).
+constexpr int kWholeTiles = 10;
 constexpr int kDecodeSlots = 768;    // workgroups aimed at
+// Keys and values past the last-level cache's 256 MB are loaded without being
+// kept in any (131071 keys of 8 heads: 89 against 95 us; 76 MB in 33 sequences:
+// 19 against 17.5).
+constexpr int64_t kCached = int64_t{256} << 20;
 constexpr int kJoinThreads = 256;
 constexpr int kJoinAhead = 4;        // rows a thread loads before the weights are known
 
@@ -59,9 +66,9 @@ struct DecodeParams {
 // Pieces that all sequences are cut into at most: each gets one, and the cut
 // itself adds at most slots / units.
 inline int64_t max_pieces(int64_t batch, int64_t units, int64_t max_keys) {
-  const int64_t whole = ceil_div(ceil_div(max_keys, kTile), kMinTiles);
+  const int64_t tiles = ceil_div(max_keys, kTile);
   const int64_t cut = batch + kDecodeSlots / units;
-  return whole <= 1 ? batch : std::min(cut, batch * whole);
+  return tiles <= kWholeTiles ? batch : std::min(cut, batch * ceil_div(tiles, kMinTiles));
 }
 
 struct Piece {
@@ -70,6 +77,7 @@ struct Piece {
   int count;   // its pieces
   int tiles;   // its tiles
   int keys;    // its keys
+  bool large;  // the batch's keys and values pass kCached
 };
 
 // The sequence of piece `slot`, or the pieces of sequence `seq` (slot < 0).
@@ -84,6 +92,7 @@ __device__ inline Piece find_piece(const DecodeParams& p, int slot, int seq) {
   int64_t total = static_cast<uint32_t>(lane_value(scan64(tiles_of(keys0)), 63));
   for (int b0 = 64; b0 < batch; b0 += 64)
     total += static_cast<uint32_t>(lane_value(scan64(tiles_of(keys_of(b0 + lane))), 63));
+  const bool large = total > kCached / (int64_t{4} * kTile * p.a.kv_heads * p.a.head_dim);
   total *= p.units;
   const int64_t share = min((total + kDecodeSlots - 1) / kDecodeSlots, int64_t{INT32_MAX / 2});
   const uint32_t cut = max(static_cast<uint32_t>(kMinTiles), static_cast<uint32_t>(share));
@@ -91,7 +100,8 @@ __device__ inline Piece find_piece(const DecodeParams& p, int slot, int seq) {
   for (int b0 = 0; b0 < batch; b0 += 64) {
     const int keys = b0 == 0 ? keys0 : keys_of(b0 + lane);
     const uint32_t tiles = tiles_of(keys);
-    const uint32_t count = b0 + lane < batch ? max(1u, (tiles + cut - 1) / cut) : 0u;
+    const uint32_t pieces = tiles <= kWholeTiles ? 1u : (tiles + cut - 1) / cut;
+    const uint32_t count = b0 + lane < batch ? pieces : 0u;
     const uint32_t upto = scan64(count);
     const bool mine = slot >= 0 ? before + static_cast<int>(upto) > slot : b0 + lane == seq;
     const uint64_t found = __ballot(mine);
@@ -99,11 +109,11 @@ __device__ inline Piece find_piece(const DecodeParams& p, int slot, int seq) {
       const int at = __ffsll(static_cast<unsigned long long>(found)) - 1;
       const int n = lane_value(count, at);
       return Piece{b0 + at, before + lane_value(upto, at) - n, n, lane_value(tiles, at),
-                   lane_value(static_cast<uint32_t>(keys), at)};
+                   lane_value(static_cast<uint32_t>(keys), at), large};
     }
     before += lane_value(upto, 63);
   }
-  return Piece{-1, 0, 0, 0, 0};
+  return Piece{-1, 0, 0, 0, 0, false};
 }
 
 template <typename T>
@@ -183,17 +193,23 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) void decode_kernel(
   auto row_of = [&](int e, int j) {
     return e >= 0 && e < pages ? e * a.c_page + (j & page_mask) * a.c_tok : int64_t{0};
   };
-  auto issue = [&](int t, const Entries& e, Tile& x) {
+  auto load = [](auto once, const auto* src) {
+    if constexpr (decltype(once)::value)
+      return __builtin_nontemporal_load(src);
+    else
+      return *src;
+  };
+  auto issue = [&](auto once, int t, const Entries& e, Tile& x) __attribute__((always_inline)) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const uint16_t* src = kb + row_of(e.k[h], t * kTile + 16 * h + r);
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         if constexpr (FULL) {
-          x.k[h][s] = *reinterpret_cast<const u32x4*>(src + 32 * s);
+          x.k[h][s] = load(once, reinterpret_cast<const u32x4*>(src + 32 * s));
         } else {
           x.k[h][s] = u32x4{0, 0, 0, 0};
-          if (live[s]) x.k[h][s] = *reinterpret_cast<const u32x4*>(src + 32 * s);
+          if (live[s]) x.k[h][s] = load(once, reinterpret_cast<const u32x4*>(src + 32 * s));
         }
       }
     }
@@ -206,7 +222,7 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) void decode_kernel(
       x.ok |= static_cast<uint32_t>(there) << i;
       const uint16_t* src = vb + row_of(there ? ev : -1, j);
       if constexpr (VW == 2) {
-        const u32x2 w = *reinterpret_cast<const u32x2*>(src);
+        const u32x2 w = load(once, reinterpret_cast<const u32x2*>(src));
         x.v[i][0] = w[0];
         x.v[i][1] = w[1];
       } else {
@@ -214,7 +230,7 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) void decode_kernel(
         for (int c = 0; c < VW; c += 4) {
           // head_dim is a multiple of 8: a lane's second half may lie past it.
           const int more = FULL || c == 0 || vd + 2 * c < D ? 2 * c : 0;
-          const u32x4 w = *reinterpret_cast<const u32x4*>(src + more);
+          const u32x4 w = load(once, reinterpret_cast<const u32x4*>(src + more));
 #pragma unroll
           for (int k = 0; k < 4; ++k) x.v[i][c + k] = w[k];
         }
@@ -228,7 +244,7 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) void decode_kernel(
   float ref = -INFINITY, l = 0.0f;
   const float sc = a.scale * kLog2e;
 
-  auto compute = [&](Tile& x) {
+  auto compute = [&](Tile& x) __attribute__((always_inline)) {
     f32x4 s0{0.0f, 0.0f, 0.0f, 0.0f}, s1 = s0;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
@@ -293,32 +309,36 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) void decode_kernel(
     }
   };
 
-  {
+  auto run = [&](auto once) __attribute__((always_inline)) {
     int t = t0 + wave;
     Entries e;
     Tile x0, x1;
     if (t < t1) {
       lookup(t, e);
-      issue(t, e, x0);
+      issue(once, t, e, x0);
       lookup(min(t + kWaves, t1 - 1), e);
     }
     while (t < t1) {
       const int tn = t + kWaves;
       if (tn < t1) {
-        issue(tn, e, x1);
+        issue(once, tn, e, x1);
         lookup(min(tn + kWaves, t1 - 1), e);
       }
       compute(x0);
       if (tn >= t1) break;
       const int tm = tn + kWaves;
       if (tm < t1) {
-        issue(tm, e, x0);
+        issue(once, tm, e, x0);
         lookup(min(tm + kWaves, t1 - 1), e);
       }
       compute(x1);
       t = tm;
     }
-  }
+  };
+  if (piece.large)
+    run(std::true_type{});
+  else
+    run(std::false_type{});
 
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);

@@ -1,6 +1,7 @@
 // extern "C" entry points of the attention core (declared in
 // include/w8a8_gfx950.h): argument checks and dispatch.  The kernels live in
-// rotary.hip and attention.hip.
+// rotary.hip, attention_decode.hip and
+// attention_prefill.hip.
 #include "w8a8_gfx950.h"
 #include "w8a8_internal.h"
 
@@ -240,6 +241,8 @@ int check_attention(PagedAttention& p, const void* q, int64_t q_st, int64_t q_sh
   if (tokens < 0 || tokens > kMaxTokens || batch < 0 || batch > kMaxTokens) return W8A8_ERR_SHAPE;
   if (q_heads <= 0 || q_heads > kMaxHeads || c.heads <= 0 || q_heads % c.heads)
     return W8A8_ERR_SHAPE;
+  // Rows of one key head are counted in 32 bits.
+  if (tokens * (q_heads / c.heads) > kMaxTokens) return W8A8_ERR_SHAPE;
   if (c.dim <= 0 || c.dim % 8 || c.dim > kAttentionMaxDim) return W8A8_ERR_SHAPE;
   if (!__builtin_isfinite(scale)) return W8A8_ERR_SHAPE;
   if (!strides_ok(q_st, q_sh) || !strides_ok(o_st, o_sh)) return W8A8_ERR_SHAPE;
@@ -293,6 +296,7 @@ bool sizes_ok(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, 
               int64_t max_keys) {
   return tokens >= 0 && tokens <= kMaxTokens && batch >= 0 && batch <= kMaxTokens &&
          q_heads > 0 && q_heads <= kMaxHeads && kv_heads > 0 && q_heads % kv_heads == 0 &&
+         tokens * (q_heads / kv_heads) <= kMaxTokens &&
          head_dim > 0 && head_dim % 8 == 0 && head_dim <= kAttentionMaxDim && max_keys >= 0 &&
          max_keys <= kMaxTokens;
 }

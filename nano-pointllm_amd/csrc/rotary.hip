@@ -193,7 +193,7 @@ hipError_t launch_w(RotaryRows const& r, hipStream_t st) {
   p.magic_qk = multiplier(p.items_qk);
   p.magic_v = multiplier(p.items_v);
   p.total = (r.q_heads + r.kv_heads) * p.items_qk + r.kv_heads * p.items_v;
-  constexpr int IPT = 2;
+  constexpr int IPT = 1;
   const dim3 grid(static_cast<uint32_t>(r.tokens),
                   static_cast<uint32_t>(ceil_div(p.total, kThreads * IPT)));
   hipLaunchKernelGGL((rotary_kernel<T, HALF, W, IPT>), grid, dim3(kThreads), 0, st, p);

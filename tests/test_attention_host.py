@@ -196,6 +196,8 @@ def test_attention_refusals(call):
     assert call(page=24) == S and call(pages=-1) == S
     assert call(ld=3) == S and call(n=1 << 30, ld=1 << 30) == S
     assert call(b=-1) == S and call(scale=math.nan) == S
+    many = {"t": 1 << 24} if call is _prefill else {"b": 1 << 24}
+    assert call(h=256, g=1, **many) == S      # rows of one key head past 32 bits
     for name in ("q", "kc", "vc", "table", "lengths", "out"):
         assert call(**{name: None}) == N, name
     for name in ("q", "kc", "vc", "out"):

@@ -313,6 +313,43 @@ def test_sharp_and_flat_rows(cuda, dtype):
     check_attention(out, rows, k, v, table[2:3], n[2:3], starts, what="chunk")
 
 
+@pytest.mark.parametrize("below", [14, 20, 23, 26])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_small_probabilities_count(cuda, dtype, below):
+    """One key ahead of 90 thousand others by 2^below each: together they weigh
+    up to 5 times as much, or 0.1%.  With values of one the result is the sum
+    of the weights over itself, 1, whatever a weight's rounding, as long as
+    numerator and denominator hold the same weights; with the first value 0
+    and the others 1 it is their share."""
+    note(f"small probabilities {dtype} 2^-{below}")
+    n, d, page = 90001, 64, 64
+    k, v, table = paged(31, [n], 1, d, page, dtype, cuda, poison=False)
+    k.zero_()
+    v.fill_(1.0)
+    k[table[0, 0].long(), 0, 0, 0] = 1.0
+    q = torch.zeros(1, 1, d, dtype=dtype, device=cuda)
+    q[..., 0] = 16.0
+    scale = below * 0.6931471805599453 / 16.0
+    lengths = torch.tensor([n], dtype=torch.int32, device=cuda)
+    starts = torch.tensor([0, 1], dtype=torch.int32, device=cuda)
+    share = (n - 1) / (n - 1 + 2.0 ** below)
+    # Weights: r of the module's bound with D sum |q k| = 16 once, the 16-bit
+    # rounding of a weight 2 e (binary16 below 2^-14 of a scale of at least 1:
+    # 2^-25 absolute, of a weight of 2^(7 - below)), sums of n terms 2 n u.
+    step = half_step(dtype)
+    if dtype == torch.float16:
+        step = max(step, 2.0 ** -25 / 2.0 ** (7 - below))
+    rel = 2 * ((d + 12) * U * 16 * scale + 16 * U) + 2 * step + 2 * n * U
+    for name, out in (("decode", A.paged_decode(q, k, v, table, lengths, scale=scale)),
+                      ("prefill", A.paged_prefill(q, k, v, table, lengths, starts, scale=scale))):
+        assert (out.float() - 1.0).abs().max() <= half_step(dtype) + 2 * n * U, name
+    v[table[0, 0].long(), 0, 0] = 0.0
+    for name, out in (("decode", A.paged_decode(q, k, v, table, lengths, scale=scale)),
+                      ("prefill", A.paged_prefill(q, k, v, table, lengths, starts, scale=scale))):
+        err = (out.double() - share).abs().max()
+        assert err <= (rel + half_step(dtype)) * share, f"{name} {float(err)} of {share}"
+
+
 def test_infinities_and_nans_stay_where_they_are_seen(cuda):
     """A NaN or infinite value is seen by the rows at and after its token, and
     by no row before it; a NaN key likewise.  The other elements stay within
