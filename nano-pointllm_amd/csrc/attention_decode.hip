@@ -40,7 +40,6 @@ namespace w8a8 {
 namespace {
 
 constexpr int kTile = 32;            // keys of a wavefront's step
-constexpr int kWaves = 4;            // wavefronts of a workgroup
 constexpr int kMinTiles = 4;         // least tiles of a workgroup of several
 // Sequences up to here are not cut: joining costs a launch (300 keys, 10 tiles,
 // of 32 heads: 8.5 us whole, 5.5 + 4.4 us in pieces; 601 keys: 13 and 9.8 us).
@@ -50,6 +49,15 @@ constexpr int kDecodeSlots = 768;    // workgroups aimed at
 // kept in any (131071 keys of 8 heads: 89 against 95 us; 76 MB in 33 sequences:
 // 19 against 17.5).
 constexpr int64_t kCached = int64_t{256} << 20;
+// A batch that gives every CU a workgroup by itself is not cut while its
+// sequences may be no longer than this: nothing is joined then, and uneven
+// lengths leave CUs idle for little time (8 sequences of 636 to 1590 keys, 32
+// heads: 32 us against 32.5 + 4.1 us cut; of 400 to 4000: 75 against 60.4 + 4.6).
+// With fewer than two workgroups per CU they have 8 wavefronts, else 4 (32
+// sequences of 1000 keys, 256 workgroups: 17.4 against 20.4 us; 64 of 2000, 512
+// workgroups: 85 against 73).
+constexpr int64_t kCus = 256;
+constexpr int64_t kWholeKeys = 2048;
 constexpr int kJoinThreads = 256;
 constexpr int kJoinAhead = 4;        // rows a thread loads before the weights are known
 
@@ -59,6 +67,8 @@ struct DecodeParams {
   int blocks;      // blocks of 16 queries per key head
   int group;       // queries per key head
   int rows;        // query rows of a workgroup: min(group, 16)
+  bool whole;      // no sequence is cut
+  bool large;      // with whole: the batch's keys and values may pass kCached
   float* part_o;   // [pieces x units, rows, head_dim]
   f32x2* part_rl;  // [pieces x units, rows]
 };
@@ -67,6 +77,7 @@ struct DecodeParams {
 // itself adds at most slots / units.
 inline int64_t max_pieces(int64_t batch, int64_t units, int64_t max_keys) {
   const int64_t tiles = ceil_div(max_keys, kTile);
+  if (batch * units >= kCus && max_keys <= kWholeKeys) return batch;
   const int64_t cut = batch + kDecodeSlots / units;
   return tiles <= kWholeTiles ? batch : std::min(cut, batch * ceil_div(tiles, kMinTiles));
 }
@@ -88,6 +99,11 @@ __device__ inline Piece find_piece(const DecodeParams& p, int slot, int seq) {
   const int batch = p.a.batch;
   auto keys_of = [&](int b) { return b < batch ? max(0, min(p.a.lengths[b], p.a.max_keys)) : 0; };
   auto tiles_of = [](int keys) { return static_cast<uint32_t>(keys + kTile - 1) / kTile; };
+  if (p.whole) {
+    const int at = slot >= 0 ? slot : seq;
+    const int keys = max(0, min(p.a.lengths[at], p.a.max_keys));
+    return Piece{at, at, 1, static_cast<int>(tiles_of(keys)), keys, p.large};
+  }
   const int keys0 = keys_of(lane);
   int64_t total = static_cast<uint32_t>(lane_value(scan64(tiles_of(keys0)), 63));
   for (int b0 = 64; b0 < batch; b0 += 64)
@@ -125,14 +141,15 @@ __device__ inline void write_out(const DecodeParams& p, int seq, int head, int d
 
 // DP: head_dim rounded up to 64, 128 or 256; FULL: head_dim == DP.  SMALL:
 // pages of fewer than 4 keys, so that each key has a table entry of its own.
-template <typename T, int DP, bool FULL, bool SMALL>
-__global__ __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) void decode_kernel(DecodeParams p) {
+// W: wavefronts.
+template <typename T, int DP, bool FULL, bool SMALL, int W>
+__global__ __launch_bounds__(64 * W, DP == 256 ? 1 : 2) void decode_kernel(DecodeParams p) {
   constexpr int KS = DP / 32;   // first product: steps over the head
   constexpr int DV = DP / 16;   // elements of a value row per lane
   constexpr int VW = DV / 2;    // ... dwords
   constexpr int NV = SMALL ? 8 : 2;  // table entries of a lane's 8 values
-  __shared__ float red_o[kWaves][16][DP];
-  __shared__ float red_r[kWaves][16], red_l[kWaves][16];
+  __shared__ float red_o[W][16][DP];
+  __shared__ float red_r[W][16], red_l[W][16];
 
   const PagedAttention& a = p.a;
   const int lane = threadIdx.x & 63;
@@ -140,7 +157,9 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) void decode_kernel(
   const int r = lane & 15, g = lane >> 4;
   const int slot = blockIdx.x / p.units, unit = blockIdx.x % p.units;
   const Piece piece = find_piece(p, slot, -1);
-  const int seq = piece.seq, count = piece.count, tiles = piece.tiles, keys = piece.keys;
+  const int seq = piece.seq, count = piece.count;
+  const int tiles = __builtin_amdgcn_readfirstlane(piece.tiles);
+  const int keys = __builtin_amdgcn_readfirstlane(piece.keys);
   if (seq < 0) return;
   const int part = slot - piece.first;
   const int t0 = static_cast<int>(static_cast<int64_t>(tiles) * part / count);
@@ -316,20 +335,20 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) void decode_kernel(
     if (t < t1) {
       lookup(t, e);
       issue(once, t, e, x0);
-      lookup(min(t + kWaves, t1 - 1), e);
+      lookup(min(t + W, t1 - 1), e);
     }
     while (t < t1) {
-      const int tn = t + kWaves;
+      const int tn = t + W;
       if (tn < t1) {
         issue(once, tn, e, x1);
-        lookup(min(tn + kWaves, t1 - 1), e);
+        lookup(min(tn + W, t1 - 1), e);
       }
       compute(x0);
       if (tn >= t1) break;
-      const int tm = tn + kWaves;
+      const int tm = tn + W;
       if (tm < t1) {
         issue(once, tm, e, x0);
-        lookup(min(tm + kWaves, t1 - 1), e);
+        lookup(min(tm + W, t1 - 1), e);
       }
       compute(x1);
       t = tm;
@@ -355,16 +374,16 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) void decode_kernel(
   }
   __syncthreads();
   const int64_t item = blockIdx.x;
-  for (int n = threadIdx.x; n < rows * DP; n += 64 * kWaves) {
+  for (int n = threadIdx.x; n < rows * DP; n += 64 * W) {
     const int q = n / DP, d = n % DP;
     if (!FULL && d >= D) continue;
     float top = red_r[0][q];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) top = fmaxf(top, red_r[w][q]);
+    for (int w = 1; w < W; ++w) top = fmaxf(top, red_r[w][q]);
     const float base = top == -INFINITY ? 0.0f : top;
     float ov = 0.0f, lv = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < W; ++w) {
       const float f = exp2_hw(red_r[w][q] - base);
       ov += red_o[w][q][d] * f;
       lv += red_l[w][q] * f;
@@ -453,11 +472,16 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(DecodeParams p) {
 
 template <typename T, int DP, bool FULL>
 hipError_t launch_d(const DecodeParams& p, int64_t pieces, hipStream_t st) {
-  const dim3 grid(static_cast<uint32_t>(pieces * p.units)), block(64 * kWaves);
-  if (p.a.page_shift < 2)
-    hipLaunchKernelGGL((decode_kernel<T, DP, FULL, true>), grid, block, 0, st, p);
+  const dim3 grid(static_cast<uint32_t>(pieces * p.units));
+  const bool small = p.a.page_shift < 2;
+  // Heads past 128 take too many registers for two wavefronts of a SIMD.
+  if (DP <= 128 && !small && p.whole && grid.x < 2 * kCus)
+    hipLaunchKernelGGL((decode_kernel<T, DP, FULL, false, DP <= 128 ? 8 : 4>), grid,
+                       dim3(64 * (DP <= 128 ? 8 : 4)), 0, st, p);
+  else if (small)
+    hipLaunchKernelGGL((decode_kernel<T, DP, FULL, true, 4>), grid, dim3(256), 0, st, p);
   else
-    hipLaunchKernelGGL((decode_kernel<T, DP, FULL, false>), grid, block, 0, st, p);
+    hipLaunchKernelGGL((decode_kernel<T, DP, FULL, false, 4>), grid, dim3(256), 0, st, p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || pieces == p.a.batch) return e;
   hipLaunchKernelGGL((join_kernel<T, DP>), dim3(p.a.batch, p.a.q_heads), dim3(kJoinThreads), 0, st,
@@ -503,6 +527,8 @@ hipError_t launch_paged_decode(const PagedAttention& a, int dtype, hipStream_t s
   p.rows = std::min(p.group, 16);
   const int64_t pieces = max_pieces(a.batch, p.units, a.max_keys);
   if (pieces * p.units > INT32_MAX) return hipErrorInvalidConfiguration;
+  p.whole = pieces == a.batch;
+  p.large = int64_t{4} * a.batch * a.max_keys * a.kv_heads * a.head_dim > kCached;
   char* ws = static_cast<char*>(a.workspace);
   p.part_rl = reinterpret_cast<f32x2*>(ws);
   p.part_o = reinterpret_cast<float*>(ws + pairs_bytes(pieces * p.units, p.rows));

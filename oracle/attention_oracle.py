@@ -31,13 +31,12 @@ def keys_of(cache, table, b, head, n):
     """The first n rows of sequence b's pages, and which of them lie in a page
     of the cache."""
     pages, _, page, dim = cache.shape
-    rows = torch.zeros(n, dim, dtype=torch.float64)
-    known = torch.zeros(n, dtype=torch.bool)
-    for j in range(n):
-        p = int(table[b, j // page])
-        if 0 <= p < pages:
-            rows[j], known[j] = cache[p, head, j % page].double(), True
-    return rows, known
+    if n == 0 or pages == 0:
+        return torch.zeros(n, dim, dtype=torch.float64), torch.zeros(n, dtype=torch.bool)
+    own = table[b, :-(-n // page)].long()
+    known = ((own >= 0) & (own < pages)).repeat_interleave(page)[:n]
+    rows = cache[own.clamp(0, pages - 1), head].flatten(0, 1)[:n].double()
+    return rows.masked_fill(~known[:, None], 0.0), known
 
 
 def attention(q, k_cache, v_cache, table, lengths, q_starts=None, scale=None):

@@ -234,6 +234,32 @@ def test_decode_against_the_definition(cuda, h, g, d, page, lengths, dtype):
     assert torch.equal(into[:, :h], out) and (into[:, h] == 7.0).all()
 
 
+@pytest.mark.parametrize("batch,h,g,d,page,longest", [
+    (130, 2, 2, 128, 16, 400),     # a workgroup of 8 wavefronts per sequence and head
+    (260, 2, 2, 64, 64, 300),      # ... of 4
+    (70, 34, 2, 96, 8, 500),       # blocks of 16 queries of one key head
+    (129, 4, 2, 80, 2, 333),       # pages smaller than a lane's four keys
+    (65, 4, 4, 256, 32, 400),      # wide heads
+    (37, 8, 8, 128, 16, 2500),     # cut, each sequence by its length
+])
+def test_decode_of_large_batches(cuda, batch, h, g, d, page, longest):
+    """Batches with a workgroup for every CU, lengths of zero and one among
+    them."""
+    note(f"decode batch {batch} {h} {g} {d} {page} {longest}")
+    r = gen_of(batch)
+    lengths = torch.randint(0, longest, (batch,), generator=r).tolist()
+    lengths[0], lengths[1], lengths[2] = longest, 0, 1
+    for dtype in DTYPES:
+        k, v, table = paged(batch + d, lengths, g, d, page, dtype, cuda)
+        q = randn(r, batch, h, d, dtype=dtype, device=cuda, std=1.7)
+        n = torch.tensor(lengths, dtype=torch.int32, device=cuda)
+        out = A.paged_decode(q, k, v, table, n)
+        check_attention(out, q, k, v, table, n)
+        # The last ten by themselves, cut otherwise.
+        few = A.paged_decode(q[-10:], k, v, table[-10:], n[-10:])
+        check_attention(few, q[-10:], k, v, table[-10:], n[-10:])
+
+
 PREFILL = [
     # heads, kv heads, dim, page, new tokens, lengths
     (4, 4, 128, 16, [560], [560]),
