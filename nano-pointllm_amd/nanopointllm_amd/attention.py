@@ -223,24 +223,21 @@ def rotary_store(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: t
         with torch.cuda.device(index):
             return rotary_store(q, k, v, positions, slots, inv_freq, k_cache, v_cache,
                                 layout=layout, attention_factor=attention_factor, out=out)
-    code = _rows(q, "q")
-    if _rows(k, "k") != code or _rows(v, "v") != code:
+    code = _CODES.get(q.dtype)
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
+    if code is None or not len(qs) == len(ks) == len(vs) == 3:
+        raise ValueError("q, k and v must be float16 / bfloat16 [tokens, heads, head_dim]")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError("q, k and v must have one dtype")
     t, h, d = q.shape
     shape = k.shape
     if shape != v.shape or shape[0] != t or shape[2] != d:
         raise ValueError("k and v must be [tokens, kv_heads, head_dim] rows of q's tokens")
-    qs, ks, vs = q.stride(), k.stride(), v.stride()
-    if d > 1:
-        if qs[2] != 1 and out is not q:
+    if not qs[2] == ks[2] == vs[2] == 1 and d > 1:
+        if out is not q:
             q = q.contiguous()
-            qs = q.stride()
-        if ks[2] != 1:
-            k = k.contiguous()
-            ks = k.stride()
-        if vs[2] != 1:
-            v = v.contiguous()
-            vs = v.stride()
+        k, v = k.contiguous(), v.contiguous()
+        qs, ks, vs = q.stride(), k.stride(), v.stride()
     (pages, g, page_size, _), cs = _cache(k_cache, v_cache, q, d)
     if g != shape[1]:
         raise ValueError("the cache and k must have the same heads")

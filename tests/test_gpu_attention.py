@@ -441,6 +441,71 @@ def test_lengths_past_the_table_are_cut(cuda):
                        A.paged_prefill(q, k, v, table, cut, starts))
 
 
+def test_refusals_of_gpu_tensors(cuda):
+    """Shapes, dtypes and layouts that no kernel may see."""
+    note("refusals")
+    q = torch.zeros(3, 4, 64, dtype=torch.float16, device=cuda)
+    kv = torch.zeros(3, 2, 64, dtype=torch.float16, device=cuda)
+    c = torch.zeros(5, 2, 16, 64, dtype=torch.float16, device=cuda)
+    c2 = torch.zeros_like(c)
+    i64 = torch.zeros(3, dtype=torch.int64, device=cuda)
+    n = torch.ones(3, dtype=torch.int32, device=cuda)
+    table = torch.zeros(3, 2, dtype=torch.int32, device=cuda)
+    starts = torch.arange(4, dtype=torch.int32, device=cuda)
+    freq = A.rotary_frequencies(64, device=cuda).inv_freq
+
+    def store(q=q, k=kv, v=kv, positions=i64, slots=i64, freq=freq, kc=c, vc=c2, **kw):
+        return A.rotary_store(q, k, v, positions, slots, freq, kc, vc, **kw)
+
+    def decode(q=q, kc=c, vc=c2, table=table, n=n, **kw):
+        return A.paged_decode(q, kc, vc, table, n, **kw)
+
+    def prefill(q=q, kc=c, vc=c2, table=table, n=n, starts=starts, **kw):
+        return A.paged_prefill(q, kc, vc, table, n, starts, **kw)
+
+    turned = q.transpose(1, 2).contiguous().transpose(1, 2)    # heads not contiguous
+    refused = [
+        lambda: store(q=q.float()), lambda: store(q=q[0]), lambda: store(k=kv.bfloat16()),
+        lambda: store(k=kv[:2]), lambda: store(v=kv[:, :1]), lambda: store(k=kv[..., :32]),
+        lambda: store(positions=i64.int()), lambda: store(slots=i64[:2]),
+        lambda: store(freq=freq.float()), lambda: store(freq=torch.cat((freq, freq))),
+        lambda: store(layout="spiral"), lambda: store(kc=c.bfloat16()), lambda: store(vc=c2[:4]),
+        lambda: store(kc=c[:, :1], vc=c2[:, :1]), lambda: store(vc=c), lambda: store(out=q[:2]),
+        lambda: store(vc=c2.transpose(1, 2).contiguous().transpose(1, 2)),
+        lambda: store(q=turned, out=turned), lambda: store(out=kv.repeat(1, 2, 1).bfloat16()),
+        lambda: store(attention_factor=float("inf")),
+        lambda: A.rotary(turned, i64, freq, out=turned), lambda: A.rotary(q, i64[:1], freq),
+        lambda: A.rotary(q, i64, freq, out=q.float()),
+    ]
+    for call in (decode, prefill):
+        refused += [
+            lambda call=call: call(q=q.float()), lambda call=call: call(q=q[..., :32]),
+            lambda call=call: call(q=q[:, :3]), lambda call=call: call(kc=c.float(), vc=c2.float()),
+            lambda call=call: call(table=table.long()), lambda call=call: call(table=table[:2]),
+            lambda call=call: call(n=n.long()), lambda call=call: call(n=n[:2]),
+            lambda call=call: call(out=q), lambda call=call: call(out=q[:2].clone()),
+            lambda call=call: call(scale=float("nan")), lambda call=call: call(vc=c2[..., :32]),
+            lambda call=call: call(kc=c[:, :, :12], vc=c2[:, :, :12]),
+        ]
+    refused += [lambda: prefill(starts=starts[:3]), lambda: prefill(starts=starts.long()),
+                lambda: prefill(n=n.reshape(3, 1))]
+    for at, call in enumerate(refused):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"refusal {at} was accepted")
+    for call in (store, decode, prefill):
+        with pytest.raises(RuntimeError, match="only on the GPU"):
+            call(q=q.cpu())
+        with pytest.raises(RuntimeError, match="only on the GPU"):
+            call(vc=c2.cpu())
+    assert not c.any() and not c2.any()
+    # What the checks make contiguous is taken: rows with scattered elements, a
+    # transposed table, lengths of every second place.
+    assert torch.equal(store(q=turned), store())
+    wide = torch.ones(6, dtype=torch.int32, device=cuda)
+    assert torch.equal(decode(n=wide[::2], table=table.T.contiguous().T), decode())
+
+
 def test_empty_calls(cuda):
     note("empty")
     k, v, table = paged(7, [64], 2, 64, 16, torch.float16, cuda)
