@@ -256,13 +256,15 @@ __device__ inline void careful_rows(const PrefillParams& p, const Place& at, int
   }
 }
 
-// DP: head_dim rounded up to 64, 128 or 256.  DMA: pages of at least 8 keys,
-// the part of a unit that a wavefront copies; else each chunk is copied through
-// registers.
-template <typename T, int DP, bool DMA>
+// DU: head_dim rounded up to 64, 96, 128 or 256, what the products run over (4096
+// tokens of 32 heads of 96 elements: 136 us, over 128 elements 157); DP: the
+// power of two that a key's row takes in LDS.  DMA: pages of at least 8
+// keys, the part of a unit that a wavefront copies; else each chunk is copied
+// through registers.
+template <typename T, int DP, int DU, bool DMA>
 __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) void prefill_kernel(PrefillParams p) {
-  constexpr int KS = DP / 16;               // first product: steps over the head
-  constexpr int DT = DP / 32;               // second product: row tiles of O^T
+  constexpr int KS = DU / 16;               // first product: steps over the head
+  constexpr int DT = DU / 32;               // second product: row tiles of O^T
   constexpr int RB = DP * 2;                // bytes of a key's row
   constexpr int RL = 1024 / RB;             // keys of a load
   constexpr int NL = kKeys / RL / kWaves;   // loads per wavefront, unit and operand
@@ -555,26 +557,22 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) void prefill_kernel
         }
       }
       const float base = ref == -INFINITY ? 0.0f : -ref;
-      constexpr int E = 16 / KS;   // probabilities per matrix instruction
 #pragma unroll
       for (int n = 0; n < 16; ++n) next[n] = 0.0f;
       __builtin_amdgcn_sched_barrier(0);
+      // Behind matrix instruction k the scores from 16 k / KS on become
+      // probabilities, and the pairs of the step before are rounded.
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
+      for (int k = 0; k <= KS; ++k) {
         if (k + DT < KS) kf[k + DT] = key_operand(kn, k + DT);
-        next = mfma_32x32x16<T>(kf[k], qf[k], next);
+        if (k < KS) next = mfma_32x32x16<T>(kf[k], qf[k], next);
 #pragma unroll
-        for (int e = 0; e < E; ++e) weight(s, k * E + e, base);
-        // The pairs of the step before.
+        for (int n = 16 * k / KS; n < 16 && n < 16 * (k + 1) / KS; ++n) weight(s, n, base);
 #pragma unroll
-        for (int n = (k - 1) * E; n < k * E; ++n)
-          if (n > 0 && (n & 1)) weights_of(s, n >> 1);
+        for (int n = 0; n < 16; ++n)
+          if (k > 0 && (n & 1) && n >= 16 * (k - 1) / KS && n < 16 * k / KS) weights_of(s, n >> 1);
         __builtin_amdgcn_sched_barrier(0);
       }
-#pragma unroll
-      for (int n = 16 - E; n < 16; ++n)
-        if (n & 1) weights_of(s, n >> 1);
-      __builtin_amdgcn_sched_barrier(0);
       page = lookup(i + 3);   // waited for with the next unit's copies
     };
     int i = u0;
@@ -717,14 +715,14 @@ int64_t cut_of(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
 
 int64_t pairs_bytes(int64_t rows) { return ceil_div(rows * 8, 256) * 256; }
 
-template <typename T, int DP>
+template <typename T, int DP, int DU>
 hipError_t launch_d(const PrefillParams& p, int64_t items, hipStream_t st) {
   const dim3 grid(static_cast<uint32_t>(items), static_cast<uint32_t>(p.cut));
   const bool dma = p.a.page_shift >= 3 && (p.a.c_tok << p.a.page_shift) < (int64_t{1} << 30);
   if (dma)
-    hipLaunchKernelGGL((prefill_kernel<T, DP, true>), grid, dim3(64 * kWaves), 0, st, p);
+    hipLaunchKernelGGL((prefill_kernel<T, DP, DU, true>), grid, dim3(64 * kWaves), 0, st, p);
   else
-    hipLaunchKernelGGL((prefill_kernel<T, DP, false>), grid, dim3(64 * kWaves), 0, st, p);
+    hipLaunchKernelGGL((prefill_kernel<T, DP, DU, false>), grid, dim3(64 * kWaves), 0, st, p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.cut == 1) return e;
   hipLaunchKernelGGL((prefill_join_kernel<T, DP>),
@@ -735,9 +733,10 @@ hipError_t launch_d(const PrefillParams& p, int64_t items, hipStream_t st) {
 
 template <typename T>
 hipError_t launch_t(const PrefillParams& p, int64_t items, hipStream_t st) {
-  if (p.a.head_dim <= 64) return launch_d<T, 64>(p, items, st);
-  if (p.a.head_dim <= 128) return launch_d<T, 128>(p, items, st);
-  return launch_d<T, 256>(p, items, st);
+  if (p.a.head_dim <= 64) return launch_d<T, 64, 64>(p, items, st);
+  if (p.a.head_dim <= 96) return launch_d<T, 128, 96>(p, items, st);
+  if (p.a.head_dim <= 128) return launch_d<T, 128, 128>(p, items, st);
+  return launch_d<T, 256, 256>(p, items, st);
 }
 
 }  // namespace
