@@ -488,7 +488,10 @@ int w8a8_dense_gemv(const void* x, int64_t ldx, const void* w, int64_t ldw, cons
  * product are taken as they are.  head_dim is a multiple of 8, at most 256.
  * A cache is two tensors of equal shape [pages, kv_heads, page_size, head_dim]
  * and equal strides (elements; head_dim contiguous, the other axes in any
- * order); page_size is a power of two up to 2^20.  Offsets are 64-bit.
+ * order); page_size is a power of two up to 2^20.  Offsets are 64-bit.  Each
+ * call launches fewer than 2^24 workgroups (else W8A8_ERR_SHAPE): rotary one or
+ * more per token, attention kv_heads x (tokens x q_heads / kv_heads / R + batch)
+ * with R = 16 (decode) or 128 (prefill).
  */
 
 /*

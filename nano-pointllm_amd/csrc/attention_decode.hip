@@ -526,9 +526,8 @@ hipError_t launch_paged_decode(const PagedAttention& a, int dtype, hipStream_t s
   p.units = a.kv_heads * p.blocks;
   p.rows = std::min(p.group, 16);
   const int64_t pieces = max_pieces(a.batch, p.units, a.max_keys);
-  if (pieces * p.units > INT32_MAX) return hipErrorInvalidConfiguration;
   p.whole = pieces == a.batch;
-  p.large = int64_t{4} * a.batch * a.max_keys * a.kv_heads * a.head_dim > kCached;
+  p.large = 4.0 * a.batch * a.max_keys * a.kv_heads * a.head_dim > static_cast<double>(kCached);
   char* ws = static_cast<char*>(a.workspace);
   p.part_rl = reinterpret_cast<f32x2*>(ws);
   p.part_o = reinterpret_cast<float*>(ws + pairs_bytes(pieces * p.units, p.rows));

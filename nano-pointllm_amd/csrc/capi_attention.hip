@@ -1,7 +1,6 @@
 // extern "C" entry points of the attention core (declared in
 // include/w8a8_gfx950.h): argument checks and dispatch.  The kernels live in
-// rotary.hip, attention_decode.hip and
-// attention_prefill.hip.
+// rotary.hip, attention_decode.hip and attention_prefill.hip.
 #include "w8a8_gfx950.h"
 #include "w8a8_internal.h"
 
@@ -18,6 +17,8 @@ inline bool half_dtype(int d) { return d == kF16 || d == kBF16; }
 
 constexpr int64_t kMaxTokens = INT32_MAX - 4096;
 constexpr int64_t kMaxHeads = 4096;
+// Workgroups of 256 threads; a launch's threads are counted in 32 bits.
+constexpr int64_t kMaxBlocks = UINT32_MAX / 256;
 constexpr int64_t kMaxStride = int64_t{1} << 60;
 constexpr i128 kMaxBytes = i128(1) << 62;  // of any tensor's address range
 
@@ -141,7 +142,7 @@ int w8a8_rotary_store(const void* q, int64_t q_stride_t, int64_t q_stride_h, con
                       int64_t head_dim, hipStream_t stream) {
   if (!half_dtype(dtype)) return W8A8_ERR_DTYPE;
   if (layout != W8A8_ROTARY_HALF && layout != W8A8_ROTARY_INTERLEAVED) return W8A8_ERR_DTYPE;
-  if (tokens < 0 || tokens > kMaxTokens || q_heads < 0 || q_heads > kMaxHeads || kv_heads < 0 ||
+  if (tokens < 0 || tokens > kMaxBlocks || q_heads < 0 || q_heads > kMaxHeads || kv_heads < 0 ||
       kv_heads > kMaxHeads)
     return W8A8_ERR_SHAPE;
   if (head_dim <= 0 || head_dim % 8 || head_dim > kRotaryMaxDim) return W8A8_ERR_SHAPE;
@@ -230,19 +231,28 @@ int w8a8_rotary_store(const void* q, int64_t q_stride_t, int64_t q_stride_h, con
 
 namespace {
 
+// Whether rows and workgroups stay inside what a launch counts: of each key
+// head's rows, counted in 32 bits, a workgroup takes `rows`, of one sequence; a
+// cut over the keys adds at most 1024 workgroups.
+bool counts_ok(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, int rows) {
+  if (tokens < 0 || tokens > kMaxTokens || batch < 0 || batch > kMaxTokens || q_heads <= 0 ||
+      q_heads > kMaxHeads || kv_heads <= 0 || q_heads % kv_heads)
+    return false;
+  const int64_t group_rows = tokens * (q_heads / kv_heads);
+  return group_rows <= kMaxTokens &&
+         kv_heads * (group_rows / rows + batch + 1) <= kMaxBlocks - 1024;
+}
+constexpr int kDecodeRows = 16, kPrefillRows = 128;
+
 // The checks that both attention entry points share; fills p but for
 // q_starts and the workspace.
 int check_attention(PagedAttention& p, const void* q, int64_t q_st, int64_t q_sh,
                     const void* k_cache, const void* v_cache, const Cache& c,
                     const int32_t* table, int64_t ld_table, int64_t table_pages,
                     const int32_t* lengths, int dtype, float scale, void* out, int64_t o_st,
-                    int64_t o_sh, int64_t tokens, int64_t batch, int64_t q_heads) {
+                    int64_t o_sh, int64_t tokens, int64_t batch, int64_t q_heads, int rows) {
   if (!half_dtype(dtype)) return W8A8_ERR_DTYPE;
-  if (tokens < 0 || tokens > kMaxTokens || batch < 0 || batch > kMaxTokens) return W8A8_ERR_SHAPE;
-  if (q_heads <= 0 || q_heads > kMaxHeads || c.heads <= 0 || q_heads % c.heads)
-    return W8A8_ERR_SHAPE;
-  // Rows of one key head are counted in 32 bits.
-  if (tokens * (q_heads / c.heads) > kMaxTokens) return W8A8_ERR_SHAPE;
+  if (!counts_ok(tokens, batch, q_heads, c.heads, rows)) return W8A8_ERR_SHAPE;
   if (c.dim <= 0 || c.dim % 8 || c.dim > kAttentionMaxDim) return W8A8_ERR_SHAPE;
   if (!__builtin_isfinite(scale)) return W8A8_ERR_SHAPE;
   if (!strides_ok(q_st, q_sh) || !strides_ok(o_st, o_sh)) return W8A8_ERR_SHAPE;
@@ -293,12 +303,9 @@ int check_attention(PagedAttention& p, const void* q, int64_t q_st, int64_t q_sh
 }
 
 bool sizes_ok(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
-              int64_t max_keys) {
-  return tokens >= 0 && tokens <= kMaxTokens && batch >= 0 && batch <= kMaxTokens &&
-         q_heads > 0 && q_heads <= kMaxHeads && kv_heads > 0 && q_heads % kv_heads == 0 &&
-         tokens * (q_heads / kv_heads) <= kMaxTokens &&
-         head_dim > 0 && head_dim % 8 == 0 && head_dim <= kAttentionMaxDim && max_keys >= 0 &&
-         max_keys <= kMaxTokens;
+              int64_t max_keys, int rows) {
+  return counts_ok(tokens, batch, q_heads, kv_heads, rows) && head_dim > 0 && head_dim % 8 == 0 &&
+         head_dim <= kAttentionMaxDim && max_keys >= 0 && max_keys <= kMaxTokens;
 }
 
 }  // namespace
@@ -307,7 +314,7 @@ extern "C" {
 
 int64_t w8a8_paged_decode_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads,
                                           int64_t head_dim, int64_t max_keys) {
-  if (!sizes_ok(batch, batch, q_heads, kv_heads, head_dim, max_keys)) return -1;
+  if (!sizes_ok(batch, batch, q_heads, kv_heads, head_dim, max_keys, kDecodeRows)) return -1;
   return paged_decode_workspace(batch, q_heads, kv_heads, head_dim, max_keys);
 }
 
@@ -324,7 +331,7 @@ int w8a8_paged_decode(const void* q, int64_t q_stride_t, int64_t q_stride_h, con
   PagedAttention p;
   const int rc = check_attention(p, q, q_stride_t, q_stride_h, k_cache, v_cache, c, page_table,
                                  ld_table, table_pages, lengths, dtype, scale, out, out_stride_t,
-                                 out_stride_h, batch, batch, q_heads);
+                                 out_stride_h, batch, batch, q_heads, kDecodeRows);
   if (rc != W8A8_OK || batch == 0) return rc;
   const int64_t need = paged_decode_workspace(batch, q_heads, kv_heads, head_dim, p.max_keys);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return W8A8_ERR_WORKSPACE;
@@ -337,7 +344,7 @@ int w8a8_paged_decode(const void* q, int64_t q_stride_t, int64_t q_stride_h, con
 int64_t w8a8_paged_prefill_workspace_bytes(int64_t tokens, int64_t batch, int64_t q_heads,
                                            int64_t kv_heads, int64_t head_dim,
                                            int64_t max_keys) {
-  if (!sizes_ok(tokens, batch, q_heads, kv_heads, head_dim, max_keys)) return -1;
+  if (!sizes_ok(tokens, batch, q_heads, kv_heads, head_dim, max_keys, kPrefillRows)) return -1;
   return paged_prefill_workspace(tokens, batch, q_heads, kv_heads, head_dim, max_keys);
 }
 
@@ -354,7 +361,7 @@ int w8a8_paged_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, co
   PagedAttention p;
   const int rc = check_attention(p, q, q_stride_t, q_stride_h, k_cache, v_cache, c, page_table,
                                  ld_table, table_pages, lengths, dtype, scale, out, out_stride_t,
-                                 out_stride_h, tokens, batch, q_heads);
+                                 out_stride_h, tokens, batch, q_heads, kPrefillRows);
   if (rc != W8A8_OK || tokens == 0 || batch == 0) return rc;
   if (q_starts == nullptr) return W8A8_ERR_NULL;
   if (!aligned(q_starts, 4)) return W8A8_ERR_ALIGN;

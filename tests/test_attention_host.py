@@ -170,6 +170,22 @@ def test_rotary_store_refusals():
     assert _store(t=0, q=None, out=None) == _lib.OK
 
 
+def test_more_rows_than_a_launch_takes():
+    """A launch's threads are counted in 32 bits: 2^24 workgroups of 256 are one
+    too many."""
+    many, S = 1 << 24, _lib.ERR_SHAPE
+    assert _store(t=many) == S
+    assert _lib.load().w8a8_rotary(Q, 8, 8, _lib.F16, AUX, AUX, 8, 0, 1.0, OUT, 8, 8, many, 1, 8,
+                                   None) == S
+    row = {"d": 8, "cs": (256, 128, 8), "qs": (8, 8), "os": (8, 8), "h": 1, "g": 1}
+    assert _decode(b=many, **row) == S and _prefill(t=5, b=many, **row) == S
+    assert _decode(b=1 << 20, **{**row, "h": 32, "g": 32, "os": (256, 8)}) == S
+    assert _prefill(t=1 << 27, **{**row, "h": 32, "g": 32, "os": (256, 8)}) == S
+    lib = _lib.load()
+    assert lib.w8a8_paged_decode_workspace_bytes(many, 1, 1, 8, 64) == -1
+    assert lib.w8a8_paged_prefill_workspace_bytes(1 << 27, 1, 32, 32, 8, 64) == -1
+
+
 def _decode(*, q=Q, qs=(256, 64), kc=KC, vc=VC, cs=(2048, 1024, 64), pages=4, page=16, table=AUX,
             ld=4, n=4, lengths=AUX, dtype=_lib.F16, scale=0.125, out=OUT, os=(256, 64), b=3, h=4,
             g=2, d=64, ws=WS, wb=1 << 30):
