@@ -327,7 +327,8 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) void prefill_kernel
   }
   // A wavefront copies eight keys of a unit.  DMA: they lie in one page, whose
   // place (of keys and of values) is formed once, in scalar registers; rows
-  // past the sequence's last key and of unknown pages arrive as zeros.
+  // past the sequence's last key and of unknown pages arrive as zeros (unless
+  // the cache's rows share elements: masked all the same).
   const int first_key = wave * (kKeys / kWaves);
   struct Source {
     int64_t offset;   // elements
@@ -341,7 +342,7 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) void prefill_kernel
     const int left = at.keys - key;
     const bool known = left > 0 && static_cast<uint32_t>(page) < static_cast<uint32_t>(pages);
     return Source{known ? page * a.c_page + (key & page_mask) * ctok : int64_t{0},
-                  known ? (left < 8 ? left : 8) * (2 * ctok) : 0};
+                  known ? ((left < 8 ? left : 8) - 1) * (2 * ctok) + 2 * D : 0};
   };
   auto copy = [&](int u, const Source& src, const uint16_t* cache, const int (&off)[NL],
                   char* dst, auto is_key) __attribute__((always_inline)) {
@@ -756,7 +757,6 @@ hipError_t launch_paged_prefill(const PagedAttention& a, int dtype, hipStream_t 
   p.group = a.q_heads / a.kv_heads;
   p.cut = static_cast<int>(cut_of(a.tokens, a.batch, a.q_heads, a.kv_heads, a.max_keys));
   const int64_t items = max_tiles(a.tokens, a.batch, p.group) * a.kv_heads;
-  if (items > INT32_MAX) return hipErrorInvalidConfiguration;
   char* ws = static_cast<char*>(a.workspace);
   p.part_rl = reinterpret_cast<f32x2*>(ws);
   p.part_o = reinterpret_cast<float*>(ws + pairs_bytes(items * p.cut * kRows));

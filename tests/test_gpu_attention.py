@@ -426,6 +426,28 @@ def test_pages_outside_the_cache_are_masked(cuda):
     check_attention(A.paged_prefill(q, k, v, table, n, starts), q, k, v, table, n, starts)
 
 
+@pytest.mark.parametrize("page", [4, 16])
+def test_caches_that_share_rows(cuda, page):
+    """A cache that repeats one row, one head or one page by a stride of zero is
+    read as its copy is."""
+    note(f"shared rows {page}")
+    g, d, lengths = 2, 64, [3 * page, 2 * page - 3]
+    table = torch.tensor([[2, 0, 1], [1, 2, 0]], dtype=torch.int32, device=cuda)
+    n = torch.tensor(lengths, dtype=torch.int32, device=cuda)
+    new = [7, 2]
+    starts = torch.tensor([0, 7, 9], dtype=torch.int32, device=cuda)
+    r = gen_of(31)
+    for shape in ((3, g, 1, d), (3, 1, page, d), (1, g, page, d), (1, 1, 1, d)):
+        k, v = (randn(r, *shape, dtype=torch.float16, device=cuda).expand(3, g, page, d)
+                for _ in range(2))
+        whole = k.contiguous(), v.contiguous()
+        q = randn(r, 2, 4, d, dtype=torch.float16, device=cuda)
+        assert torch.equal(A.paged_decode(q, k, v, table, n), A.paged_decode(q, *whole, table, n))
+        q = randn(r, sum(new), 4, d, dtype=torch.float16, device=cuda)
+        out = A.paged_prefill(q, k, v, table, n, starts)
+        check_attention(out, q, *whole, table, n, starts, what=f"{shape}")
+
+
 def test_lengths_past_the_table_are_cut(cuda):
     note("long lengths")
     k, v, table = paged(7, [64, 64], 2, 64, 16, torch.float16, cuda)
