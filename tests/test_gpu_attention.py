@@ -272,6 +272,11 @@ PREFILL = [
     # few rows far into a long context
     (8, 2, 128, 64, [3], [5000]), (4, 4, 64, 16, [40, 1], [3333, 2000]),
     (2, 1, 128, 16, [300], [4400]),
+    # many sequences; row tiles of uneven prompts by their keys; more than 2048
+    # workgroups
+    (8, 1, 64, 16, [1 + 7 * i % 41 for i in range(70)], [1 + 11 * i % 60 for i in range(70)]),
+    (16, 2, 96, 32, [200, 0, 77, 31, 130], [200, 40, 500, 31, 300]),
+    (128, 128, 8, 16, [900, 350, 600], [900, 700, 590]),
 ]
 
 
