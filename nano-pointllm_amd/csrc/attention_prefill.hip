@@ -6,30 +6,38 @@
 // r per row (Reference in attention_common.h), rounded to 16 bits; O^T = V^T P
 // and l = sum P over the rounded values; the result is O / l.
 //
-// Bound by the matrix units and the exponentials together: per 64 keys and 32
-// rows of 128 elements a wavefront issues 32 matrix instructions of 32 cycles
-// and about as many cycles of vector work.
+// Bound by the matrix units and the exponentials together: per 32 keys and 32
+// rows of 128 elements a wavefront issues 16 matrix instructions of 32 cycles
+// and 400 to 450 cycles of vector work, which run side by side only as far as
+// the order of the instructions lets them.  8192 tokens of 32 heads: 0.59 to
+// 0.60 ms, 0.92 PFLOP/s, 77% of what a large matrix product reaches; the matrix
+// units are busy 47% of the time and the vector units 40%, at a clock that this
+// load holds at 1.9 to 2.0 GHz.  LDS is busy for a quarter of the time, so
+// copying ahead by three units instead of one changes nothing, and neither does
+// a barrier for every second unit only.
 //
 // Design:
 //   * A workgroup takes 128 rows of one key head, 32 per wavefront, held in
 //     registers; the queries that share a key head are packed as rows, so a
-//     short chunk fills its tiles and every key is read once per 128 rows.
+//     short chunk fills its tiles and every key is read once per 128 rows.  Two
+//     workgroups share a CU: alone one takes 0.77 us per unit, two 1.2 us for
+//     one each.
 //   * Units of 32 keys and of 32 values pass through double buffers in LDS,
 //     filled by LDS-DMA buffer loads straight from the pages, a unit ahead of
-//     their use: one descriptor per load, whose range ends at the
-//     sequence's last key, so what lies behind it arrives as zeros.  16-byte
-//     chunks are permuted by key (in the source address), which leaves the
-//     reads of both operands without bank conflicts.
+//     their use: a wavefront forms one descriptor per operand and unit, whose
+//     range ends at the sequence's last key, so what lies behind it arrives as
+//     zeros.  16-byte chunks are permuted by key (in the source address), which
+//     leaves the reads of both operands without bank conflicts.
 //   * While a unit's scores become probabilities on the vector unit, the
-//     matrix unit forms the next one's scores and the product of the one
-//     before with its values: neither waits for the other.
+//     matrix unit forms the next one's scores; the product of the unit before
+//     with its values comes first, with the operands of both read ahead.
 //   * The score tile's registers are the second product's operand as they
 //     are: its inner index is summed over, so the values are read (transposing
 //     ds_read_b64_tr_b16) in the key order that the scores have.
 //   * Masks are formed for the units that a row of the wavefront sees in part,
 //     the last ones; the others have none.
 //   * Few rows far into a long cache are cut over its length: each piece
-//     leaves (O, r, l) in the workspace and join_kernel adds them up.
+//     leaves (O, r, l) in the workspace and prefill_join_kernel adds them up.
 //   * A masked key's probability is 0, but 0 times an infinite or NaN value is
 //     NaN.  Such values are not searched for: a row whose sums are not finite
 //     is computed again by careful_rows, key by key.
@@ -51,8 +59,11 @@ typedef const int32_t __attribute__((address_space(4))) const_i32;   // scalar l
 constexpr int kKeys = 32;            // keys of a unit
 constexpr int kWaves = 4;
 constexpr int kRows = 32 * kWaves;   // rows of a workgroup
-constexpr int kSlots = 512;          // workgroups below which the keys are cut
-constexpr int kMinUnits = 16;        // least units of a piece
+// Below so many workgroups (two per CU) the keys are cut, into pieces of at
+// least 16 units: a join costs 4 to 9 us (512 tokens behind 7680, 32 heads over 8:
+// 80 + 9 us in 4 pieces, 96 + 8 in 3, 188 whole).
+constexpr int kSlots = 512;
+constexpr int kMinUnits = 16;
 constexpr int kMaxCut = 32;
 // Up to so many workgroups the longest go first: 7 prompts of 100 to 1000 keys,
 // 840 workgroups, take 54 us instead of 60, 12 of 450 to 700, 836 workgroups, 41
@@ -748,9 +759,9 @@ __global__ __launch_bounds__(kJoinThreads) void prefill_join_kernel(PrefillParam
       u32x2{pack2_bits<T>(o[0] * inv, o[1] * inv), pack2_bits<T>(o[2] * inv, o[3] * inv)};
 }
 
-// Row tiles of a call at most.
+// Row tiles of a call at most: each sequence's last one may lack kRows - 1 rows.
 int64_t max_tiles(int64_t tokens, int64_t batch, int64_t group) {
-  return ceil_div(tokens * group, kRows) + batch;
+  return (tokens * group + batch * (kRows - 1)) / kRows;
 }
 
 // Pieces of a row tile: as many as the slots ask for that the tiles leave
