@@ -65,8 +65,8 @@ constexpr int kRows = 32 * kWaves;   // rows of a workgroup
 constexpr int kSlots = 512;
 constexpr int kMinUnits = 16;
 constexpr int kMaxCut = 32;
-// Up to so many workgroups the longest go first: 7 prompts of 100 to 1000 keys,
-// 840 workgroups, take 54 us instead of 60, 12 of 450 to 700, 836 workgroups, 41
+// Up to so many workgroups the longest go first: 7 prompts of 40 to 777 tokens,
+// 840 workgroups, take 54 us instead of 60, 12 of 420 to 655, 836 workgroups, 41
 // instead of 47.  More of them even out by themselves, and read less when a
 // sequence's run together (12 chunks of 40 heads, 5360 workgroups: 870 us by
 // sequence, 1165 sorted).
@@ -341,8 +341,8 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) void prefill_kernel
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 31, h = lane >> 5;
-  // Consecutive workgroups, key heads here, go to the eight dies in turn (a die's workgroups on one head at a time
-  // instead, for its L2, measures the same).
+  // Consecutive workgroups, key heads here, go to the eight dies in turn (a die's
+  // workgroups on one head at a time instead, for its L2, measures the same).
   const int kvh = blockIdx.x % a.kv_heads;
   const Place at = find_tile(p, blockIdx.x / a.kv_heads);
   if (at.seq < 0) return;

@@ -299,7 +299,9 @@ def paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     ``lengths`` int32 ``[batch]``; a length of zero (a padded row) gives zeros,
     table entries past a sequence's pages are not used.  ``heads`` is a
     multiple of the cache's heads, which consecutive queries share.  ``scale``
-    defaults to ``head_dim ** -0.5``."""
+    defaults to ``head_dim ** -0.5``.  A NaN or infinite value among a row's
+    keys makes the elements that it enters NaN or infinite, one behind its
+    length does nothing."""
     index = _gpu(q, k_cache, v_cache, page_table, lengths, out)
     if index != torch._C._cuda_getDevice():
         with torch.cuda.device(index):

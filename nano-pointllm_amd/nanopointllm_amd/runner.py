@@ -15,8 +15,8 @@ with the quantization of its output:
    is the same numbers, since quantization is per token and per output row).
    Every route sums the norm's squares in the same order, so a row's result
    does not depend on the batch it runs in;
-3. the attention core, supplied by the caller (rotary, KV cache and the
-   attention kernel are not part of the W8A8 path):
+3. the attention core (rotary, KV cache and attention),
+   :class:`nanopointllm_amd.attention.PagedAttentionCore` or the caller's own:
    ``core(q [T, H, D], k [T, Hkv, D], v [T, Hkv, D], layer_index, state)``
    returns the context ``[T, H * D]``;
 4. ``o_proj`` as a W8A8 linear (paged_attention.py:1376, 1488);
