@@ -61,9 +61,15 @@ constexpr int kWaves = 4;
 constexpr int kRows = 32 * kWaves;   // rows of a workgroup
 // Below so many workgroups (two per CU) the keys are cut, into pieces of at
 // least 16 units: a join costs 4 to 9 us (512 tokens behind 7680, 32 heads over 8:
-// 80 + 9 us in 4 pieces, 96 + 8 in 3, 188 whole).
+// 80 + 9 us in 4 pieces, 188 whole).
 constexpr int kSlots = 512;
 constexpr int kMinUnits = 16;
+// While there is no workgroup for every CU, into pieces of 8 units and more, from
+// 24 units on (4 tokens behind 4000, 32 heads over 8: 13 + 4 us, in pieces of 16
+// 19 + 4; 19 units: 13 + 4 cut, 19 whole, less than a second launch saves).
+constexpr int kCus = 256;
+constexpr int kFewUnits = 8;
+constexpr int kWholeUnits = 24;
 constexpr int kMaxCut = 32;
 // Up to so many workgroups the longest go first: 7 prompts of 40 to 777 tokens,
 // 840 workgroups, take 54 us instead of 60, 12 of 420 to 655, 836 workgroups, 41
@@ -74,11 +80,13 @@ constexpr int kSortedItems = 2048;
 constexpr int kOutside = 0x7ffffff0;   // a buffer offset past every range
 constexpr int kBufferWord3 = 0x00020000;
 constexpr int kJoinThreads = 256;
+constexpr int kJoinAhead = 8;          // pieces that a thread of the join has in flight
 
 struct PrefillParams {
   PagedAttention a;
   int group;           // query heads per key head
   int cut;             // most pieces of a row tile
+  int few;             // ... of kFewUnits and more
   bool sorted;         // row tiles go by the keys they see, at most 64 sequences
   float* part_o;       // [row tiles x kv_heads x cut, kRows, head_dim]
   f32x2* part_rl;      // [row tiles x kv_heads x cut, kRows]
@@ -190,7 +198,8 @@ __device__ inline int key_units(const PrefillParams& p, const Place& at) {
   return (max(seen, 0) + kKeys - 1) / kKeys;
 }
 __device__ inline int pieces_of(const PrefillParams& p, int units) {
-  return max(1, min(p.cut, units / kMinUnits));
+  const int few = units < kWholeUnits ? 1 : min(p.few, units / kFewUnits);
+  return max(few, min(p.cut, units / kMinUnits));
 }
 
 template <typename T>
@@ -259,11 +268,12 @@ __device__ inline T* out_row(const PagedAttention& a, int start, int token, int 
 
 // The rows of `bad` (bit c: row c of the wavefront's 32), key by key: lane i
 // holds elements i, i + 64, ... of the head.  Masked and unknown keys are not
-// read.
+// read.  Rare, so kept simple: 2048 tokens of 32 heads that all see a NaN take 42
+// ms (64 keys at a time, 23 ms).
 template <typename T, int DP>
 __device__ inline void careful_rows(const PrefillParams& p, const Place& at, int kvh,
-                                          int wave_row, uint32_t bad, int k0, int k1,
-                                          int64_t item, bool whole) {
+                                    int wave_row, uint32_t bad, int k0, int k1, int64_t item,
+                                    bool whole) {
   constexpr int N = DP / 64;
   const PagedAttention& a = p.a;
   const int lane = threadIdx.x & 63;
@@ -722,7 +732,8 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) void prefill_kernel
 }
 
 // Adds up the pieces of a row tile that was cut: four elements of a row per
-// thread.
+// thread, kJoinAhead pieces of them in flight (32 pieces of 16 rows and 8 key
+// heads: 6.0 us, one after the other 13.4).
 template <typename T, int DP>
 __global__ __launch_bounds__(kJoinThreads) void prefill_join_kernel(PrefillParams p) {
   constexpr int C = DP / 4;             // threads of a row
@@ -737,21 +748,47 @@ __global__ __launch_bounds__(kJoinThreads) void prefill_join_kernel(PrefillParam
   const int in_tile = blockIdx.y * R + threadIdx.x / C;
   const int row = at.row0 + in_tile;
   const int D = a.head_dim;
-  if (in_tile >= kRows || row >= at.count * p.group || 4 * c >= D) return;
+  if (in_tile >= kRows || row >= at.count * p.group) return;
   const int64_t r0 = static_cast<int64_t>(blockIdx.x) * p.cut * kRows + in_tile;
+  // Thread c of a row weighs pieces c, c + C, ...
+  constexpr int M = (kMaxCut + C - 1) / C;
+  f32x2 rl[M];
   float top = -INFINITY;
-  for (int i = 0; i < pieces; ++i) top = fmaxf(top, p.part_rl[r0 + i * kRows][0]);
-  const float base = top == -INFINITY ? 0.0f : top;
-  float l = 0.0f;
-  f32x4 o{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-  for (int i = 0; i < pieces; ++i) {
-    const int64_t r = r0 + i * kRows;
-    const f32x2 rl = p.part_rl[r];
-    const float f = exp2_hw(rl[0] - base);
-    l += rl[1] * f;
-    o += *reinterpret_cast<const f32x4*>(p.part_o + r * D + 4 * c) * f;
+#pragma unroll
+  for (int m = 0; m < M; ++m) {
+    rl[m] = f32x2{-INFINITY, 0.0f};
+    if (c + m * C < pieces) rl[m] = p.part_rl[r0 + (c + m * C) * kRows];
+    top = fmaxf(top, rl[m][0]);
   }
+#pragma unroll
+  for (int w = 1; w < C; w <<= 1) top = fmaxf(top, __shfl_xor(top, w));
+  const float base = top == -INFINITY ? 0.0f : top;
+  float weight[M], l = 0.0f;
+#pragma unroll
+  for (int m = 0; m < M; ++m) {
+    weight[m] = exp2_hw(rl[m][0] - base);
+    l += rl[m][1] * weight[m];
+  }
+#pragma unroll
+  for (int w = 1; w < C; w <<= 1) l += __shfl_xor(l, w);
+  const float* src = p.part_o + r0 * D + 4 * c;
+  const int64_t step = static_cast<int64_t>(kRows) * D;
+  const bool inside = 4 * c < D;
+  f32x4 o{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+    for (int i0 = m * C; i0 < min(pieces, (m + 1) * C); i0 += kJoinAhead) {
+      f32x4 x[kJoinAhead];
+#pragma unroll
+      for (int k = 0; k < kJoinAhead; ++k) {
+        x[k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (inside && i0 + k < pieces)
+          x[k] = *reinterpret_cast<const f32x4*>(src + (i0 + k) * step);
+      }
+#pragma unroll
+      for (int k = 0; k < kJoinAhead; ++k) o += x[k] * __shfl(weight[m], i0 + k, C);
+    }
+  if (!inside) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   const int token = divide_rows(row, p.group);
   T* dst = out_row<T>(a, at.start, token, kvh * p.group + row - token * p.group) + 4 * c;
@@ -764,14 +801,17 @@ int64_t max_tiles(int64_t tokens, int64_t batch, int64_t group) {
   return (tokens * group + batch * (kRows - 1)) / kRows;
 }
 
-// Pieces of a row tile: as many as the slots ask for that the tiles leave
-// empty.
-int64_t cut_of(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
-               int64_t max_keys) {
-  const int64_t items = max_tiles(tokens, batch, q_heads / kv_heads) * kv_heads;
-  const int64_t room = kSlots / items;
+// Pieces of a row tile at most: of kMinUnits while two workgroups per CU are not
+// there, of kFewUnits while one is not (few).
+int64_t few_of(int64_t items, int64_t max_keys) {
+  if (ceil_div(max_keys, kKeys) < kWholeUnits) return 1;
+  return std::max<int64_t>(
+      1, std::min<int64_t>({kCus / items, ceil_div(max_keys, kKeys) / kFewUnits, kMaxCut}));
+}
+int64_t cut_of(int64_t items, int64_t max_keys) {
   const int64_t most = ceil_div(max_keys, kKeys) / kMinUnits;
-  return std::max<int64_t>(1, std::min<int64_t>({room, most, kMaxCut}));
+  return std::max(few_of(items, max_keys),
+                  std::min<int64_t>({kSlots / items, most, kMaxCut}));
 }
 
 int64_t pairs_bytes(int64_t rows) { return ceil_div(rows * 8, 256) * 256; }
@@ -805,9 +845,10 @@ hipError_t launch_t(const PrefillParams& p, int64_t items, hipStream_t st) {
 int64_t paged_prefill_workspace(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
                                 int64_t head_dim, int64_t max_keys) {
   if (tokens == 0 || batch == 0) return 0;
-  const int64_t cut = cut_of(tokens, batch, q_heads, kv_heads, max_keys);
+  const int64_t items = max_tiles(tokens, batch, q_heads / kv_heads) * kv_heads;
+  const int64_t cut = cut_of(items, max_keys);
   if (cut == 1) return 0;
-  const int64_t rows = max_tiles(tokens, batch, q_heads / kv_heads) * kv_heads * cut * kRows;
+  const int64_t rows = items * cut * kRows;
   return pairs_bytes(rows) + rows * head_dim * 4;
 }
 
@@ -815,8 +856,9 @@ hipError_t launch_paged_prefill(const PagedAttention& a, int dtype, hipStream_t 
   PrefillParams p;
   p.a = a;
   p.group = a.q_heads / a.kv_heads;
-  p.cut = static_cast<int>(cut_of(a.tokens, a.batch, a.q_heads, a.kv_heads, a.max_keys));
   const int64_t items = max_tiles(a.tokens, a.batch, p.group) * a.kv_heads;
+  p.cut = static_cast<int>(cut_of(items, a.max_keys));
+  p.few = static_cast<int>(few_of(items, a.max_keys));
   p.sorted = a.batch <= 64 && items <= kSortedItems;
   char* ws = static_cast<char*>(a.workspace);
   p.part_rl = reinterpret_cast<f32x2*>(ws);

@@ -277,6 +277,8 @@ PREFILL = [
     (8, 1, 64, 16, [1 + 7 * i % 41 for i in range(70)], [1 + 11 * i % 60 for i in range(70)]),
     (16, 2, 96, 32, [200, 0, 77, 31, 130], [200, 40, 500, 31, 300]),
     (128, 128, 8, 16, [900, 350, 600], [900, 700, 590]),
+    # a token's queries over more than one row tile
+    (200, 1, 64, 16, [3, 0, 70], [40, 9, 70]),
 ]
 
 
