@@ -3,15 +3,18 @@
 //
 // Mathematics.  Rows (token, query head of one key head) are the columns of
 // S^T = K Q^T; P = 2^(S^T c - r) with c = scale log2(e) and a running reference
-// r per row (Reference in attention_common.h), rounded to 16 bits; O^T = V^T P
-// and l = sum P over the rounded values; the result is O / l.
+// r per row (Reference in attention_common.h), rounded to the rows' type; O^T =
+// V^T P and l = sum P over the rounded values; the result is O / l.  The rounding
+// of P is the one that is not forced: half a step each, independent of each other
+// and the same in O and l, it leaves 1.3 to 1.4 times the error of the rounded
+// result alone, where P in two parts would double the second product.
 //
 // Bound by the matrix units and the exponentials together: per 32 keys and 32
 // rows of 128 elements a wavefront issues 16 matrix instructions of 32 cycles
 // and 400 to 450 cycles of vector work, which run side by side only as far as
 // the order of the instructions lets them.  8192 tokens of 32 heads: 0.59 to
 // 0.60 ms, 0.92 PFLOP/s, 77% of what a large matrix product reaches; the matrix
-// units are busy 47% of the time and the vector units 40%, at a clock that this
+// units are busy 46% of the time and the vector units 42%, at a clock that this
 // load holds at 1.9 to 2.0 GHz.  LDS is busy for a quarter of the time, so
 // copying ahead by three units instead of one changes nothing, and neither does
 // a barrier for every second unit only.
