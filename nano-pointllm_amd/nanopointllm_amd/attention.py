@@ -47,6 +47,50 @@ class RotaryFrequencies(NamedTuple):
     attention_factor: float   # amplitude of cos and sin
 
 
+# The keys of a scaling dictionary that each kind needs, and those that it may
+# have besides its name and the base.
+_SCALING_KEYS = {
+    "default": ((), ("factor",)),
+    "linear": (("factor",), ()),
+    "ntk": (("factor",), ()),
+    "llama3": (("factor", "original_max_position_embeddings", "low_freq_factor",
+                "high_freq_factor"), ()),
+    "yarn": (("factor", "original_max_position_embeddings"),
+             ("beta_fast", "beta_slow", "truncate", "attention_factor", "mscale",
+              "mscale_all_dim")),
+}
+
+
+def _scaling_of(scaling: dict[str, Any] | None, base: float) -> tuple[str, dict[str, Any]]:
+    """(kind, its values as numbers); a key of None is one left out."""
+    given = {k: v for k, v in (scaling or {}).items() if v is not None}
+    kind = given.pop("rope_type", given.get("type", "default"))
+    if given.pop("type", kind) != kind:
+        raise ValueError("rope_type and type of the rotary scaling differ")
+    if kind not in _SCALING_KEYS:
+        raise ValueError(f"unknown rotary scaling {kind!r}")
+    if given.pop("rope_theta", base) != base:
+        raise ValueError("rope_theta of the rotary scaling is not the given base")
+    needed, optional = _SCALING_KEYS[kind]
+    for key in needed:
+        if key not in given:
+            raise ValueError(f"{kind} rotary scaling needs {key}")
+    for key, value in given.items():
+        if key not in needed + optional:
+            raise ValueError(f"{kind} rotary scaling does not use {key}")
+        if key == "truncate":
+            if not isinstance(value, bool):
+                raise ValueError("truncate of the rotary scaling must be a truth value")
+            continue
+        try:
+            given[key] = float(value)
+        except (TypeError, ValueError):
+            given[key] = math.nan
+        if not 0.0 < given[key] < math.inf:
+            raise ValueError(f"{key} of the rotary scaling must be a positive number")
+    return kind, given
+
+
 def rotary_frequencies(rotary_dim: int, *, base: float = 10000.0,
                        scaling: dict[str, Any] | None = None,
                        device: torch.device | str = "cuda") -> RotaryFrequencies:
@@ -62,21 +106,25 @@ def rotary_frequencies(rotary_dim: int, *, base: float = 10000.0,
     * ``"llama3"``: frequencies whose wavelength is past
       ``original_max_position_embeddings / low_freq_factor`` divided by
       ``factor``, those below ``.../high_freq_factor`` kept, blended between;
-    * ``"yarn"``: blended by the number of turns over the original context
-      (``beta_fast``, ``beta_slow``), with the amplitude
-      ``attention_factor`` (default ``0.1 ln(factor) + 1``).
-    """
+    * ``"yarn"``: blended by the number of turns over
+      ``original_max_position_embeddings``, from ``beta_fast`` (32) to
+      ``beta_slow`` (1), the pairs of both as whole numbers outwards unless
+      ``truncate`` is False; with the amplitude ``attention_factor``, else
+      ``s(mscale) / s(mscale_all_dim)`` where both are given, else ``s(1)``, of
+      ``s(m) = 0.1 m ln(factor) + 1``.
+
+    A key that is missing, or that the kind does not use, is refused, and so
+    is a ``rope_theta`` that is not ``base``."""
     if rotary_dim < 0 or rotary_dim % 2:
         raise ValueError("rotary_dim must be even")
-    if not base > 0:
+    if not 0 < base < math.inf:
         raise ValueError("the rotary base must be positive")
-    scaling = dict(scaling or {})
-    kind = scaling.get("rope_type", scaling.get("type", "default"))
-    factor = float(scaling.get("factor", 1.0))
-    if kind not in ("default", "linear", "ntk", "llama3", "yarn"):
-        raise ValueError(f"unknown rotary scaling {kind!r}")
+    kind, given = _scaling_of(scaling, base)
+    factor = given.get("factor", 1.0)
     if not factor >= 1.0:
         raise ValueError("the rotary scaling factor must be at least 1")
+    if kind == "default" and factor != 1.0:
+        raise ValueError("unscaled rotary frequencies do not use factor")
     d = rotary_dim
     if kind == "ntk" and d > 2:
         base = base * factor ** (d / (d - 2))
@@ -86,25 +134,39 @@ def rotary_frequencies(rotary_dim: int, *, base: float = 10000.0,
     if kind == "linear":
         freq = freq / factor
     elif kind == "llama3":
-        context = float(scaling["original_max_position_embeddings"])
-        low, high = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
-        if not 0 < low < high:
+        context = given["original_max_position_embeddings"]
+        low, high = given["low_freq_factor"], given["high_freq_factor"]
+        if not low < high:
             raise ValueError("llama3 scaling needs 0 < low_freq_factor < high_freq_factor")
         kept = ((context * freq / (2 * math.pi) - low) / (high - low)).clamp(0.0, 1.0)
         freq = freq * (kept + (1.0 - kept) / factor)
-    elif kind == "yarn" and d:
-        context = float(scaling["original_max_position_embeddings"])
+    elif kind == "yarn":
+        context = given["original_max_position_embeddings"]
+        fast, slow = given.get("beta_fast", 32.0), given.get("beta_slow", 1.0)
+        if fast < slow:
+            raise ValueError("yarn scaling needs beta_slow <= beta_fast")
+        if not base > 1.0:
+            raise ValueError("yarn scaling needs a rotary base above 1")
 
         def pair_of(turns: float) -> float:   # the pair that turns so often in the context
             return d * math.log(context / (turns * 2 * math.pi)) / (2 * math.log(base))
 
-        low = max(math.floor(pair_of(float(scaling.get("beta_fast", 32.0)))), 0)
-        high = min(math.ceil(pair_of(float(scaling.get("beta_slow", 1.0)))), d - 1)
+        low, high = pair_of(fast), pair_of(slow)
+        if given.get("truncate", True):
+            low, high = math.floor(low), math.ceil(high)
+        low, high = max(low, 0), min(high, d - 1)
         slowed = ((i - low) / (high - low if high != low else 0.001)).clamp(0.0, 1.0)
         freq = freq * (1.0 - slowed + slowed / factor)
-    if kind == "yarn":
-        amplitude = scaling.get("attention_factor")
-        amplitude = 0.1 * math.log(factor) + 1.0 if amplitude is None else float(amplitude)
+
+        def size(m: float) -> float:
+            return 0.1 * m * math.log(factor) + 1.0
+
+        if ("mscale" in given) != ("mscale_all_dim" in given):
+            raise ValueError("yarn scaling takes mscale and mscale_all_dim together")
+        amplitude = given.get("attention_factor")
+        if amplitude is None:
+            amplitude = (size(given["mscale"]) / size(given["mscale_all_dim"])
+                         if "mscale" in given else size(1.0))
     return RotaryFrequencies(freq.to(device), amplitude)
 
 
