@@ -332,10 +332,12 @@ def _prefill_workspace(tokens: int, batch: int, heads: int, kv_heads: int, dim: 
 
 
 def _queries(q: torch.Tensor) -> tuple[torch.Tensor, tuple[int, ...]]:
-    """Query rows whose addresses the kernels' 16-byte loads take."""
+    """Query rows whose addresses the kernels' 16-byte loads take: a copy where
+    q's are not (not by contiguous(), which returns a contiguous view at an odd
+    address, or of one row with a stride of its own, as it is)."""
     strides = q.stride()
     if strides[2] != 1 or strides[0] % 8 or strides[1] % 8 or q.data_ptr() % 16:
-        q = q.contiguous()
+        q = q.clone(memory_format=torch.contiguous_format)
         strides = q.stride()
     return q, strides
 

@@ -1,0 +1,41 @@
+"""Calls of the attention core that its documentation allows at the edges:
+addresses, tables, padded rows, values that are not finite.
+
+Tolerances as in test_gpu_attention.py where its check is used; others are
+derived at the test."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from nanopointllm_amd import attention as A
+from test_gpu_attention import DTYPES, check_attention, gen_of, note, paged, randn
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------ addresses and strides
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_queries_at_any_address_and_stride(cuda, dtype):
+    """A contiguous q at an odd element, and one row or one head of a stride
+    that is no multiple of 8, give the bits of an aligned copy."""
+    note(f"misaligned queries {dtype}")
+    h, g, d, lengths = 4, 2, 64, [300, 45]
+    k, v, table = paged(3, lengths, g, d, 16, dtype, cuda)
+    n = torch.tensor(lengths, dtype=torch.int32, device=cuda)
+    flat = randn(gen_of(4), 3 * h * d + 8, dtype=dtype, device=cuda)
+    wide = randn(gen_of(5), 3, h * d + 3, dtype=dtype, device=cuda)
+    cases = [(flat[i:i + 2 * h * d].view(2, h, d), slice(0, 2)) for i in (0, 1, 3, 4)]
+    cases += [(wide[:1, :h * d].view(1, h, d), slice(0, 1)),
+              (wide[1:2, 1:h * d + 1].view(1, h, d), slice(1, 2)),
+              (wide[:2, :h * d].view(2, h, d), slice(0, 2))]
+    for q, at in cases:
+        copy = torch.empty_like(q, memory_format=torch.contiguous_format)
+        copy.copy_(q)
+        out = A.paged_decode(q, k, v, table[at], n[at])
+        assert torch.equal(out, A.paged_decode(copy, k, v, table[at], n[at]))
+        check_attention(out, q, k, v, table[at], n[at], what="decode")
+        starts = torch.arange(len(q) + 1, dtype=torch.int32, device=cuda)
+        out = A.paged_prefill(q, k, v, table[at], n[at], starts)
+        assert torch.equal(out, A.paged_prefill(copy, k, v, table[at], n[at], starts))
+        check_attention(out, q, k, v, table[at], n[at], starts, what="prefill")
