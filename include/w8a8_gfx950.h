@@ -537,8 +537,8 @@ int w8a8_rotary_store(const void* q, int64_t q_stride_t, int64_t q_stride_h, con
  * lengths[b] <= 0 gives zeros; a length past table_pages * page_size is cut
  * to it.  Entries of the table past a sequence's pages are not used.  A page
  * outside [0, pages) is never read: its keys are masked.
- * q and out: 16-byte aligned, strides multiples of 8, as the cache's; out
- * overlaps no input.  Workspace: w8a8_paged_decode_workspace_bytes(batch,
+ * q and out: 16-byte aligned, strides multiples of 8, as the cache's (of an
+ * axis of one the stride is not used); out overlaps no input.  Workspace: w8a8_paged_decode_workspace_bytes(batch,
  * q_heads, kv_heads, head_dim, table_pages * page_size) bytes (0 where the
  * cache is not split over its length), 16-byte aligned; no state survives the
  * call.

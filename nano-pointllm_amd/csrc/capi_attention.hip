@@ -112,7 +112,9 @@ int check_cache(const Cache& c, int64_t align_elems) {
   if (!strides_ok(c.c_page, c.c_head) || !strides_ok(c.c_tok, 0)) return W8A8_ERR_SHAPE;
   // An offset in the cache stays below 2^62 bytes.
   if (c.pages > 0 && cache_bytes(c) > kMaxBytes) return W8A8_ERR_SHAPE;
-  if (c.c_page % align_elems || c.c_head % align_elems || c.c_tok % align_elems)
+  // The stride of an axis of one is multiplied by zero only.
+  if ((c.pages > 1 && c.c_page % align_elems) || (c.heads > 1 && c.c_head % align_elems) ||
+      (c.page_size > 1 && c.c_tok % align_elems))
     return W8A8_ERR_ALIGN;
   return W8A8_OK;
 }
@@ -267,7 +269,8 @@ int check_attention(PagedAttention& p, const void* q, int64_t q_st, int64_t q_sh
       (table == nullptr || k_cache == nullptr || v_cache == nullptr))
     return W8A8_ERR_NULL;
   if (!aligned(q, 16) || !aligned(out, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16) ||
-      !aligned(table, 4) || !aligned(lengths, 4) || q_st % 8 || q_sh % 8 || o_st % 8 || o_sh % 8)
+      !aligned(table, 4) || !aligned(lengths, 4) || (tokens > 1 && (q_st % 8 || o_st % 8)) ||
+      (q_heads > 1 && (q_sh % 8 || o_sh % 8)))
     return W8A8_ERR_ALIGN;
   const Rows qr{q, q_st, q_sh, tokens, q_heads, c.dim};
   const Rows orr{out, o_st, o_sh, tokens, q_heads, c.dim};

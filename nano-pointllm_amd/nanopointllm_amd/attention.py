@@ -214,7 +214,8 @@ def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor, q: torch.Tensor, d: int
         raise ValueError("the cache must have the rows' dtype")
     if shape[3] != d:
         raise ValueError("the cache and the rows must have one head_dim")
-    if strides != v_cache.stride() or strides[3] != 1:
+    if strides[3] != 1 or strides != v_cache.stride() and any(
+            n > 1 and a != b for n, a, b in zip(shape, strides, v_cache.stride())):
         raise ValueError("k_cache and v_cache must have equal strides and contiguous heads")
     return shape, strides
 

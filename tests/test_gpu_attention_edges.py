@@ -39,3 +39,23 @@ def test_queries_at_any_address_and_stride(cuda, dtype):
         out = A.paged_prefill(q, k, v, table[at], n[at], starts)
         assert torch.equal(out, A.paged_prefill(copy, k, v, table[at], n[at], starts))
         check_attention(out, q, k, v, table[at], n[at], starts, what="prefill")
+
+
+def test_one_page_one_head_and_one_row_of_unused_strides(cuda):
+    """out and caches whose axes of one carry odd strides."""
+    note("unused strides")
+    d, page = 64, 16
+    r = gen_of(6)
+    wide = [randn(r, page * d + 8, dtype=torch.float16, device=cuda) for _ in range(2)]
+    k, v = (w.as_strided((1, 1, page, d), (page * d + 3, 5, d, 1)) for w in wide)
+    table = torch.zeros(1, 1, dtype=torch.int32, device=cuda)
+    n = torch.tensor([11], dtype=torch.int32, device=cuda)
+    starts = torch.tensor([0, 1], dtype=torch.int32, device=cuda)
+    q = randn(r, 1, 1, d, dtype=torch.float16, device=cuda)
+    into = torch.zeros(2 * d, dtype=torch.float16, device=cuda)
+    out = into.as_strided((1, 1, d), (d + 1, 3, 1))
+    want = A.paged_decode(q, k.contiguous(), v.contiguous(), table, n)
+    assert torch.equal(A.paged_decode(q, k, v, table, n, out=out), want)
+    check_attention(out, q, k, v, table, n)
+    check_attention(A.paged_prefill(q, k, v, table, n, starts, out=out), q, k, v, table, n, starts)
+    assert not into[d:].any()
