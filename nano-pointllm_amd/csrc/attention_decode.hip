@@ -377,9 +377,28 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 1 : 2) void decode_kernel(Decod
       for (int i = 0; i < DV; ++i) red_o[wave][r][DV * (4 * g + k) + i] = o[i][k];
   }
   __syncthreads();
+  // What infinities and NaNs among the piece's values make of element d: an
+  // infinity times a part of its weight that is 0 must not make it NaN.  0
+  // without any (the sum itself passed binary32).
+  auto not_finite = [&](int d) {
+    bool up = false, down = false, nan = false;
+    const T* v = static_cast<const T*>(a.v) + kvh * a.c_head + d;
+    const int last = min(t1 * kTile, keys);
+    for (int j = t0 * kTile; j < last; ++j) {
+      const int e = table[j >> a.page_shift];
+      if (e < 0 || e >= pages) continue;
+      const float x = to_f32(v[e * a.c_page + (j & page_mask) * a.c_tok]);
+      up |= x == INFINITY;
+      down |= x == -INFINITY;
+      nan |= x != x;
+    }
+    return nan || (up && down) ? NAN : up ? INFINITY : down ? -INFINITY : 0.0f;
+  };
   const int64_t item = blockIdx.x;
+  bool searched = false;
+  float special = 0.0f;
   for (int n = threadIdx.x; n < rows * DP; n += 64 * W) {
-    const int q = n / DP, d = n % DP;
+    const int q = n / DP, d = n % DP;   // one d per thread
     if (!FULL && d >= D) continue;
     float top = red_r[0][q];
 #pragma unroll
@@ -391,6 +410,11 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 1 : 2) void decode_kernel(Decod
       const float f = exp2_hw(red_r[w][q] - base);
       ov += red_o[w][q][d] * f;
       lv += red_l[w][q] * f;
+    }
+    if (!(fabsf(ov) < INFINITY) && fabsf(lv) < INFINITY) {
+      if (!searched) special = not_finite(d);
+      searched = true;
+      ov = special == 0.0f ? ov : special;
     }
     if (count == 1) {
       write_out<T>(p, seq, head0 + q, d, ov, lv);

@@ -59,3 +59,72 @@ def test_one_page_one_head_and_one_row_of_unused_strides(cuda):
     check_attention(out, q, k, v, table, n)
     check_attention(A.paged_prefill(q, k, v, table, n, starts, out=out), q, k, v, table, n, starts)
     assert not into[d:].any()
+
+
+# ------------------------------------------------- values that are not finite
+INF, NAN = float("inf"), float("nan")
+
+
+def place_of(table, b, key, page):
+    return int(table[b, key // page]), key % page
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("h,g,d,page,length", [
+    (2, 1, 64, 16, 1), (2, 2, 128, 16, 33), (4, 2, 80, 2, 200), (34, 2, 64, 16, 300),
+    (4, 1, 256, 16, 300), (4, 2, 128, 16, 700), (2, 1, 96, 64, 5000), (6, 2, 256, 32, 2500)])
+def test_decode_of_infinities_and_nans(cuda, h, g, d, page, length, dtype):
+    """A visible value's infinity is the element's, whatever its weight; both
+    signs, or a NaN, make it NaN; every other element and head keeps its bits,
+    as does the sequence next to it.  Weights here are above 2^-40 of the
+    largest, far from underflow."""
+    note(f"decode non-finite {h} {g} {d} {page} {length} {dtype}")
+    lengths, grp = [length, 77], h // g
+    k, v, table = paged(length + d, lengths, g, d, page, dtype, cuda)
+    q = randn(gen_of(d), 2, h, d, dtype=dtype, device=cuda)
+    n = torch.tensor(lengths, dtype=torch.int32, device=cuda)
+    clean = A.paged_decode(q, k, v, table, n)
+    check_attention(clean, q, k, v, table, n, what="clean")
+    for key in sorted({0, length // 3, length - 1}):
+        at, row = place_of(table, 0, key, page)
+        bad = v.clone()
+        for e, value in ((1, INF), (d // 2, -INF), (d - 1, NAN)):
+            bad[at, 0, row, e] = value
+        out = A.paged_decode(q, k, bad, table, n)
+        assert (out[0, :grp, 1] == INF).all() and (out[0, :grp, d // 2] == -INF).all()
+        assert torch.isnan(out[0, :grp, d - 1]).all()
+        for e in (1, d // 2, d - 1):
+            out[0, :grp, e] = clean[0, :grp, e]
+        assert torch.equal(out, clean)
+        if length > 1:
+            at, row = place_of(table, 0, (key + length // 2) % length, page)
+            bad[at, 0, row, 1] = -INF if (key + length // 2) % length != key else NAN
+            assert torch.isnan(A.paged_decode(q, k, bad, table, n)[0, :grp, 1]).all()
+        at, row = place_of(table, 0, key, page)
+        bad = k.clone()
+        bad[at, g - 1, row, 3] = NAN
+        out = A.paged_decode(q, bad, v, table, n)
+        assert torch.isnan(out[0, h - grp:]).all()
+        out[0, h - grp:] = clean[0, h - grp:]
+        assert torch.equal(out, clean)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_infinite_keys(cuda, dtype):
+    """An infinite key weighs nothing for a query that it scores -inf for, and
+    makes the rows that it scores inf for NaN."""
+    note(f"infinite keys {dtype}")
+    h, d, length, key = 8, 64, 420, 200
+    k, v, table = paged(2, [length], 1, d, 1, dtype, cuda)
+    q = randn(gen_of(7), 1, h, d, dtype=dtype, device=cuda)
+    q[..., 9] = torch.tensor([1.0, -1.0] * (h // 2)).to(dtype).to(cuda)
+    n = torch.tensor([length], dtype=torch.int32, device=cuda)
+    without = table.clone()
+    without[0, key] = -1
+    bad = k.clone()
+    bad[int(table[0, key]), 0, 0, 9] = INF
+    starts = torch.tensor([0, 1], dtype=torch.int32, device=cuda)
+    for name, out in (("decode", A.paged_decode(q, bad, v, table, n)),
+                      ("prefill", A.paged_prefill(q, bad, v, table, n, starts))):
+        assert torch.isnan(out[0, ::2]).all(), name
+        check_attention(out[:, 1::2], q[:, 1::2], k, v, without, n, what=name)
