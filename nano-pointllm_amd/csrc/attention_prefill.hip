@@ -309,7 +309,7 @@ __device__ inline void careful_rows(const PrefillParams& p, const Place& at, int
 #pragma unroll
       for (int w = 1; w < 64; w <<= 1) s += __shfl_xor(s, w);
       s *= sc;
-      const float next = fmaxf(ref, s);
+      const float next = fmaxf(ref, s - Reference<T>::kBelow);
       const float base = next == -INFINITY ? 0.0f : next;
       const float f = exp2_hw(ref - base), w = exp2_hw(s - base);
       ref = next;

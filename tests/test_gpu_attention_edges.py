@@ -128,3 +128,23 @@ def test_infinite_keys(cuda, dtype):
                       ("prefill", A.paged_prefill(q, bad, v, table, n, starts))):
         assert torch.isnan(out[0, ::2]).all(), name
         check_attention(out[:, 1::2], q[:, 1::2], k, v, without, n, what=name)
+
+
+def test_large_values_next_to_a_masked_nan(cuda):
+    """bfloat16 values near the type's largest: 40 of them weigh alike, their
+    mean is one of them, and a NaN that only the last row sees changes no row
+    before it.  (Sums of 40 products of 2^-8 and 2e38 stay finite.)"""
+    note("large values")
+    n, d = 40, 64
+    k, v, table = paged(1, [n], 1, d, 16, torch.bfloat16, cuda, poison=False)
+    v.fill_(2e38)
+    q = torch.zeros(n, 2, d, dtype=torch.bfloat16, device=cuda)
+    lengths = torch.tensor([n], dtype=torch.int32, device=cuda)
+    starts = torch.tensor([0, n], dtype=torch.int32, device=cuda)
+    want = v[0, 0, 0, 0]
+    assert (A.paged_prefill(q, k, v, table, lengths, starts) == want).all()
+    assert (A.paged_decode(q[:1], k, v, table, lengths) == want).all()
+    at, row = place_of(table, 0, n - 1, 16)
+    v[at, 0, row] = NAN
+    out = A.paged_prefill(q, k, v, table, lengths, starts)
+    assert (out[:-1] == want).all() and torch.isnan(out[-1]).all()
