@@ -5,11 +5,15 @@ Tolerances as in test_gpu_attention.py where its check is used; others are
 derived at the test."""
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
 from nanopointllm_amd import attention as A
-from test_gpu_attention import DTYPES, check_attention, gen_of, note, paged, randn
+from oracle import attention_oracle as O
+from test_gpu_attention import (DTYPES, check_attention, check_rotary, gen_of, note, paged, randn,
+                                smallest)
 
 pytestmark = pytest.mark.gpu
 
@@ -130,6 +134,54 @@ def test_infinite_keys(cuda, dtype):
         check_attention(out[:, 1::2], q[:, 1::2], k, v, without, n, what=name)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("h,g,d,page,new,length", [
+    (4, 2, 64, 16, 40, 40), (4, 2, 128, 16, 9, 3000), (4, 1, 64, 32, 7, 5000),
+    (2, 1, 80, 8, 11, 2500), (2, 2, 256, 16, 6, 1800), (6, 2, 96, 4, 5, 1200),
+    (2, 1, 24, 16, 20, 900), (3, 1, 192, 64, 30, 2100)])
+def test_prefill_of_infinities_and_nans(cuda, h, g, d, page, new, length, dtype):
+    """Rows recomputed key by key, whole tiles and tiles cut over the keys: an
+    infinity that every row sees, a NaN among the newest tokens that only the
+    later ones see, with and without a page that is unknown."""
+    note(f"prefill non-finite {h} {g} {d} {page} {new} {length} {dtype}")
+    grp = h // g
+    k, v, table = paged(length + d, [length], g, d, page, dtype, cuda)
+    q = randn(gen_of(d), new, h, d, dtype=dtype, device=cuda)
+    n = torch.tensor([length], dtype=torch.int32, device=cuda)
+    starts = torch.tensor([0, new], dtype=torch.int32, device=cuda)
+    early, late = 2, length - new // 2          # keys; `late` is token new - new // 2
+    for unknown in (False, True):
+        if unknown:
+            if length - new < 8 * page:
+                continue
+            table[0, (length // 2) // page] = -1
+        clean = A.paged_prefill(q, k, v, table, n, starts)
+        check_attention(clean, q, k, v, table, n, starts, what=f"clean {unknown}")
+        bad = v.clone()
+        at, row = place_of(table, 0, early, page)
+        bad[at, 0, row, 1] = INF
+        at, row = place_of(table, 0, late, page)
+        bad[at, 0, row, 5] = NAN
+        bad[at, 0, row, d - 1] = -INF
+        out = A.paged_prefill(q, k, bad, table, n, starts)
+        first = new - new // 2
+        sees_early = 0 if new < length else early
+        assert (out[sees_early:, :grp, 1] == INF).all()
+        assert torch.isnan(out[first:, :grp, 5]).all()
+        assert (out[first:, :grp, d - 1] == -INF).all()
+        out[sees_early:, :grp, 1] = clean[sees_early:, :grp, 1]
+        out[first:, :grp, 5] = clean[first:, :grp, 5]
+        out[first:, :grp, d - 1] = clean[first:, :grp, d - 1]
+        check_attention(out, q, k, v, table, n, starts, what=f"values {unknown}")
+        assert torch.equal(out[:, grp:], clean[:, grp:])
+        bad = k.clone()
+        bad[at, g - 1, row, 3] = NAN
+        out = A.paged_prefill(q, bad, v, table, n, starts)
+        assert torch.isnan(out[first:, h - grp:]).all()
+        out[first:, h - grp:] = clean[first:, h - grp:]
+        check_attention(out, q, k, v, table, n, starts, what=f"key {unknown}")
+
+
 def test_large_values_next_to_a_masked_nan(cuda):
     """bfloat16 values near the type's largest: 40 of them weigh alike, their
     mean is one of them, and a NaN that only the last row sees changes no row
@@ -148,3 +200,139 @@ def test_large_values_next_to_a_masked_nan(cuda):
     v[at, 0, row] = NAN
     out = A.paged_prefill(q, k, v, table, lengths, starts)
     assert (out[:-1] == want).all() and torch.isnan(out[-1]).all()
+
+
+# -------------------------------------------------- weights, and what sums them
+@pytest.mark.parametrize("below", [10, 14, 20, 23, 26])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_numerator_and_denominator_hold_the_same_weights(cuda, dtype, below):
+    """One key ahead of 20 thousand by about 2^below each, all of one value v:
+    the result is v.  The weights lie just off a step of the 16-bit type, so
+    that a denominator of unrounded ones would be off by half a step, and past
+    2^-14 binary16 holds them in fewer bits or drops them.
+
+    v has the mantissa next to 2, where half a step is e / 2 of it (e =
+    finfo.eps / 2).  Sums: a piece has at most 20 units of 32 keys (32 pieces of
+    626), so its denominator is at most 20 x 8 + 10 additions deep and its
+    numerator 40 matrix instructions of at most 17, and a wavefront of a decode
+    workgroup takes no more; 1100 u with the join's.  Decode's weights lose
+    at most 2^-15 (bfloat16) or 2^-21, and 2^-24 of a scale of at least 2^7:
+    n 2^-31.  All of it stays below e / 2, so the result is v exactly."""
+    note(f"same weights {dtype} {below}")
+    n, d, page = 20001, 64, 64
+    e, u = torch.finfo(dtype).eps / 2, 2.0 ** -24
+    lost = 2.0 ** -21 + n * 2.0 ** -31 if dtype == torch.float16 else 2.0 ** -15
+    assert 1100 * u + lost < e / 2
+    k, v, table = paged(31, [n], 1, d, page, dtype, cuda, poison=False)
+    v.fill_(2.0 - torch.finfo(dtype).eps)
+    k.zero_()
+    k[table[0, 0].long(), 0, 0, 0] = 1.0
+    q = torch.zeros(1, 2, d, dtype=dtype, device=cuda)
+    q[..., 0] = 16.0
+    scale = (below - math.log2(1.0 + 0.96 * e)) * math.log(2.0) / 16.0
+    lengths = torch.tensor([n], dtype=torch.int32, device=cuda)
+    starts = torch.tensor([0, 1], dtype=torch.int32, device=cuda)
+    for name, out in (("decode", A.paged_decode(q, k, v, table, lengths, scale=scale)),
+                      ("prefill", A.paged_prefill(q, k, v, table, lengths, starts, scale=scale))):
+        assert (out == v[0, 0, 0, 0]).all(), f"{name} {out.flatten()[0]} {v[0, 0, 0, 0]}"
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("h,g,d,lengths", [(8, 2, 128, [64, 33, 200]), (4, 4, 64, [600, 64]),
+                                           (4, 1, 256, [90, 400])])
+def test_decode_weights_keep_two_parts(cuda, h, g, d, lengths, dtype):
+    """Decode's weights enter the product with more bits than the 16-bit type
+    holds.  One element of a query is not zero, so a score is one product: with
+    u = 2^-24, r = 2 (13 u |score| + 16 u) for both sums' weights, 2 n u for
+    sums over n keys, 2^-15 (bfloat16: 8 + 8 bits cut off) or 2^-21 + n 2^-31
+    (binary16: 11 + 11 bits, steps of 2^-24 at a scale of 2^7) for the two
+    parts; e |out| for the result's rounding.  The definition with weights cut
+    to the type misses this bound."""
+    note(f"two parts {h} {g} {d} {lengths} {dtype}")
+    k, v, table = paged(d, lengths, g, d, 16, dtype, cuda)
+    q = torch.zeros(len(lengths), h, d, dtype=dtype, device=cuda)
+    q[..., 2] = randn(gen_of(1), len(lengths), h, dtype=dtype, device=cuda, std=1.7 * d ** 0.5)
+    n = torch.tensor(lengths, dtype=torch.int32, device=cuda)
+    want, size, dots = O.attention(q, k, v, table, n)
+    u, e, most = 2.0 ** -24, torch.finfo(dtype).eps / 2, max(lengths)
+    parts = 2.0 ** -21 + most * 2.0 ** -31 if dtype == torch.float16 else 2.0 ** -15
+    tol = (2 * (13 * u * dots + 16 * u) + 2 * most * u + parts)[..., None] * size
+    tol = tol + e * want.abs() + smallest(dtype)
+    out = A.paged_decode(q, k, v, table, n).double().cpu()
+    assert ((out - want).abs() <= tol).all(), float(((out - want).abs() - tol).max())
+    # One part: the weights of the definition cut to the type's bits.
+    bits, missed = (11 if dtype == torch.float16 else 8), 0
+    for b, total in enumerate(lengths):
+        for i in range(h):
+            keys, _ = O.keys_of(k.cpu(), table.cpu(), b, i // (h // g), total)
+            values, _ = O.keys_of(v.cpu(), table.cpu(), b, i // (h // g), total)
+            s = keys @ q[b, i].double().cpu() * d ** -0.5
+            p = torch.exp(s - s.max())
+            m, x = torch.frexp(p)
+            cut = torch.ldexp(torch.floor(m * 2.0 ** bits) * 2.0 ** -bits, x)
+            missed += int((((cut @ values) / p.sum() - want[b, i]).abs() > tol[b, i]).sum())
+    assert missed > 0
+
+
+# ------------------------------------------------------- tables, strides, rows
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_tables_wider_than_any_sequence(cuda, dtype):
+    """A captured step's table has room to grow: 4096 keys and more where the
+    sequences have at most 1590, the entries behind them unknown."""
+    note(f"wide tables {dtype}")
+    h, g, d, page = 8, 8, 64, 16
+    lengths = [1590, 0, 1, 636, 1000, 31, 32, 1500] * 4
+    k, v, table = paged(8, lengths, g, d, page, dtype, cuda)
+    wide = torch.full((len(lengths), 640), 2 ** 31 - 1, dtype=torch.int32, device=cuda)
+    wide[:, :table.shape[1]] = table
+    q = randn(gen_of(9), len(lengths), h, d, dtype=dtype, device=cuda, std=1.7)
+    n = torch.tensor(lengths, dtype=torch.int32, device=cuda)
+    check_attention(A.paged_decode(q, k, v, wide, n), q, k, v, table, n, what="decode")
+    new = [9, 0, 1, 40, 130, 31, 1, 5]
+    starts = torch.tensor([0] + new).cumsum(0).to(torch.int32).to(cuda)
+    q = randn(gen_of(9), sum(new), h, d, dtype=dtype, device=cuda, std=1.7)
+    check_attention(A.paged_prefill(q, k, v, wide[:8], n[:8], starts), q, k, v, table[:8], n[:8],
+                    starts, what="prefill")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_what_the_checks_make_contiguous(cuda, dtype):
+    """Rows with scattered elements, a transposed table, lengths, positions and
+    slots of every second place: the same bits as their copies, on values that
+    all differ."""
+    note(f"made contiguous {dtype}")
+    h, g, d, page, lengths = 4, 2, 64, 16, [40, 300, 7]
+    k, v, table = paged(12, lengths, g, d, page, dtype, cuda)
+    r = gen_of(13)
+    q = randn(r, 3, h, d, dtype=dtype, device=cuda)
+    turned = q.transpose(1, 2).contiguous().transpose(1, 2)
+    n = torch.tensor(lengths, dtype=torch.int32, device=cuda)
+
+    def every_second(x):
+        wide = torch.full((2 * len(x),), 10 ** 6, dtype=x.dtype, device=cuda)
+        wide[::2] = x
+        return wide[::2]
+
+    columns = table.T.contiguous().T
+    want = A.paged_decode(q, k, v, table, n)
+    check_attention(want, q, k, v, table, n, what="decode")
+    assert torch.equal(A.paged_decode(turned, k, v, columns, every_second(n)), want)
+    starts = torch.tensor([0, 1, 3, 3], dtype=torch.int32, device=cuda)
+    want = A.paged_prefill(q, k, v, table, n, starts)
+    check_attention(want, q, k, v, table, n, starts, what="prefill")
+    assert torch.equal(A.paged_prefill(turned, k, v, columns, every_second(n),
+                                       every_second(starts)), want)
+    kv = [randn(r, 3, g, d, dtype=dtype, device=cuda) for _ in range(2)]
+    positions, slots = (torch.tensor(x, device=cuda) for x in ([5, 900, 77], [3, 49, 18]))
+    freq = A.rotary_frequencies(d, device=cuda).inv_freq
+    got = []
+    for rows, other, at, to, f in (
+            (q, kv, positions, slots, freq),
+            (turned, [x.transpose(1, 2).contiguous().transpose(1, 2) for x in kv],
+             every_second(positions), every_second(slots), every_second(freq))):
+        caches = torch.zeros(2, 4, g, page, d, dtype=dtype, device=cuda)
+        out = A.rotary_store(rows, *other, at, to, f, caches[0], caches[1])
+        got.append((out, caches, A.rotary(rows, at, f)))
+    check_rotary(got[0][0], q, positions, freq, "half", 1.0)
+    for a, b in zip(*got):
+        assert a.any() and torch.equal(a, b)
