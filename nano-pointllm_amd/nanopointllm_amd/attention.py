@@ -535,4 +535,4 @@ class PagedAttentionCore:
                          out=out[:n])
             paged_prefill(q[n:], k_cache, v_cache, table[n:], lengths[n:], state.q_starts,
                           scale=self.scale, out=out[n:])
-        return out.view(out.shape[0], -1)
+        return out.flatten(1)

@@ -336,3 +336,15 @@ def test_what_the_checks_make_contiguous(cuda, dtype):
     check_rotary(got[0][0], q, positions, freq, "half", 1.0)
     for a, b in zip(*got):
         assert a.any() and torch.equal(a, b)
+
+
+def test_core_of_empty_steps(cuda):
+    """A step of no row is one, with sequences or without."""
+    note("core empty")
+    h, g, d, page = 4, 2, 64, 16
+    cache = A.PagedKVCache(1, 8, g, d, page_size=page, device=cuda)
+    core = A.PagedAttentionCore(cache, A.rotary_frequencies(d, device=cuda))
+    q, k, v = (torch.empty(0, n, d, dtype=torch.float16, device=cuda) for n in (h, g, g))
+    for pages, lengths, new in (([], [], []), ([[0, 1]], [22], [0])):
+        state = A.AttentionState.build(pages, lengths, new, page, device=cuda)
+        assert core(q, k, v, 0, state).shape == (0, h * d)
