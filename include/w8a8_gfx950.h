@@ -35,7 +35,7 @@
 extern "C" {
 #endif
 
-#define W8A8_ABI_VERSION 8
+#define W8A8_ABI_VERSION 9
 
 typedef enum w8a8_dtype {
   W8A8_F32 = 0,
@@ -538,10 +538,10 @@ int w8a8_rotary_store(const void* q, int64_t q_stride_t, int64_t q_stride_h, con
  * to it.  Entries of the table past a sequence's pages are not used.  A page
  * outside [0, pages) is never read: its keys are masked.
  * q and out: 16-byte aligned, strides multiples of 8, as the cache's (of an
- * axis of one the stride is not used); out overlaps no input.  Workspace: w8a8_paged_decode_workspace_bytes(batch,
- * q_heads, kv_heads, head_dim, table_pages * page_size) bytes (0 where the
- * cache is not split over its length), 16-byte aligned; no state survives the
- * call.
+ * axis of one the stride is not used); out overlaps no input.  Workspace:
+ * w8a8_paged_decode_workspace_bytes(batch, q_heads, kv_heads, head_dim,
+ * table_pages * page_size) bytes (0 where the cache is not split over its
+ * length), 16-byte aligned; no state survives the call.
  */
 int w8a8_paged_decode(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_cache,
                       const void* v_cache, int64_t cache_stride_page, int64_t cache_stride_head,
@@ -576,6 +576,20 @@ int w8a8_paged_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, co
                        void* out, int64_t out_stride_t, int64_t out_stride_h, int64_t tokens,
                        int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                        void* workspace, int64_t workspace_bytes, hipStream_t stream);
+
+/*
+ * w8a8_paged_prefill into a buffer of unknown contents: rows of no sequence (a
+ * padded batch's) become zeros.  batch may be 0 only without tokens.
+ */
+int w8a8_paged_prefill_padded(const void* q, int64_t q_stride_t, int64_t q_stride_h,
+                              const void* k_cache, const void* v_cache, int64_t cache_stride_page,
+                              int64_t cache_stride_head, int64_t cache_stride_token, int64_t pages,
+                              int64_t page_size, const int32_t* page_table, int64_t ld_table,
+                              int64_t table_pages, const int32_t* lengths, const int32_t* q_starts,
+                              int dtype, float scale, void* out, int64_t out_stride_t,
+                              int64_t out_stride_h, int64_t tokens, int64_t batch, int64_t q_heads,
+                              int64_t kv_heads, int64_t head_dim, void* workspace,
+                              int64_t workspace_bytes, hipStream_t stream);
 
 /* Workspace bytes of w8a8_paged_prefill; -1 for sizes it does not take. */
 int64_t w8a8_paged_prefill_workspace_bytes(int64_t tokens, int64_t batch, int64_t q_heads,

@@ -91,6 +91,7 @@ struct PrefillParams {
   int cut;             // most pieces of a row tile
   int few;             // ... of kFewUnits and more
   bool sorted;         // row tiles go by the keys they see, at most 64 sequences
+  bool clear;          // rows of no sequence become zeros
   float* part_o;       // [row tiles x kv_heads x cut, kRows, head_dim]
   f32x2* part_rl;      // [row tiles x kv_heads x cut, kRows]
 };
@@ -113,10 +114,10 @@ __device__ inline int divide_rows(int r, int group) {
 
 // One row tile: which rows of which sequence, and the keys that they see.
 struct Place {
-  int seq;      // or -1
+  int seq;      // or -1: the batch has no such tile
   int start;    // the sequence's first row of q
   int count;    // its tokens
-  int row0;     // the tile's first row of count x group
+  int row0;     // the tile's first row of count x group; without one, the batch's tiles
   int keys;     // the sequence's keys
 };
 
@@ -150,7 +151,7 @@ __device__ inline Place find_tile(const PrefillParams& p, int rank) {
   if (p.sorted) {
     const Seq s = read(lane);
     const int tiles = lane_value(scan64(s.tiles), 63);
-    if (tiles <= rank) return Place{-1, 0, 0, 0, 0};
+    if (tiles <= rank) return Place{-1, 0, 0, tiles, 0};
     if (a.batch == 1) return place(0, s, 0, tiles - 1 - rank);
     // How many of the lane's tiles see fewer than u units: its first ones, up to
     // the first token that sees more than (u - 1) kKeys keys.
@@ -190,7 +191,7 @@ __device__ inline Place find_tile(const PrefillParams& p, int rank) {
     }
     before += lane_value(upto, 63);
   }
-  return Place{-1, 0, 0, 0, 0};
+  return Place{-1, 0, 0, before, 0};
 }
 
 // Units of keys that the rows of a tile see, and how many pieces they are cut
@@ -267,6 +268,21 @@ template <int DP> __device__ inline int swizzle_v(int key) {
 template <typename T>
 __device__ inline T* out_row(const PagedAttention& a, int start, int token, int head) {
   return static_cast<T*>(a.out) + (start + token) * a.o_st + head * a.o_sh;
+}
+
+// Zeros in the rows of no sequence, those before the first one's and behind the
+// last one's: workgroup i of n takes every n-th.
+__device__ inline void clear_rows(const PrefillParams& p, int kvh, int i, int n) {
+  const PagedAttention& a = p.a;
+  const int first = max(0, min(a.q_starts[0], a.tokens));
+  const int end = max(first, min(a.q_starts[a.batch], a.tokens));
+  const int chunks = a.head_dim / 8;   // of 16 bytes
+  for (int64_t r = i; r < first + (a.tokens - end); r += n) {
+    uint16_t* row = static_cast<uint16_t*>(a.out) + (r < first ? r : r - first + end) * a.o_st;
+    for (int c = threadIdx.x; c < p.group * chunks; c += 64 * kWaves)
+      *reinterpret_cast<u32x4*>(row + (kvh * p.group + c / chunks) * a.o_sh + c % chunks * 8) =
+          u32x4{0, 0, 0, 0};
+  }
 }
 
 // The rows of `bad` (bit c: row c of the wavefront's 32), key by key: lane i
@@ -358,7 +374,11 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) void prefill_kernel
   // workgroups on one head at a time instead, for its L2, measures the same).
   const int kvh = blockIdx.x % a.kv_heads;
   const Place at = find_tile(p, blockIdx.x / a.kv_heads);
-  if (at.seq < 0) return;
+  if (at.seq < 0) {
+    if (p.clear && blockIdx.y == 0)
+      clear_rows(p, kvh, blockIdx.x / a.kv_heads - at.row0, gridDim.x / a.kv_heads - at.row0);
+    return;
+  }
   const int all_units = key_units(p, at);
   const int pieces = pieces_of(p, all_units);
   const int piece = blockIdx.y;
@@ -821,7 +841,9 @@ int64_t pairs_bytes(int64_t rows) { return ceil_div(rows * 8, 256) * 256; }
 
 template <typename T, int DP, int DU>
 hipError_t launch_d(const PrefillParams& p, int64_t items, hipStream_t st) {
-  const dim3 grid(static_cast<uint32_t>(items), static_cast<uint32_t>(p.cut));
+  // To clear rows, at least one workgroup per key head without a row tile.
+  const dim3 grid(static_cast<uint32_t>(items + (p.clear ? p.a.kv_heads : 0)),
+                  static_cast<uint32_t>(p.cut));
   const bool dma = p.a.page_shift >= 3 && (p.a.c_tok << p.a.page_shift) < (int64_t{1} << 30);
   if (dma)
     hipLaunchKernelGGL((prefill_kernel<T, DP, DU, true>), grid, dim3(64 * kWaves), 0, st, p);
@@ -855,9 +877,10 @@ int64_t paged_prefill_workspace(int64_t tokens, int64_t batch, int64_t q_heads, 
   return pairs_bytes(rows) + rows * head_dim * 4;
 }
 
-hipError_t launch_paged_prefill(const PagedAttention& a, int dtype, hipStream_t st) {
+hipError_t launch_paged_prefill(const PagedAttention& a, bool clear, int dtype, hipStream_t st) {
   PrefillParams p;
   p.a = a;
+  p.clear = clear;
   p.group = a.q_heads / a.kv_heads;
   const int64_t items = max_tiles(a.tokens, a.batch, p.group) * a.kv_heads;
   p.cut = static_cast<int>(cut_of(items, a.max_keys));

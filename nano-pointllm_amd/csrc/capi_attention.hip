@@ -311,6 +311,35 @@ bool sizes_ok(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, 
          head_dim <= kAttentionMaxDim && max_keys >= 0 && max_keys <= kMaxTokens;
 }
 
+// Both prefill entry points; clear: rows of no sequence become zeros.
+int paged_prefill(bool clear, const void* q, int64_t q_stride_t, int64_t q_stride_h,
+                  const void* k_cache, const void* v_cache, int64_t cache_stride_page,
+                  int64_t cache_stride_head, int64_t cache_stride_token, int64_t pages,
+                  int64_t page_size, const int32_t* page_table, int64_t ld_table,
+                  int64_t table_pages, const int32_t* lengths, const int32_t* q_starts, int dtype,
+                  float scale, void* out, int64_t out_stride_t, int64_t out_stride_h,
+                  int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                  int64_t head_dim, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+  const Cache c{cache_stride_page, cache_stride_head, cache_stride_token, pages,
+                page_size,         kv_heads,          head_dim};
+  PagedAttention p;
+  const int rc = check_attention(p, q, q_stride_t, q_stride_h, k_cache, v_cache, c, page_table,
+                                 ld_table, table_pages, lengths, dtype, scale, out, out_stride_t,
+                                 out_stride_h, tokens, batch, q_heads, kPrefillRows);
+  if (rc != W8A8_OK || tokens == 0) return rc;
+  // Nothing says then which rows the batch's workgroups would clear.
+  if (batch == 0) return clear ? W8A8_ERR_SHAPE : W8A8_OK;
+  if (q_starts == nullptr) return W8A8_ERR_NULL;
+  if (!aligned(q_starts, 4)) return W8A8_ERR_ALIGN;
+  const int64_t need =
+      paged_prefill_workspace(tokens, batch, q_heads, kv_heads, head_dim, p.max_keys);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return W8A8_ERR_WORKSPACE;
+  if (need > 0 && !aligned(workspace, 16)) return W8A8_ERR_ALIGN;
+  p.workspace = workspace;
+  p.q_starts = q_starts;
+  return status_of(launch_paged_prefill(p, clear, dtype, stream));
+}
+
 }  // namespace
 
 extern "C" {
@@ -359,22 +388,27 @@ int w8a8_paged_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, co
                        void* out, int64_t out_stride_t, int64_t out_stride_h, int64_t tokens,
                        int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                        void* workspace, int64_t workspace_bytes, hipStream_t stream) {
-  const Cache c{cache_stride_page, cache_stride_head, cache_stride_token, pages,
-                page_size,         kv_heads,          head_dim};
-  PagedAttention p;
-  const int rc = check_attention(p, q, q_stride_t, q_stride_h, k_cache, v_cache, c, page_table,
-                                 ld_table, table_pages, lengths, dtype, scale, out, out_stride_t,
-                                 out_stride_h, tokens, batch, q_heads, kPrefillRows);
-  if (rc != W8A8_OK || tokens == 0 || batch == 0) return rc;
-  if (q_starts == nullptr) return W8A8_ERR_NULL;
-  if (!aligned(q_starts, 4)) return W8A8_ERR_ALIGN;
-  const int64_t need =
-      paged_prefill_workspace(tokens, batch, q_heads, kv_heads, head_dim, p.max_keys);
-  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return W8A8_ERR_WORKSPACE;
-  if (need > 0 && !aligned(workspace, 16)) return W8A8_ERR_ALIGN;
-  p.workspace = workspace;
-  p.q_starts = q_starts;
-  return status_of(launch_paged_prefill(p, dtype, stream));
+  return paged_prefill(false, q, q_stride_t, q_stride_h, k_cache, v_cache, cache_stride_page,
+                       cache_stride_head, cache_stride_token, pages, page_size, page_table,
+                       ld_table, table_pages, lengths, q_starts, dtype, scale, out, out_stride_t,
+                       out_stride_h, tokens, batch, q_heads, kv_heads, head_dim, workspace,
+                       workspace_bytes, stream);
+}
+
+int w8a8_paged_prefill_padded(const void* q, int64_t q_stride_t, int64_t q_stride_h,
+                              const void* k_cache, const void* v_cache, int64_t cache_stride_page,
+                              int64_t cache_stride_head, int64_t cache_stride_token, int64_t pages,
+                              int64_t page_size, const int32_t* page_table, int64_t ld_table,
+                              int64_t table_pages, const int32_t* lengths, const int32_t* q_starts,
+                              int dtype, float scale, void* out, int64_t out_stride_t,
+                              int64_t out_stride_h, int64_t tokens, int64_t batch, int64_t q_heads,
+                              int64_t kv_heads, int64_t head_dim, void* workspace,
+                              int64_t workspace_bytes, hipStream_t stream) {
+  return paged_prefill(true, q, q_stride_t, q_stride_h, k_cache, v_cache, cache_stride_page,
+                       cache_stride_head, cache_stride_token, pages, page_size, page_table,
+                       ld_table, table_pages, lengths, q_starts, dtype, scale, out, out_stride_t,
+                       out_stride_h, tokens, batch, q_heads, kv_heads, head_dim, workspace,
+                       workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -291,7 +291,8 @@ int64_t paged_decode_workspace(int64_t batch, int64_t q_heads, int64_t kv_heads,
 int64_t paged_prefill_workspace(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
                                 int64_t head_dim, int64_t max_keys);
 hipError_t launch_paged_decode(const PagedAttention& p, int dtype, hipStream_t st);
-hipError_t launch_paged_prefill(const PagedAttention& p, int dtype, hipStream_t st);
+// clear: rows of no sequence become zeros.
+hipError_t launch_paged_prefill(const PagedAttention& p, bool clear, int dtype, hipStream_t st);
 
 // The w8a8_status of a launch; a failure is kept for w8a8_last_hip_error.
 int status_of(hipError_t e);

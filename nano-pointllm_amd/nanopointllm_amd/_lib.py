@@ -13,7 +13,7 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "libw8a8_gfx950.so"
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 F32, F16, BF16, I32, I8 = 0, 1, 2, 3, 4
 EPI_I32, EPI_DEQUANT, EPI_SILU_MUL, EPI_SILU_MUL_Q8 = 0, 1, 2, 3
@@ -76,6 +76,7 @@ EXPORTED_SYMBOLS = (
     "w8a8_paged_decode",
     "w8a8_paged_decode_workspace_bytes",
     "w8a8_paged_prefill",
+    "w8a8_paged_prefill_padded",
     "w8a8_paged_prefill_workspace_bytes",
 )
 
@@ -142,6 +143,9 @@ _SIGNATURES = {
     "w8a8_paged_prefill": (_int, [_vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp,
                                   _i64, _i64, _vp, _vp, _int, _f32, _vp, _i64, _i64, _i64, _i64,
                                   _i64, _i64, _i64, _vp, _i64, _vp]),
+    "w8a8_paged_prefill_padded": (_int, [_vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
+                                         _vp, _i64, _i64, _vp, _vp, _int, _f32, _vp, _i64, _i64,
+                                         _i64, _i64, _i64, _i64, _i64, _vp, _i64, _vp]),
     "w8a8_paged_prefill_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64]),
 }
 

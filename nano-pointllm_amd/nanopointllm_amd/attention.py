@@ -398,13 +398,20 @@ def paged_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     (int32 ``[batch + 1]``, not decreasing) are the newest tokens of sequence
     ``b``, whose ``lengths[b]`` keys, theirs among them, are in the cache.  The
     last row sees all of them, each row before it one fewer; a row that sees
-    none is zeros.  Rows of no sequence are not written (``out``'s keep what
-    they hold).  Otherwise as :func:`paged_decode`."""
+    none is zeros.  Rows of no sequence (a padded batch's) are zeros too, but
+    in a given ``out`` they keep what they hold.  Otherwise as
+    :func:`paged_decode`."""
+    return _prefill(q, k_cache, v_cache, page_table, lengths, q_starts, scale, out, out is None)
+
+
+def _prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+             page_table: torch.Tensor, lengths: torch.Tensor, q_starts: torch.Tensor,
+             scale: float | None, out: torch.Tensor | None, clear: bool) -> torch.Tensor:
+    """:func:`paged_prefill`; ``clear``: rows of no sequence become zeros."""
     index = _gpu(q, k_cache, v_cache, page_table, lengths, q_starts, out)
     if index != torch._C._cuda_getDevice():
         with torch.cuda.device(index):
-            return paged_prefill(q, k_cache, v_cache, page_table, lengths, q_starts, scale=scale,
-                                 out=out)
+            return _prefill(q, k_cache, v_cache, page_table, lengths, q_starts, scale, out, clear)
     code = _rows(q, "q")
     q, qs = _queries(q)
     t, h, d = q.shape
@@ -417,7 +424,10 @@ def paged_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     os = out.stride()
     need = _prefill_workspace(t, b, h, g, d, width * page_size)
     ws = q.new_empty(((need + 1) // 2,)) if need > 0 else None
-    _lib.check(_lib.load().w8a8_paged_prefill(
+    if clear and b == 0:
+        return out.zero_()
+    lib = _lib.load()
+    _lib.check((lib.w8a8_paged_prefill_padded if clear else lib.w8a8_paged_prefill)(
         q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2],
         pages, page_size, page_table.data_ptr(), ld, width, lengths.data_ptr(),
         q_starts.data_ptr(), code, d ** -0.5 if scale is None else scale, out.data_ptr(), os[0],
@@ -452,7 +462,8 @@ class PagedKVCache:
 @dataclass
 class AttentionState:
     """What one step of the stack attends to, all on the GPU: per row its
-    position and its slot in the cache (-1: a padded row, not stored), per
+    position and its slot in the cache (-1: a padded row, not stored; behind
+    the chunks' rows it belongs to no sequence, and its result is zeros), per
     sequence its pages and its length with this step's tokens.  The first
     ``decode_rows`` rows are one new token each of the first ``decode_rows``
     sequences; the others are chunks, ``q_starts`` giving where each of the
@@ -533,6 +544,6 @@ class PagedAttentionCore:
             out = torch.empty_like(q)
             paged_decode(q[:n], k_cache, v_cache, table[:n], lengths[:n], scale=self.scale,
                          out=out[:n])
-            paged_prefill(q[n:], k_cache, v_cache, table[n:], lengths[n:], state.q_starts,
-                          scale=self.scale, out=out[n:])
+            _prefill(q[n:], k_cache, v_cache, table[n:], lengths[n:], state.q_starts,
+                     self.scale, out[n:], True)
         return out.flatten(1)

@@ -338,6 +338,62 @@ def test_what_the_checks_make_contiguous(cuda, dtype):
         assert a.any() and torch.equal(a, b)
 
 
+@pytest.mark.parametrize("h,g,d,page,before,new,lengths,behind", [
+    (4, 2, 64, 16, 0, [5, 20], [5, 90], 1), (8, 2, 128, 16, 3, [17, 0, 40], [30, 9, 40], 2100),
+    (4, 4, 64, 16, 129, [128], [128], 0), (4, 1, 80, 8, 1, [3], [5000], 7),
+    (2, 1, 24, 4, 2, [0, 0], [9, 0], 30), (3, 3, 256, 32, 0, [64, 64], [64, 200], 640),
+    (8, 1, 64, 16, 0, [1 + i % 3 for i in range(70)], [9 + i for i in range(70)], 300)])
+def test_padded_prompt_rows_are_zeros(cuda, h, g, d, page, before, new, lengths, behind):
+    """Rows of no sequence, before the first one's and behind the last one's, in
+    a tensor that the call allocates (of memory that held NaN), and nothing of
+    them in a given one."""
+    note(f"padded rows {h} {g} {d} {page} {before} {new[:4]} {behind}")
+    for dtype in DTYPES:
+        k, v, table = paged(h + d, lengths, g, d, page, dtype, cuda)
+        starts = torch.tensor([before] + new).cumsum(0).to(torch.int32).to(cuda)
+        t = before + sum(new) + behind
+        q = randn(gen_of(t), t, h, d, dtype=dtype, device=cuda)
+        n = torch.tensor(lengths, dtype=torch.int32, device=cuda)
+        for _ in range(2):
+            junk = [torch.full((t, h, d), NAN, dtype=dtype, device=cuda) for _ in range(8)]
+            places = {x.data_ptr() for x in junk}
+            del junk
+            out = A.paged_prefill(q, k, v, table, n, starts)
+            assert out.data_ptr() in places  # the NaNs' memory, or this shows nothing
+            assert (out[:before] == 0).all() and (out[t - behind:] == 0).all()
+            check_attention(out, q, k, v, table, n, starts)
+        into = torch.full((t, h, d), 7.0, dtype=dtype, device=cuda)
+        A.paged_prefill(q, k, v, table, n, starts, out=into)
+        assert (into[:before] == 7.0).all() and (into[t - behind:] == 7.0).all()
+        assert torch.equal(into[before:t - behind], out[before:t - behind])
+    none = A.paged_prefill(q, k, v, table[:0], n[:0], starts[:1])
+    assert none.shape == q.shape and not none.any()
+
+
+def test_core_of_padded_steps(cuda):
+    """Padded rows behind a step's chunks come out as zeros, with and without
+    decode rows before them, whatever the memory held."""
+    note("core padded")
+    h, g, d, page, dtype = 4, 2, 64, 16, torch.float16
+    cache = A.PagedKVCache(1, 8, g, d, page_size=page, dtype=dtype, device=cuda)
+    core = A.PagedAttentionCore(cache, A.rotary_frequencies(d, device=cuda))
+    r = gen_of(5)
+    for pages, lengths, new, pad in (([[0, 1], [2]], [20, 9], [20, 9], 5),
+                                     ([[0, 1], [2]], [21, 12], [1, 3], 6),
+                                     ([[0, 1]], [22], [1], 0)):
+        state = A.AttentionState.build(pages, lengths, new, page, device=cuda)
+        rows = sum(new)
+        x = [randn(r, rows + pad, n, d, dtype=dtype, device=cuda) for n in (h, g, g)]
+        want = core(*[y[:rows] for y in x], 0, state)
+        state.positions = torch.cat((state.positions, state.positions.new_zeros(pad)))
+        state.slots = torch.cat((state.slots, state.slots.new_full((pad,), -1)))
+        junk = [torch.full((rows + pad, h, d), NAN, dtype=dtype, device=cuda) for _ in range(8)]
+        del junk
+        out = core(*x, 0, state)
+        assert out.shape == (rows + pad, h * d)
+        assert torch.equal(out[:rows], want) and not out[rows:].any()
+
+
 def test_core_of_empty_steps(cuda):
     """A step of no row is one, with sequences or without."""
     note("core empty")
