@@ -67,12 +67,13 @@ constexpr int kRows = 32 * kWaves;   // rows of a workgroup
 // 80 + 9 us in 4 pieces, 188 whole).
 constexpr int kSlots = 512;
 constexpr int kMinUnits = 16;
-// While there is no workgroup for every CU, into pieces of 8 units and more, from
-// 24 units on (4 tokens behind 4000, 32 heads over 8: 13 + 4 us, in pieces of 16
-// 19 + 4; 19 units: 13 + 4 cut, 19 whole, less than a second launch saves).
+// While there is no workgroup for every CU, into pieces of 8 units and more (4
+// tokens behind 4000, 32 heads over 8: 13 + 4 us, in pieces of 16 19 + 4; back to
+// back in a graph 4 behind 600, 19 units: 15.8 in two pieces, 20.0 whole; 150
+// behind 500, 21 units: 19.0 and 21.9; a prompt of 520 rows of 8 heads, 17 units
+// at most: 18.9 and 18.3, of 760: 19.4 and 24.3).
 constexpr int kCus = 256;
 constexpr int kFewUnits = 8;
-constexpr int kWholeUnits = 24;
 constexpr int kMaxCut = 32;
 // Up to so many workgroups the longest go first: 7 prompts of 40 to 777 tokens,
 // 840 workgroups, take 54 us instead of 60, 12 of 420 to 655, 836 workgroups, 41
@@ -202,8 +203,7 @@ __device__ inline int key_units(const PrefillParams& p, const Place& at) {
   return (max(seen, 0) + kKeys - 1) / kKeys;
 }
 __device__ inline int pieces_of(const PrefillParams& p, int units) {
-  const int few = units < kWholeUnits ? 1 : min(p.few, units / kFewUnits);
-  return max(few, min(p.cut, units / kMinUnits));
+  return max(1, max(min(p.few, units / kFewUnits), min(p.cut, units / kMinUnits)));
 }
 
 template <typename T>
@@ -827,7 +827,6 @@ int64_t max_tiles(int64_t tokens, int64_t batch, int64_t group) {
 // Pieces of a row tile at most: of kMinUnits while two workgroups per CU are not
 // there, of kFewUnits while one is not (few).
 int64_t few_of(int64_t items, int64_t max_keys) {
-  if (ceil_div(max_keys, kKeys) < kWholeUnits) return 1;
   return std::max<int64_t>(
       1, std::min<int64_t>({kCus / items, ceil_div(max_keys, kKeys) / kFewUnits, kMaxCut}));
 }

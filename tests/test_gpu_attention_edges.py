@@ -404,3 +404,17 @@ def test_core_of_empty_steps(cuda):
     for pages, lengths, new in (([], [], []), ([[0, 1]], [22], [0])):
         state = A.AttentionState.build(pages, lengths, new, page, device=cuda)
         assert core(q, k, v, 0, state).shape == (0, h * d)
+
+
+@pytest.mark.parametrize("h,g,d,page,new,lengths", [
+    (8, 2, 128, 16, [4], [510]), (8, 2, 128, 16, [4], [512]), (8, 2, 128, 16, [4], [513]),
+    (8, 8, 64, 16, [150, 4], [650, 604]), (4, 4, 96, 32, [520], [520]),
+    (4, 1, 256, 16, [3, 0, 40], [700, 3, 41]), (3, 1, 80, 8, [760], [760])])
+def test_prompts_cut_into_a_few_pieces(cuda, h, g, d, page, new, lengths):
+    note(f"few pieces {h} {g} {d} {new} {lengths}")
+    for dtype in DTYPES:
+        k, v, table = paged(h + d, lengths, g, d, page, dtype, cuda)
+        starts = torch.tensor([0] + new).cumsum(0).to(torch.int32).to(cuda)
+        q = randn(gen_of(d), sum(new), h, d, dtype=dtype, device=cuda, std=1.7)
+        n = torch.tensor(lengths, dtype=torch.int32, device=cuda)
+        check_attention(A.paged_prefill(q, k, v, table, n, starts), q, k, v, table, n, starts)
