@@ -8,10 +8,10 @@
 //
 // Bound by memory: every key and value is read once, 4 head_dim bytes per key
 // and key head against 4 head_dim G operations.  131071 keys of 8 heads (538 MB):
-// 89 us, 6.0 TB/s, and 6 to join them; 64 sequences of 160 to 8190 keys of
-// 8 heads (1.1 GB): 194 us, 5.7 TB/s; 8 of up to 1590 keys of 32 heads (157 MB):
+// 89 us, 6.0 TB/s, and 6 to join them; 64 sequences of 229 to 8190 keys of
+// 8 heads (1.1 GB): 193 us, 5.7 TB/s; 8 of 775 to 1590 keys of 32 heads (157 MB):
 // 31 us, 5.1 TB/s.  A small call is bound by its launches: 601 keys of 32 heads
-// take 5.9 us and the join 4.2.
+// take 6.0 us and the join 4.2.
 //
 // Design:
 //   * A wavefront takes tiles of 32 keys through v_mfma_f32_16x16x32 with the
@@ -31,9 +31,12 @@
 //     registers; table entries are read a tile further ahead.
 //   * Work is cut by the keys there are, on the device: the tiles of all
 //     sequences are counted, and a sequence gets as many workgroups as its
-//     share of kDecodeSlots asks for, so uneven batches and tables wider than
-//     the lengths cost nothing.  A sequence of more than one workgroup leaves
-//     (O, r, l) per workgroup in the workspace, which join_kernel adds up.
+//     share of kDecodeSlots asks for, so uneven batches cost nothing.  A
+//     sequence of more than one workgroup leaves (O, r, l) per workgroup in the
+//     workspace, which join_kernel adds up.  Whether any may be cut the host
+//     decides, by the table's width: of one wider than the sequences' lengths the
+//     joining launch may find nothing to do, and short sequences are cut that a
+//     narrow table would leave whole (kWholeKeys).
 #include <algorithm>
 #include <type_traits>
 
@@ -46,7 +49,7 @@ namespace {
 constexpr int kTile = 32;            // keys of a wavefront's step
 constexpr int kMinTiles = 4;         // least tiles of a workgroup of several
 // Sequences up to here are not cut: joining costs a launch (300 keys, 10 tiles,
-// of 32 heads: 8.5 us whole, 5.5 + 4.4 us in pieces; 601 keys: 13 and 9.8 us).
+// of 32 heads: 8.5 us whole, 5.5 + 4.4 us in pieces; 601 keys: 13 and 6.0 + 4.2).
 constexpr int kWholeTiles = 10;
 constexpr int kDecodeSlots = 768;    // workgroups aimed at
 // Keys and values past the last-level cache's 256 MB are loaded without being
@@ -54,9 +57,10 @@ constexpr int kDecodeSlots = 768;    // workgroups aimed at
 // 19 against 17.5).
 constexpr int64_t kCached = int64_t{256} << 20;
 // A batch that gives every CU a workgroup by itself is not cut while its
-// sequences may be no longer than this: nothing is joined then, and uneven
-// lengths leave CUs idle for little time (8 sequences of 636 to 1590 keys, 32
-// heads: 32 us against 32.5 + 4.1 us cut; of 400 to 4000: 75 against 60.4 + 4.6).
+// sequences may be no longer than this, by the table's width: nothing is joined
+// then, and uneven lengths leave CUs idle for little time (8 sequences of 775 to
+// 1590 keys, 32 heads: 30 us against 36 cut, which is also what they take over a
+// table of 4096 keys; of 925 to 4000: 75 against 65).
 // With fewer than two workgroups per CU they have 8 wavefronts, else 4 (32
 // sequences of 1000 keys, 256 workgroups: 17.4 against 20.4 us; 64 of 2000, 512
 // workgroups: 85 against 73).

@@ -12,10 +12,10 @@
 // Bound by the matrix units and the exponentials together: per 32 keys and 32
 // rows of 128 elements a wavefront issues 16 matrix instructions of 32 cycles
 // and 400 to 450 cycles of vector work, which run side by side only as far as
-// the order of the instructions lets them.  8192 tokens of 32 heads: 0.59 to
-// 0.60 ms, 0.92 PFLOP/s, 77% of what a large matrix product reaches; the matrix
-// units are busy 46% of the time and the vector units 42%, at a clock that this
-// load holds at 1.9 to 2.0 GHz.  LDS is busy for a quarter of the time, so
+// the order of the instructions lets them.  8192 tokens of 32 heads: 0.58 to
+// 0.60 ms (0.64 on one card of many), 0.92 to 0.95 PFLOP/s, 77 to 79% of what a
+// large matrix product reaches; the matrix units are busy 47% of the time and
+// the vector units 42%, at a clock that this load holds at 1.9 to 2.0 GHz.  LDS is busy for a quarter of the time, so
 // copying ahead by three units instead of one changes nothing, and neither does
 // a barrier for every second unit only.
 //
@@ -41,6 +41,9 @@
 //     the last ones; the others have none.
 //   * Few rows far into a long cache are cut over its length: each piece
 //     leaves (O, r, l) in the workspace and prefill_join_kernel adds them up.
+//     Whether there may be pieces the host decides by the table's width: 560
+//     rows over a table of 2048 keys or more take 21.1 us instead of 18.8, for a
+//     join that finds nothing to do.
 //   * A masked key's probability is 0, but 0 times an infinite or NaN value is
 //     NaN.  Such values are not searched for: a row whose sums are not finite
 //     is computed again by careful_rows, key by key.
@@ -64,7 +67,7 @@ constexpr int kWaves = 4;
 constexpr int kRows = 32 * kWaves;   // rows of a workgroup
 // Below so many workgroups (two per CU) the keys are cut, into pieces of at
 // least 16 units: a join costs 4 to 9 us (512 tokens behind 7680, 32 heads over 8:
-// 80 + 9 us in 4 pieces, 188 whole).
+// 78 + 8 us in 4 pieces, 179 whole).
 constexpr int kSlots = 512;
 constexpr int kMinUnits = 16;
 // While there is no workgroup for every CU, into pieces of 8 units and more (4
@@ -75,11 +78,13 @@ constexpr int kMinUnits = 16;
 constexpr int kCus = 256;
 constexpr int kFewUnits = 8;
 constexpr int kMaxCut = 32;
-// Up to so many workgroups the longest go first: 7 prompts of 40 to 777 tokens,
-// 840 workgroups, take 54 us instead of 60, 12 of 420 to 655, 836 workgroups, 41
-// instead of 47.  More of them even out by themselves, and read less when a
-// sequence's run together (12 chunks of 40 heads, 5360 workgroups: 870 us by
-// sequence, 1165 sorted).
+// Up to so many workgroups the longest go first: 7 prompts of 146 to 777 tokens,
+// 832 workgroups, take 49 us instead of 53; 12 of 432 to 655, 822 workgroups, 36
+// instead of 43, 1264 workgroups 54 instead of 58, 1672 workgroups 69 instead of
+// 66; 12 of 98 to 655, 1168 workgroups, 46 instead of 49.  More of them even out
+// by themselves, and read less when a sequence's run together (12 chunks of 739
+// to 1400 tokens of 40 heads, 4200 workgroups: 383 us by sequence, 462 sorted;
+// 2072 workgroups: 80 and 84).
 constexpr int kSortedItems = 2048;
 constexpr int kOutside = 0x7ffffff0;   // a buffer offset past every range
 constexpr int kBufferWord3 = 0x00020000;

@@ -13,12 +13,12 @@
 // Products and sums run in binary32 with one rounding to the 16-bit type.
 //
 // Bound by memory: 2 bytes in and 2 out per element, 6 operations per pair.
-// 4097 tokens of 32 query heads and 8 key heads: 20.2 us, 5.0 TB/s.  Small calls
-// are bound by their launch: one token 3.0 us, 560 tokens of 32 and 32 heads 7.6.
+// 4097 tokens of 32 query heads and 8 key heads: 19.7 us, 5.1 TB/s.  Small calls
+// are bound by their launch: one token 3.2 us, 560 tokens of 32 and 32 heads 7.3.
 // A workgroup takes one token and up to kThreads items of it (an item is one
 // 16-byte chunk, or the two chunks of a half pair), so cos and sin are formed
 // once per workgroup by R/2 threads, in LDS, while the row loads are in flight.
-// Two items per thread, for half the sines, measure 22.1 us against 20.2.
+// Two items per thread, for half the sines, are 9% slower at 4097 tokens.
 #include <algorithm>
 
 #include "w8a8_internal.h"
