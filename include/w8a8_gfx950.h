@@ -35,7 +35,7 @@
 extern "C" {
 #endif
 
-#define W8A8_ABI_VERSION 9
+#define W8A8_ABI_VERSION 10
 
 typedef enum w8a8_dtype {
   W8A8_F32 = 0,
@@ -594,6 +594,112 @@ int w8a8_paged_prefill_padded(const void* q, int64_t q_stride_t, int64_t q_strid
 /* Workspace bytes of w8a8_paged_prefill; -1 for sizes it does not take. */
 int64_t w8a8_paged_prefill_workspace_bytes(int64_t tokens, int64_t batch, int64_t q_heads,
                                            int64_t kv_heads, int64_t head_dim, int64_t max_keys);
+
+/*
+ * w8a8_paged_decode and w8a8_paged_prefill (clear_rows nonzero: _padded) with a
+ * sliding window and sinks: a row at place i of its sequence (the last row: place
+ * lengths[b] - 1) sees the keys j <= i with j < sinks or j > i - window.
+ * window >= 1, sinks >= 0; a window of table_pages * page_size keys or more hides
+ * nothing.  Keys between the sinks and the windows of a workgroup's rows are not
+ * read, and the pages that hold only such keys need not exist: their table
+ * entries may be anything.  Workspace: w8a8_paged_*_window_workspace_bytes.
+ */
+int w8a8_paged_decode_window(const void* q, int64_t q_stride_t, int64_t q_stride_h,
+                             const void* k_cache, const void* v_cache, int64_t cache_stride_page,
+                             int64_t cache_stride_head, int64_t cache_stride_token, int64_t pages,
+                             int64_t page_size, const int32_t* page_table, int64_t ld_table,
+                             int64_t table_pages, const int32_t* lengths, int64_t window,
+                             int64_t sinks, int dtype, float scale, void* out,
+                             int64_t out_stride_t, int64_t out_stride_h, int64_t batch,
+                             int64_t q_heads, int64_t kv_heads, int64_t head_dim, void* workspace,
+                             int64_t workspace_bytes, hipStream_t stream);
+
+/* Workspace bytes of w8a8_paged_decode_window; -1 for sizes it does not take. */
+int64_t w8a8_paged_decode_window_workspace_bytes(int64_t batch, int64_t q_heads,
+                                                 int64_t kv_heads, int64_t head_dim,
+                                                 int64_t max_keys, int64_t window, int64_t sinks);
+
+int w8a8_paged_prefill_window(const void* q, int64_t q_stride_t, int64_t q_stride_h,
+                              const void* k_cache, const void* v_cache, int64_t cache_stride_page,
+                              int64_t cache_stride_head, int64_t cache_stride_token, int64_t pages,
+                              int64_t page_size, const int32_t* page_table, int64_t ld_table,
+                              int64_t table_pages, const int32_t* lengths, const int32_t* q_starts,
+                              int64_t window, int64_t sinks, int clear_rows, int dtype,
+                              float scale, void* out, int64_t out_stride_t, int64_t out_stride_h,
+                              int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                              int64_t head_dim, void* workspace, int64_t workspace_bytes,
+                              hipStream_t stream);
+
+/* Workspace bytes of w8a8_paged_prefill_window; -1 for sizes it does not take. */
+int64_t w8a8_paged_prefill_window_workspace_bytes(int64_t tokens, int64_t batch, int64_t q_heads,
+                                                  int64_t kv_heads, int64_t head_dim,
+                                                  int64_t max_keys, int64_t window,
+                                                  int64_t sinks);
+
+/*
+ * Attention of trees of drafted tokens over the paged cache.  Rows q_starts[b] ..
+ * q_starts[b + 1] - 1 of q (n of them) are drafted tokens of sequence b, whose
+ * keys, the last n of its lengths[b], the cache already holds.  Each row sees all
+ * lengths[b] - n keys before them and, of the drafted ones, key j where bit j % 64
+ * of masks[row * ld_masks + j / 64] is set (its own among them only if its bit
+ * is); key j of 64 * mask_words or more is not seen.  A row that sees no key is
+ * zeros; clear_rows nonzero: so are rows of no sequence, else they are left as
+ * they were.  Otherwise as w8a8_paged_prefill.
+ */
+int w8a8_paged_tree(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_cache,
+                    const void* v_cache, int64_t cache_stride_page, int64_t cache_stride_head,
+                    int64_t cache_stride_token, int64_t pages, int64_t page_size,
+                    const int32_t* page_table, int64_t ld_table, int64_t table_pages,
+                    const int32_t* lengths, const int32_t* q_starts, const uint64_t* masks,
+                    int64_t ld_masks, int64_t mask_words, int clear_rows, int dtype, float scale,
+                    void* out, int64_t out_stride_t, int64_t out_stride_h, int64_t tokens,
+                    int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                    void* workspace, int64_t workspace_bytes, hipStream_t stream);
+
+/* Workspace bytes of w8a8_paged_tree; -1 for sizes it does not take. */
+int64_t w8a8_paged_tree_workspace_bytes(int64_t tokens, int64_t batch, int64_t q_heads,
+                                        int64_t kv_heads, int64_t head_dim, int64_t max_keys);
+
+/*
+ * Keeps the accepted path of each sequence's drafted tokens: in `layers` caches
+ * (cache_stride_layer elements apart, one launch) the key and value of drafted
+ * token path[b * ld_path + i] go from place lengths[b] + path to place
+ * lengths[b] + i, where lengths[b] keys were cached before the draft.  path
+ * entries rise; one below i (behind the path's end: -1) moves nothing, and
+ * neither does a place past the table or in a page outside [0, pages).  The pages
+ * of places from lengths[b] on belong to one sequence only.  batch <= 65535,
+ * layers <= 32767; a layer's k and v may lie side by side ([layers, 2, ...]).
+ */
+int w8a8_cache_accept(void* k_cache, void* v_cache, int64_t cache_stride_layer,
+                      int64_t cache_stride_page, int64_t cache_stride_head,
+                      int64_t cache_stride_token, int64_t layers, int64_t pages,
+                      int64_t page_size, const int32_t* page_table, int64_t ld_table,
+                      int64_t table_pages, const int32_t* lengths, const int32_t* path,
+                      int64_t ld_path, int64_t path_length, int dtype, int64_t batch,
+                      int64_t kv_heads, int64_t head_dim, hipStream_t stream);
+
+/*
+ * Log probabilities of given tokens from logits [rows, ld_logits] of `vocab`
+ * columns (W8A8_F16, W8A8_BF16 or W8A8_F32, any alignment of the type):
+ *   logprobs[r, i] = x[t] - log sum_j exp(x[j]),  t = tokens[r * ld_tokens + i]
+ * for `given` tokens a row (0: none); token -1 (a padded place) gives 0, any
+ * other outside [0, vocab) NaN.  entropy[r] (nullable): -sum p log p in nats.
+ * top_tokens[r, k] and top_logprobs[r, k], k < top <= min(64, vocab): the largest
+ * logits' tokens, largest first, equal ones by their number (a NaN counts as the
+ * largest).  All results are binary32 from binary32 sums; -inf logits have
+ * probability 0, a row with +inf, NaN or nothing above -inf gives NaN.
+ * rows < 2^22, vocab <= 2^20; outputs are contiguous and overlap nothing.
+ * Workspace: w8a8_token_logprobs_workspace_bytes(rows, vocab, top, dtype) bytes,
+ * 16-byte aligned; no state survives the call.
+ */
+int w8a8_token_logprobs(const void* logits, int64_t ld_logits, int dtype, const int64_t* tokens,
+                        int64_t ld_tokens, int64_t given, int64_t top, float* logprobs,
+                        float* entropy, float* top_logprobs, int64_t* top_tokens, int64_t rows,
+                        int64_t vocab, void* workspace, int64_t workspace_bytes,
+                        hipStream_t stream);
+
+/* Workspace bytes of w8a8_token_logprobs; -1 for sizes it does not take. */
+int64_t w8a8_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int64_t top, int dtype);
 
 #ifdef __cplusplus
 }

@@ -77,6 +77,7 @@ struct DecodeParams {
   int rows;        // query rows of a workgroup: min(group, 16)
   bool whole;      // no sequence is cut
   bool large;      // with whole: the batch's keys and values may pass kCached
+  int window, sinks;   // of a windowed call
   float* part_o;   // [pieces x units, rows, head_dim]
   f32x2* part_rl;  // [pieces x units, rows]
 };
@@ -94,19 +95,39 @@ struct Piece {
   int seq;     // the sequence, or -1
   int first;   // its first piece
   int count;   // its pieces
-  int tiles;   // its tiles
+  int tiles;   // its tiles, of a windowed call those that are seen
   int keys;    // its keys
   bool large;  // the batch's keys and values pass kCached
 };
 
+// Of a windowed call: the tiles of a sequence that hold a seen key, in order: its
+// first `head` tiles and, from tile head + skip on, the others.
+struct Tiles {
+  int low;    // the first key of the window
+  int head;
+  int skip;
+  int count;
+};
+__device__ inline Tiles window_tiles(const DecodeParams& p, int keys) {
+  const int low = max(keys - p.window, 0);
+  const int all = (keys + kTile - 1) / kTile;
+  const int head = (min(p.sinks, low) + kTile - 1) / kTile;
+  const int from = max(low / kTile, head);
+  return Tiles{low, head, from - head, all - from + head};
+}
+
 // The sequence of piece `slot`, or the pieces of sequence `seq` (slot < 0).
 // Every lane of the wavefront takes part and gets the same answer, in scalar
 // registers.  A lane's tiles stay below 2^26, so 64 of them fit 32 bits.
+template <bool WINDOW>
 __device__ inline Piece find_piece(const DecodeParams& p, int slot, int seq) {
   const int lane = threadIdx.x & 63;
   const int batch = p.a.batch;
   auto keys_of = [&](int b) { return b < batch ? max(0, min(p.a.lengths[b], p.a.max_keys)) : 0; };
-  auto tiles_of = [](int keys) { return static_cast<uint32_t>(keys + kTile - 1) / kTile; };
+  auto tiles_of = [&](int keys) {
+    if constexpr (WINDOW) return static_cast<uint32_t>(window_tiles(p, keys).count);
+    return static_cast<uint32_t>(keys + kTile - 1) / kTile;
+  };
   if (p.whole) {
     const int at = slot >= 0 ? slot : seq;
     const int keys = max(0, min(p.a.lengths[at], p.a.max_keys));
@@ -149,8 +170,8 @@ __device__ inline void write_out(const DecodeParams& p, int seq, int head, int d
 
 // DP: head_dim rounded up to 64, 128 or 256; FULL: head_dim == DP.  SMALL:
 // pages of fewer than 4 keys, so that each key has a table entry of its own.
-// W: wavefronts.
-template <typename T, int DP, bool FULL, bool SMALL, int W>
+// W: wavefronts.  WINDOW: the keys between the sinks and the window are not seen.
+template <typename T, int DP, bool FULL, bool SMALL, int W, bool WINDOW>
 __global__ __launch_bounds__(64 * W, DP == 256 ? 1 : 2) void decode_kernel(DecodeParams p) {
   constexpr int KS = DP / 32;   // first product: steps over the head
   constexpr int DV = DP / 16;   // elements of a value row per lane
@@ -164,11 +185,16 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 1 : 2) void decode_kernel(Decod
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, g = lane >> 4;
   const int slot = blockIdx.x / p.units, unit = blockIdx.x % p.units;
-  const Piece piece = find_piece(p, slot, -1);
+  const Piece piece = find_piece<WINDOW>(p, slot, -1);
   const int seq = piece.seq, count = piece.count;
   const int tiles = __builtin_amdgcn_readfirstlane(piece.tiles);
   const int keys = __builtin_amdgcn_readfirstlane(piece.keys);
   if (seq < 0) return;
+  Tiles seen{0, tiles, 0, tiles};
+  if constexpr (WINDOW) seen = window_tiles(p, keys);
+  // The first key of the piece's tile t, and whether key j is seen.
+  auto key_of = [&](int t) { return (WINDOW && t >= seen.head ? t + seen.skip : t) * kTile; };
+  auto is_seen = [&](int j) { return j < keys && (!WINDOW || j >= seen.low || j < p.sinks); };
   const int part = slot - piece.first;
   const int t0 = static_cast<int>(static_cast<int64_t>(tiles) * part / count);
   const int t1 = static_cast<int>(static_cast<int64_t>(tiles) * (part + 1) / count);
@@ -205,16 +231,22 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 1 : 2) void decode_kernel(Decod
   };
   auto entry = [&](int j) {
     int e = -1;
-    if (j < keys) e = table[j >> a.page_shift];
+    if (is_seen(j)) e = table[j >> a.page_shift];
+    return e;
+  };
+  // Of the page of keys j .. j + 3, any of which may be the first of the window.
+  auto entry_of_four = [&](int j) {
+    int e = -1;
+    if (j < keys && (!WINDOW || j + 3 >= seen.low || j < p.sinks)) e = table[j >> a.page_shift];
     return e;
   };
   auto lookup = [&](int t, Entries& e) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) e.k[h] = entry(t * kTile + 16 * h + r);
+    for (int h = 0; h < 2; ++h) e.k[h] = entry(key_of(t) + 16 * h + r);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      e.v[i] = SMALL ? entry(t * kTile + (i < 4 ? 0 : 16) + 4 * g + (i & 3))
-                     : entry(t * kTile + 16 * i + 4 * g);
+      e.v[i] = SMALL ? entry(key_of(t) + (i < 4 ? 0 : 16) + 4 * g + (i & 3))
+                     : entry_of_four(key_of(t) + 16 * i + 4 * g);
   };
   // A key that is not there reads row 0 of page 0 instead.
   auto row_of = [&](int e, int j) {
@@ -229,7 +261,7 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 1 : 2) void decode_kernel(Decod
   auto issue = [&](auto once, int t, const Entries& e, Tile& x) __attribute__((always_inline)) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint16_t* src = kb + row_of(e.k[h], t * kTile + 16 * h + r);
+      const uint16_t* src = kb + row_of(e.k[h], key_of(t) + 16 * h + r);
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         if constexpr (FULL) {
@@ -243,9 +275,9 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 1 : 2) void decode_kernel(Decod
     x.ok = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int j = t * kTile + (i < 4 ? 0 : 16) + 4 * g + (i & 3);
+      const int j = key_of(t) + (i < 4 ? 0 : 16) + 4 * g + (i & 3);
       const int ev = e.v[SMALL ? i : i >> 2];
-      const bool there = j < keys && ev >= 0 && ev < pages;
+      const bool there = is_seen(j) && ev >= 0 && ev < pages;
       x.ok |= static_cast<uint32_t>(there) << i;
       const uint16_t* src = vb + row_of(there ? ev : -1, j);
       if constexpr (VW == 2) {
@@ -389,12 +421,17 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 1 : 2) void decode_kernel(Decod
     constexpr int N = 16;
     bool up = false, down = false, nan = false;
     const T* v = static_cast<const T*>(a.v) + kvh * a.c_head + d;
-    const int last = min(t1 * kTile, keys);
-    for (int j0 = t0 * kTile; j0 < last; j0 += N) {
+    const int last = t1 > t0 ? min(key_of(t1 - 1) + kTile, keys) : 0;
+    for (int i0 = t0 * kTile; i0 < t1 * kTile; i0 += N) {
+      const int j0 = key_of(i0 / kTile) + i0 % kTile;
+      if (j0 >= last) break;
       int e[N];
       T y[N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) e[i] = table[min(j0 + i, last - 1) >> a.page_shift];
+      for (int i = 0; i < N; ++i) {
+        const int j = min(j0 + i, last - 1);
+        e[i] = !WINDOW || is_seen(j) ? table[j >> a.page_shift] : -1;
+      }
 #pragma unroll
       for (int i = 0; i < N; ++i) y[i] = v[row_of(e[i], min(j0 + i, last - 1))];
 #pragma unroll
@@ -442,7 +479,7 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 1 : 2) void decode_kernel(Decod
 // One workgroup per query row: adds up what the pieces of its sequence left.
 // A thread takes four elements of every eighth (D = 128) piece, the first
 // kJoinAhead of them in flight while the weights are formed.
-template <typename T, int DP>
+template <typename T, int DP, bool WINDOW>
 __global__ __launch_bounds__(kJoinThreads) void join_kernel(DecodeParams p) {
   constexpr int C = DP / 4;              // threads of a row
   constexpr int R = kJoinThreads / C;    // rows at a time
@@ -452,7 +489,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(DecodeParams p) {
   __shared__ float red[2][W];
   const int seq = blockIdx.x, head = blockIdx.y, tid = threadIdx.x;
   const int D = p.a.head_dim;
-  const Piece piece = find_piece(p, -1, seq);
+  const Piece piece = find_piece<WINDOW>(p, -1, seq);
   const int n = piece.count;
   if (n <= 1) return;
   const int q = head % p.group;
@@ -512,34 +549,34 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(DecodeParams p) {
   }
 }
 
-template <typename T, int DP, bool FULL>
+template <typename T, int DP, bool FULL, bool WINDOW>
 hipError_t launch_d(const DecodeParams& p, int64_t pieces, hipStream_t st) {
   const dim3 grid(static_cast<uint32_t>(pieces * p.units));
   const bool small = p.a.page_shift < 2;
   // Heads past 128 take too many registers for two wavefronts of a SIMD.
   if (DP <= 128 && !small && p.whole && grid.x < 2 * kCus)
-    hipLaunchKernelGGL((decode_kernel<T, DP, FULL, false, DP <= 128 ? 8 : 4>), grid,
+    hipLaunchKernelGGL((decode_kernel<T, DP, FULL, false, DP <= 128 ? 8 : 4, WINDOW>), grid,
                        dim3(64 * (DP <= 128 ? 8 : 4)), 0, st, p);
   else if (small)
-    hipLaunchKernelGGL((decode_kernel<T, DP, FULL, true, 4>), grid, dim3(256), 0, st, p);
+    hipLaunchKernelGGL((decode_kernel<T, DP, FULL, true, 4, WINDOW>), grid, dim3(256), 0, st, p);
   else
-    hipLaunchKernelGGL((decode_kernel<T, DP, FULL, false, 4>), grid, dim3(256), 0, st, p);
+    hipLaunchKernelGGL((decode_kernel<T, DP, FULL, false, 4, WINDOW>), grid, dim3(256), 0, st, p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || pieces == p.a.batch) return e;
-  hipLaunchKernelGGL((join_kernel<T, DP>), dim3(p.a.batch, p.a.q_heads), dim3(kJoinThreads), 0, st,
+  hipLaunchKernelGGL((join_kernel<T, DP, WINDOW>), dim3(p.a.batch, p.a.q_heads), dim3(kJoinThreads), 0, st,
                      p);
   return hipGetLastError();
 }
 
-template <typename T>
+template <typename T, bool WINDOW>
 hipError_t launch_t(const DecodeParams& p, int64_t pieces, hipStream_t st) {
   const int d = p.a.head_dim;
-  if (d == 64) return launch_d<T, 64, true>(p, pieces, st);
-  if (d < 64) return launch_d<T, 64, false>(p, pieces, st);
-  if (d == 128) return launch_d<T, 128, true>(p, pieces, st);
-  if (d < 128) return launch_d<T, 128, false>(p, pieces, st);
-  if (d == 256) return launch_d<T, 256, true>(p, pieces, st);
-  return launch_d<T, 256, false>(p, pieces, st);
+  if (d == 64) return launch_d<T, 64, true, WINDOW>(p, pieces, st);
+  if (d < 64) return launch_d<T, 64, false, WINDOW>(p, pieces, st);
+  if (d == 128) return launch_d<T, 128, true, WINDOW>(p, pieces, st);
+  if (d < 128) return launch_d<T, 128, false, WINDOW>(p, pieces, st);
+  if (d == 256) return launch_d<T, 256, true, WINDOW>(p, pieces, st);
+  return launch_d<T, 256, false, WINDOW>(p, pieces, st);
 }
 
 int64_t units_of(int64_t q_heads, int64_t kv_heads) {
@@ -549,10 +586,8 @@ int64_t units_of(int64_t q_heads, int64_t kv_heads) {
 // Bytes of the (r, l) pairs in front of the O rows.
 int64_t pairs_bytes(int64_t items, int64_t rows) { return ceil_div(items * rows * 8, 256) * 256; }
 
-}  // namespace
-
-int64_t paged_decode_workspace(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
-                               int64_t max_keys) {
+int64_t workspace_of(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                     int64_t max_keys) {
   const int64_t units = units_of(q_heads, kv_heads);
   const int64_t pieces = max_pieces(batch, units, max_keys);
   if (pieces <= batch) return 0;
@@ -560,20 +595,55 @@ int64_t paged_decode_workspace(int64_t batch, int64_t q_heads, int64_t kv_heads,
   return pairs_bytes(items, rows) + items * rows * head_dim * 4;
 }
 
-hipError_t launch_paged_decode(const PagedAttention& a, int dtype, hipStream_t st) {
-  DecodeParams p;
+// keys: what workspace_of was asked with.
+template <bool WINDOW>
+hipError_t launch(DecodeParams& p, const PagedAttention& a, int64_t keys, int dtype,
+                  hipStream_t st) {
   p.a = a;
   p.group = a.q_heads / a.kv_heads;
   p.blocks = static_cast<int>(ceil_div(p.group, 16));
   p.units = a.kv_heads * p.blocks;
   p.rows = std::min(p.group, 16);
-  const int64_t pieces = max_pieces(a.batch, p.units, a.max_keys);
+  const int64_t pieces = max_pieces(a.batch, p.units, keys);
   p.whole = pieces == a.batch;
-  p.large = 4.0 * a.batch * a.max_keys * a.kv_heads * a.head_dim > static_cast<double>(kCached);
+  p.large = 4.0 * a.batch * keys * a.kv_heads * a.head_dim > static_cast<double>(kCached);
   char* ws = static_cast<char*>(a.workspace);
   p.part_rl = reinterpret_cast<f32x2*>(ws);
   p.part_o = reinterpret_cast<float*>(ws + pairs_bytes(pieces * p.units, p.rows));
-  return dtype == kF16 ? launch_t<__half>(p, pieces, st) : launch_t<__hip_bfloat16>(p, pieces, st);
+  return dtype == kF16 ? launch_t<__half, WINDOW>(p, pieces, st)
+                       : launch_t<__hip_bfloat16, WINDOW>(p, pieces, st);
+}
+
+// The keys of the tiles that a row sees at most: all, or those of the sinks and of
+// the window.
+int64_t seen_keys(int64_t max_keys, int64_t window, int64_t sinks) {
+  return std::min(max_keys, (ceil_div(sinks, kTile) + ceil_div(window, kTile) + 1) * kTile);
+}
+
+}  // namespace
+
+int64_t paged_decode_workspace(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                               int64_t max_keys) {
+  return workspace_of(batch, q_heads, kv_heads, head_dim, max_keys);
+}
+
+int64_t paged_decode_window_workspace(int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                      int64_t head_dim, int64_t max_keys, int64_t window,
+                                      int64_t sinks) {
+  return workspace_of(batch, q_heads, kv_heads, head_dim, seen_keys(max_keys, window, sinks));
+}
+
+hipError_t launch_paged_decode(const PagedAttention& a, int dtype, hipStream_t st) {
+  DecodeParams p{};
+  return launch<false>(p, a, a.max_keys, dtype, st);
+}
+
+hipError_t launch_paged_decode_window(const PagedAttention& a, int window, int sinks, int dtype,
+                                      hipStream_t st) {
+  DecodeParams p{};
+  p.window = window;
+  p.sinks = sinks;
+  return launch<true>(p, a, seen_keys(a.max_keys, window, sinks), dtype, st);
 }
 
 }  // namespace w8a8

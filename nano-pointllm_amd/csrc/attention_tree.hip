@@ -1,0 +1,21 @@
+// Attention of trees of drafted tokens (attention_prefill.h): a sequence's rows
+// see all of its cached keys and, by a mask, each other's.
+#include "attention_prefill.h"
+
+namespace w8a8 {
+
+int64_t paged_tree_workspace(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                             int64_t head_dim, int64_t max_keys) {
+  return workspace_of(tokens, batch, q_heads, kv_heads, head_dim, max_keys);
+}
+
+hipError_t launch_paged_tree(const PagedAttention& a, const uint64_t* masks, int64_t ld_masks,
+                             int words, bool clear, int dtype, hipStream_t st) {
+  PrefillParams p{};
+  p.masks = masks;
+  p.ld_masks = ld_masks;
+  p.words = words;
+  return launch<Seen::kTree>(p, a, a.max_keys, clear, dtype, st);
+}
+
+}  // namespace w8a8

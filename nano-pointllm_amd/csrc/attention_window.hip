@@ -1,0 +1,24 @@
+// Attention of prompts and prompt chunks of which a row sees its last `window`
+// keys and the sequence's first `sinks` (attention_prefill.h): the units of keys
+// between the two are neither read nor computed, nor are their pages looked up.
+#include "attention_prefill.h"
+
+namespace w8a8 {
+
+int64_t paged_prefill_window_workspace(int64_t tokens, int64_t batch, int64_t q_heads,
+                                       int64_t kv_heads, int64_t head_dim, int64_t max_keys,
+                                       int64_t window, int64_t sinks) {
+  return workspace_of(tokens, batch, q_heads, kv_heads, head_dim,
+                      seen_keys(max_keys, q_heads / kv_heads, window, sinks));
+}
+
+hipError_t launch_paged_prefill_window(const PagedAttention& a, int window, int sinks, bool clear,
+                                       int dtype, hipStream_t st) {
+  PrefillParams p{};
+  p.window = window;
+  p.sinks = sinks;
+  return launch<Seen::kWindow>(p, a, seen_keys(a.max_keys, a.q_heads / a.kv_heads, window, sinks),
+                               clear, dtype, st);
+}
+
+}  // namespace w8a8

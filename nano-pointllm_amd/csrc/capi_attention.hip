@@ -1,6 +1,9 @@
 // extern "C" entry points of the attention core (declared in
 // include/w8a8_gfx950.h): argument checks and dispatch.  The kernels live in
-// rotary.hip, attention_decode.hip and attention_prefill.hip.
+// rotary.hip, attention_decode.hip, attention_prefill.h and cache_accept.hip.
+#include <algorithm>
+#include <utility>
+
 #include "w8a8_gfx950.h"
 #include "w8a8_internal.h"
 
@@ -19,6 +22,7 @@ constexpr int64_t kMaxTokens = INT32_MAX - 4096;
 constexpr int64_t kMaxHeads = 4096;
 // Workgroups of 256 threads; a launch's threads are counted in 32 bits.
 constexpr int64_t kMaxBlocks = UINT32_MAX / 256;
+constexpr int64_t kMaxGridYZ = 65535;
 constexpr int64_t kMaxStride = int64_t{1} << 60;
 constexpr i128 kMaxBytes = i128(1) << 62;  // of any tensor's address range
 
@@ -73,16 +77,16 @@ inline i128 cache_bytes(const Cache& c) {
               i128(c.page_size - 1) * c.c_tok + c.dim);
 }
 
-// Whether no two rows of the cache share an element: each stride covers the
-// extent of the axes with smaller strides.
-inline bool cache_distinct(const Cache& c) {
-  int64_t stride[3] = {c.c_page, c.c_head, c.c_tok};
-  int64_t count[3] = {c.pages, c.heads, c.page_size};
+// Whether no two rows of the cache, or of `layers` of them at a stride, share an
+// element: each stride covers the extent of the axes with smaller strides.
+inline bool cache_distinct(const Cache& c, int64_t c_layer = 0, int64_t layers = 1) {
+  int64_t stride[4] = {c_layer, c.c_page, c.c_head, c.c_tok};
+  int64_t count[4] = {layers, c.pages, c.heads, c.page_size};
   i128 extent = c.dim;
-  bool used[3] = {};
-  for (int n = 0; n < 3; ++n) {
+  bool used[4] = {};
+  for (int n = 0; n < 4; ++n) {
     int best = -1;
-    for (int i = 0; i < 3; ++i)
+    for (int i = 0; i < 4; ++i)
       if (!used[i] && (best < 0 || stride[i] < stride[best])) best = i;
     used[best] = true;
     if (count[best] > 1) {
@@ -97,6 +101,19 @@ inline bool clear_of(const Rows& r, const void* cache, const Cache& c) {
   if (r.p == nullptr || cache == nullptr) return true;
   const i128 a0 = begin_of(r), b0 = i128(reinterpret_cast<uintptr_t>(cache));
   return a0 + bytes_of(r) <= b0 || b0 + cache_bytes(c) <= a0;
+}
+
+// Whether k and v share no element: apart, or each inside the other's gaps
+// between layers (one tensor [layers, 2, ...]).
+inline bool caches_apart(const void* k, const void* v, const Cache& c, int64_t stride,
+                         int64_t layers) {
+  const i128 a = i128(reinterpret_cast<uintptr_t>(k)), b = i128(reinterpret_cast<uintptr_t>(v));
+  const i128 one = cache_bytes(c), all = one + 2 * i128(layers - 1) * stride;
+  if (a + all <= b || b + all <= a) return true;
+  if (layers == 1) return false;
+  const i128 step = 2 * i128(stride);
+  const i128 off = (((b - a) % step) + step) % step;
+  return off >= one && off + one <= step;
 }
 
 // log2 of a power of two up to 2^20, or -1.
@@ -311,8 +328,37 @@ bool sizes_ok(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, 
          head_dim <= kAttentionMaxDim && max_keys >= 0 && max_keys <= kMaxTokens;
 }
 
-// Both prefill entry points; clear: rows of no sequence become zeros.
-int paged_prefill(bool clear, const void* q, int64_t q_stride_t, int64_t q_stride_h,
+// What a row sees: all keys up to its own place, or of those the first `sinks`
+// and the last `window`, or by the masks of a tree.
+struct Sight {
+  int64_t window = 0, sinks = 0;
+  bool windowed = false;
+  bool tree = false;
+  const uint64_t* masks = nullptr;
+  int64_t ld_masks = 0, words = 0;
+};
+
+// A window that no table's keys pass hides nothing, whatever the lengths.
+bool window_ok(int64_t window, int64_t sinks) { return window >= 1 && sinks >= 0; }
+Sight window_of(int64_t window, int64_t sinks, int64_t max_keys) {
+  Sight s;
+  s.windowed = window < max_keys;
+  s.window = std::min(window, max_keys);
+  s.sinks = std::min(sinks, max_keys);
+  return s;
+}
+
+int64_t prefill_workspace(const Sight& s, int64_t tokens, int64_t batch, int64_t q_heads,
+                          int64_t kv_heads, int64_t head_dim, int64_t max_keys) {
+  if (s.windowed)
+    return paged_prefill_window_workspace(tokens, batch, q_heads, kv_heads, head_dim, max_keys,
+                                          s.window, s.sinks);
+  if (s.tree) return paged_tree_workspace(tokens, batch, q_heads, kv_heads, head_dim, max_keys);
+  return paged_prefill_workspace(tokens, batch, q_heads, kv_heads, head_dim, max_keys);
+}
+
+// All prefill entry points; clear: rows of no sequence become zeros.
+int paged_prefill(Sight sight, bool clear, const void* q, int64_t q_stride_t, int64_t q_stride_h,
                   const void* k_cache, const void* v_cache, int64_t cache_stride_page,
                   int64_t cache_stride_head, int64_t cache_stride_token, int64_t pages,
                   int64_t page_size, const int32_t* page_table, int64_t ld_table,
@@ -331,13 +377,62 @@ int paged_prefill(bool clear, const void* q, int64_t q_stride_t, int64_t q_strid
   if (batch == 0) return clear ? W8A8_ERR_SHAPE : W8A8_OK;
   if (q_starts == nullptr) return W8A8_ERR_NULL;
   if (!aligned(q_starts, 4)) return W8A8_ERR_ALIGN;
+  if (sight.windowed) sight = window_of(sight.window, sight.sinks, p.max_keys);
+  if (sight.tree) {
+    if (sight.words > 0 && sight.masks == nullptr) return W8A8_ERR_NULL;
+    if (!aligned(sight.masks, 8)) return W8A8_ERR_ALIGN;
+    const Rows orr{out, out_stride_t, out_stride_h, tokens, q_heads, head_dim};
+    const i128 m0 = i128(reinterpret_cast<uintptr_t>(sight.masks));
+    const i128 m1 = m0 + 8 * (i128(tokens - 1) * sight.ld_masks + sight.words);
+    if (m1 - m0 > kMaxBytes) return W8A8_ERR_SHAPE;
+    if (sight.words > 0 && m0 < begin_of(orr) + bytes_of(orr) && begin_of(orr) < m1)
+      return W8A8_ERR_OVERLAP;
+  }
   const int64_t need =
-      paged_prefill_workspace(tokens, batch, q_heads, kv_heads, head_dim, p.max_keys);
+      prefill_workspace(sight, tokens, batch, q_heads, kv_heads, head_dim, p.max_keys);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return W8A8_ERR_WORKSPACE;
   if (need > 0 && !aligned(workspace, 16)) return W8A8_ERR_ALIGN;
   p.workspace = workspace;
   p.q_starts = q_starts;
+  if (sight.tree)
+    return status_of(launch_paged_tree(p, sight.masks, sight.ld_masks,
+                                       static_cast<int>(sight.words), clear, dtype, stream));
+  if (sight.windowed)
+    return status_of(launch_paged_prefill_window(p, static_cast<int>(sight.window),
+                                                 static_cast<int>(sight.sinks), clear, dtype,
+                                                 stream));
   return status_of(launch_paged_prefill(p, clear, dtype, stream));
+}
+
+// Both decode entry points.
+int paged_decode(Sight sight, const void* q, int64_t q_stride_t, int64_t q_stride_h,
+                 const void* k_cache, const void* v_cache, int64_t cache_stride_page,
+                 int64_t cache_stride_head, int64_t cache_stride_token, int64_t pages,
+                 int64_t page_size, const int32_t* page_table, int64_t ld_table,
+                 int64_t table_pages, const int32_t* lengths, int dtype, float scale, void* out,
+                 int64_t out_stride_t, int64_t out_stride_h, int64_t batch, int64_t q_heads,
+                 int64_t kv_heads, int64_t head_dim, void* workspace, int64_t workspace_bytes,
+                 hipStream_t stream) {
+  const Cache c{cache_stride_page, cache_stride_head, cache_stride_token, pages,
+                page_size,         kv_heads,          head_dim};
+  PagedAttention p;
+  const int rc = check_attention(p, q, q_stride_t, q_stride_h, k_cache, v_cache, c, page_table,
+                                 ld_table, table_pages, lengths, dtype, scale, out, out_stride_t,
+                                 out_stride_h, batch, batch, q_heads, kDecodeRows);
+  if (rc != W8A8_OK || batch == 0) return rc;
+  if (sight.windowed) sight = window_of(sight.window, sight.sinks, p.max_keys);
+  const int64_t need =
+      sight.windowed ? paged_decode_window_workspace(batch, q_heads, kv_heads, head_dim,
+                                                     p.max_keys, sight.window, sight.sinks)
+                     : paged_decode_workspace(batch, q_heads, kv_heads, head_dim, p.max_keys);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return W8A8_ERR_WORKSPACE;
+  if (need > 0 && !aligned(workspace, 16)) return W8A8_ERR_ALIGN;
+  p.workspace = workspace;
+  p.q_starts = nullptr;
+  if (sight.windowed)
+    return status_of(launch_paged_decode_window(p, static_cast<int>(sight.window),
+                                                static_cast<int>(sight.sinks), dtype, stream));
+  return status_of(launch_paged_decode(p, dtype, stream));
 }
 
 }  // namespace
@@ -358,19 +453,11 @@ int w8a8_paged_decode(const void* q, int64_t q_stride_t, int64_t q_stride_h, con
                       int64_t out_stride_t, int64_t out_stride_h, int64_t batch, int64_t q_heads,
                       int64_t kv_heads, int64_t head_dim, void* workspace,
                       int64_t workspace_bytes, hipStream_t stream) {
-  const Cache c{cache_stride_page, cache_stride_head, cache_stride_token, pages,
-                page_size,         kv_heads,          head_dim};
-  PagedAttention p;
-  const int rc = check_attention(p, q, q_stride_t, q_stride_h, k_cache, v_cache, c, page_table,
-                                 ld_table, table_pages, lengths, dtype, scale, out, out_stride_t,
-                                 out_stride_h, batch, batch, q_heads, kDecodeRows);
-  if (rc != W8A8_OK || batch == 0) return rc;
-  const int64_t need = paged_decode_workspace(batch, q_heads, kv_heads, head_dim, p.max_keys);
-  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return W8A8_ERR_WORKSPACE;
-  if (need > 0 && !aligned(workspace, 16)) return W8A8_ERR_ALIGN;
-  p.workspace = workspace;
-  p.q_starts = nullptr;
-  return status_of(launch_paged_decode(p, dtype, stream));
+  return paged_decode(Sight{}, q, q_stride_t, q_stride_h, k_cache, v_cache, cache_stride_page,
+                      cache_stride_head, cache_stride_token, pages, page_size, page_table,
+                      ld_table, table_pages, lengths, dtype, scale, out, out_stride_t,
+                      out_stride_h, batch, q_heads, kv_heads, head_dim, workspace,
+                      workspace_bytes, stream);
 }
 
 int64_t w8a8_paged_prefill_workspace_bytes(int64_t tokens, int64_t batch, int64_t q_heads,
@@ -388,7 +475,7 @@ int w8a8_paged_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, co
                        void* out, int64_t out_stride_t, int64_t out_stride_h, int64_t tokens,
                        int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                        void* workspace, int64_t workspace_bytes, hipStream_t stream) {
-  return paged_prefill(false, q, q_stride_t, q_stride_h, k_cache, v_cache, cache_stride_page,
+  return paged_prefill(Sight{}, false, q, q_stride_t, q_stride_h, k_cache, v_cache, cache_stride_page,
                        cache_stride_head, cache_stride_token, pages, page_size, page_table,
                        ld_table, table_pages, lengths, q_starts, dtype, scale, out, out_stride_t,
                        out_stride_h, tokens, batch, q_heads, kv_heads, head_dim, workspace,
@@ -404,11 +491,175 @@ int w8a8_paged_prefill_padded(const void* q, int64_t q_stride_t, int64_t q_strid
                               int64_t out_stride_h, int64_t tokens, int64_t batch, int64_t q_heads,
                               int64_t kv_heads, int64_t head_dim, void* workspace,
                               int64_t workspace_bytes, hipStream_t stream) {
-  return paged_prefill(true, q, q_stride_t, q_stride_h, k_cache, v_cache, cache_stride_page,
+  return paged_prefill(Sight{}, true, q, q_stride_t, q_stride_h, k_cache, v_cache, cache_stride_page,
                        cache_stride_head, cache_stride_token, pages, page_size, page_table,
                        ld_table, table_pages, lengths, q_starts, dtype, scale, out, out_stride_t,
                        out_stride_h, tokens, batch, q_heads, kv_heads, head_dim, workspace,
                        workspace_bytes, stream);
+}
+
+int64_t w8a8_paged_decode_window_workspace_bytes(int64_t batch, int64_t q_heads,
+                                                 int64_t kv_heads, int64_t head_dim,
+                                                 int64_t max_keys, int64_t window,
+                                                 int64_t sinks) {
+  if (!sizes_ok(batch, batch, q_heads, kv_heads, head_dim, max_keys, kDecodeRows) ||
+      !window_ok(window, sinks))
+    return -1;
+  const Sight s = window_of(window, sinks, max_keys);
+  return s.windowed ? paged_decode_window_workspace(batch, q_heads, kv_heads, head_dim, max_keys,
+                                                    s.window, s.sinks)
+                    : paged_decode_workspace(batch, q_heads, kv_heads, head_dim, max_keys);
+}
+
+int w8a8_paged_decode_window(const void* q, int64_t q_stride_t, int64_t q_stride_h,
+                             const void* k_cache, const void* v_cache, int64_t cache_stride_page,
+                             int64_t cache_stride_head, int64_t cache_stride_token, int64_t pages,
+                             int64_t page_size, const int32_t* page_table, int64_t ld_table,
+                             int64_t table_pages, const int32_t* lengths, int64_t window,
+                             int64_t sinks, int dtype, float scale, void* out,
+                             int64_t out_stride_t, int64_t out_stride_h, int64_t batch,
+                             int64_t q_heads, int64_t kv_heads, int64_t head_dim, void* workspace,
+                             int64_t workspace_bytes, hipStream_t stream) {
+  if (!window_ok(window, sinks)) return W8A8_ERR_SHAPE;
+  Sight s;
+  s.windowed = true;
+  s.window = window;
+  s.sinks = sinks;
+  return paged_decode(s, q, q_stride_t, q_stride_h, k_cache, v_cache, cache_stride_page,
+                      cache_stride_head, cache_stride_token, pages, page_size, page_table,
+                      ld_table, table_pages, lengths, dtype, scale, out, out_stride_t,
+                      out_stride_h, batch, q_heads, kv_heads, head_dim, workspace,
+                      workspace_bytes, stream);
+}
+
+int64_t w8a8_paged_prefill_window_workspace_bytes(int64_t tokens, int64_t batch, int64_t q_heads,
+                                                  int64_t kv_heads, int64_t head_dim,
+                                                  int64_t max_keys, int64_t window,
+                                                  int64_t sinks) {
+  if (!sizes_ok(tokens, batch, q_heads, kv_heads, head_dim, max_keys, kPrefillRows) ||
+      !window_ok(window, sinks))
+    return -1;
+  return prefill_workspace(window_of(window, sinks, max_keys), tokens, batch, q_heads, kv_heads,
+                           head_dim, max_keys);
+}
+
+int w8a8_paged_prefill_window(const void* q, int64_t q_stride_t, int64_t q_stride_h,
+                              const void* k_cache, const void* v_cache, int64_t cache_stride_page,
+                              int64_t cache_stride_head, int64_t cache_stride_token, int64_t pages,
+                              int64_t page_size, const int32_t* page_table, int64_t ld_table,
+                              int64_t table_pages, const int32_t* lengths, const int32_t* q_starts,
+                              int64_t window, int64_t sinks, int clear_rows, int dtype,
+                              float scale, void* out, int64_t out_stride_t, int64_t out_stride_h,
+                              int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                              int64_t head_dim, void* workspace, int64_t workspace_bytes,
+                              hipStream_t stream) {
+  if (!window_ok(window, sinks)) return W8A8_ERR_SHAPE;
+  Sight s;
+  s.windowed = true;
+  s.window = window;
+  s.sinks = sinks;
+  return paged_prefill(s, clear_rows != 0, q, q_stride_t, q_stride_h, k_cache, v_cache,
+                       cache_stride_page, cache_stride_head, cache_stride_token, pages, page_size,
+                       page_table, ld_table, table_pages, lengths, q_starts, dtype, scale, out,
+                       out_stride_t, out_stride_h, tokens, batch, q_heads, kv_heads, head_dim,
+                       workspace, workspace_bytes, stream);
+}
+
+int64_t w8a8_paged_tree_workspace_bytes(int64_t tokens, int64_t batch, int64_t q_heads,
+                                        int64_t kv_heads, int64_t head_dim, int64_t max_keys) {
+  if (!sizes_ok(tokens, batch, q_heads, kv_heads, head_dim, max_keys, kPrefillRows)) return -1;
+  return paged_tree_workspace(tokens, batch, q_heads, kv_heads, head_dim, max_keys);
+}
+
+int w8a8_paged_tree(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_cache,
+                    const void* v_cache, int64_t cache_stride_page, int64_t cache_stride_head,
+                    int64_t cache_stride_token, int64_t pages, int64_t page_size,
+                    const int32_t* page_table, int64_t ld_table, int64_t table_pages,
+                    const int32_t* lengths, const int32_t* q_starts, const uint64_t* masks,
+                    int64_t ld_masks, int64_t mask_words, int clear_rows, int dtype, float scale,
+                    void* out, int64_t out_stride_t, int64_t out_stride_h, int64_t tokens,
+                    int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                    void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+  if (mask_words < 0 || mask_words > kMaxTokens / 64 || ld_masks < mask_words ||
+      ld_masks > kMaxStride)
+    return W8A8_ERR_SHAPE;
+  Sight s;
+  s.tree = true;
+  s.masks = masks;
+  s.ld_masks = ld_masks;
+  s.words = mask_words;
+  return paged_prefill(s, clear_rows != 0, q, q_stride_t, q_stride_h, k_cache, v_cache,
+                       cache_stride_page, cache_stride_head, cache_stride_token, pages, page_size,
+                       page_table, ld_table, table_pages, lengths, q_starts, dtype, scale, out,
+                       out_stride_t, out_stride_h, tokens, batch, q_heads, kv_heads, head_dim,
+                       workspace, workspace_bytes, stream);
+}
+
+int w8a8_cache_accept(void* k_cache, void* v_cache, int64_t cache_stride_layer,
+                      int64_t cache_stride_page, int64_t cache_stride_head,
+                      int64_t cache_stride_token, int64_t layers, int64_t pages,
+                      int64_t page_size, const int32_t* page_table, int64_t ld_table,
+                      int64_t table_pages, const int32_t* lengths, const int32_t* path,
+                      int64_t ld_path, int64_t path_length, int dtype, int64_t batch,
+                      int64_t kv_heads, int64_t head_dim, hipStream_t stream) {
+  if (!half_dtype(dtype)) return W8A8_ERR_DTYPE;
+  const Cache c{cache_stride_page, cache_stride_head, cache_stride_token, pages,
+                page_size,         kv_heads,          head_dim};
+  if (head_dim <= 0 || head_dim % 8 || head_dim > kAttentionMaxDim || kv_heads <= 0 ||
+      kv_heads > kMaxHeads || batch < 0 || batch > kMaxGridYZ || layers < 0 ||
+      layers > kMaxGridYZ / 2)
+    return W8A8_ERR_SHAPE;
+  const int rc = check_cache(c, 8);
+  if (rc != W8A8_OK) return rc;
+  if (table_pages < 0 || ld_table < table_pages || ld_table > kMaxStride ||
+      table_pages > kMaxTokens / page_size || path_length < 0 || path_length > kMaxTokens ||
+      ld_path < path_length || ld_path > kMaxStride || !strides_ok(cache_stride_layer, 0))
+    return W8A8_ERR_SHAPE;
+  if (layers > 1 && cache_stride_layer % 8) return W8A8_ERR_ALIGN;
+  if (batch == 0 || layers == 0 || pages == 0 || table_pages == 0 || path_length == 0)
+    return W8A8_OK;
+  if (k_cache == nullptr || v_cache == nullptr || page_table == nullptr || lengths == nullptr ||
+      path == nullptr)
+    return W8A8_ERR_NULL;
+  if (!aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(page_table, 4) ||
+      !aligned(lengths, 4) || !aligned(path, 4))
+    return W8A8_ERR_ALIGN;
+  const i128 bytes = cache_bytes(c) + 2 * i128(layers - 1) * cache_stride_layer;
+  if (bytes > kMaxBytes || i128(batch) * ld_table > kMaxBytes || i128(batch) * ld_path > kMaxBytes)
+    return W8A8_ERR_SHAPE;
+  if (!cache_distinct(c, cache_stride_layer, layers) ||
+      !caches_apart(k_cache, v_cache, c, cache_stride_layer, layers))
+    return W8A8_ERR_OVERLAP;
+  for (const auto& in : {std::pair<const void*, i128>{page_table, 4 * i128(batch) * ld_table},
+                         {lengths, 4 * i128(batch)},
+                         {path, 4 * i128(batch) * ld_path}}) {
+    const i128 a0 = i128(reinterpret_cast<uintptr_t>(in.first));
+    for (const void* cache : {k_cache, v_cache}) {
+      const i128 b0 = i128(reinterpret_cast<uintptr_t>(cache));
+      if (a0 < b0 + bytes && b0 < a0 + in.second) return W8A8_ERR_OVERLAP;
+    }
+  }
+  CacheAccept p;
+  p.k = k_cache;
+  p.v = v_cache;
+  p.c_layer = cache_stride_layer;
+  p.c_page = cache_stride_page;
+  p.c_head = cache_stride_head;
+  p.c_tok = cache_stride_token;
+  p.pages = pages;
+  p.table = page_table;
+  p.ld_table = ld_table;
+  p.lengths = lengths;
+  p.path = path;
+  p.ld_path = ld_path;
+  p.steps = static_cast<int>(path_length);
+  p.page_shift = page_shift_of(page_size);
+  p.max_keys = static_cast<int>(table_pages * page_size);
+  p.layers = static_cast<int>(layers);
+  p.batch = static_cast<int>(batch);
+  p.kv_heads = static_cast<int>(kv_heads);
+  p.head_dim = static_cast<int>(head_dim);
+  return status_of(launch_cache_accept(p, stream));
 }
 
 }  // extern "C"

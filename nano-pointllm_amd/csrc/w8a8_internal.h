@@ -293,6 +293,68 @@ int64_t paged_prefill_workspace(int64_t tokens, int64_t batch, int64_t q_heads, 
 hipError_t launch_paged_decode(const PagedAttention& p, int dtype, hipStream_t st);
 // clear: rows of no sequence become zeros.
 hipError_t launch_paged_prefill(const PagedAttention& p, bool clear, int dtype, hipStream_t st);
+// The same where a row at place i of its sequence sees only keys j <= i with
+// j < sinks or j > i - window; 1 <= window < max_keys, 0 <= sinks <= max_keys.
+int64_t paged_decode_window_workspace(int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                      int64_t head_dim, int64_t max_keys, int64_t window,
+                                      int64_t sinks);
+int64_t paged_prefill_window_workspace(int64_t tokens, int64_t batch, int64_t q_heads,
+                                       int64_t kv_heads, int64_t head_dim, int64_t max_keys,
+                                       int64_t window, int64_t sinks);
+hipError_t launch_paged_decode_window(const PagedAttention& p, int window, int sinks, int dtype,
+                                      hipStream_t st);
+hipError_t launch_paged_prefill_window(const PagedAttention& p, int window, int sinks, bool clear,
+                                       int dtype, hipStream_t st);
+// Rows q_starts[b] .. are drafted tokens of sequence b, whose keys are the last
+// of its lengths[b]: each row sees all keys before those, and of them those of
+// its mask, bit j % 64 of masks[row * ld_masks + j / 64] (none from 64 words on).
+int64_t paged_tree_workspace(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                             int64_t head_dim, int64_t max_keys);
+hipError_t launch_paged_tree(const PagedAttention& p, const uint64_t* masks, int64_t ld_masks,
+                             int words, bool clear, int dtype, hipStream_t st);
+
+// Keys and values of accepted drafted tokens to the places behind the cached
+// ones (cache_accept.hip), in every layer: those of sequence b's drafted token
+// path[b * ld_path + i] from place lengths[b] + path to place lengths[b] + i.
+// Entries below i (the last ones, -1) move nothing, nor does a place past
+// max_keys or in a page outside [0, pages).
+struct CacheAccept {
+  void* k;
+  void* v;
+  int64_t c_layer, c_page, c_head, c_tok;  // strides in 16-bit elements
+  int64_t pages;
+  const int32_t* table;
+  int64_t ld_table;
+  const int32_t* lengths;
+  const int32_t* path;
+  int64_t ld_path;
+  int steps;
+  int page_shift;
+  int max_keys;
+  int layers, batch, kv_heads, head_dim;
+};
+hipError_t launch_cache_accept(const CacheAccept& p, hipStream_t st);
+
+// Log probabilities of given tokens from logits [rows, vocab] (logprobs.hip),
+// the entropy of each row and its `top` largest logits' tokens, largest first,
+// equal ones by their number.  dtype kF16, kBF16 or kF32.
+constexpr int64_t kLogprobsMaxVocab = int64_t{1} << 20;
+constexpr int kLogprobsMaxTop = 64;
+struct TokenLogprobs {
+  const void* logits;
+  int64_t ld;
+  const int64_t* tokens;   // [rows, given]
+  int64_t ld_tokens;
+  float* logprobs;         // [rows, given]
+  float* entropy;          // [rows], nullable
+  float* top_logprobs;     // [rows, top]
+  int64_t* top_tokens;     // [rows, top]
+  void* workspace;
+  int64_t rows;
+  int vocab, given, top;
+};
+int64_t token_logprobs_workspace(int64_t rows, int64_t vocab, int64_t top, int dtype);
+hipError_t launch_token_logprobs(const TokenLogprobs& p, int dtype, hipStream_t st);
 
 // The w8a8_status of a launch; a failure is kept for w8a8_last_hip_error.
 int status_of(hipError_t e);

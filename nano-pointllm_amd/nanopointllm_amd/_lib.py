@@ -13,7 +13,7 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "libw8a8_gfx950.so"
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 F32, F16, BF16, I32, I8 = 0, 1, 2, 3, 4
 EPI_I32, EPI_DEQUANT, EPI_SILU_MUL, EPI_SILU_MUL_Q8 = 0, 1, 2, 3
@@ -78,6 +78,15 @@ EXPORTED_SYMBOLS = (
     "w8a8_paged_prefill",
     "w8a8_paged_prefill_padded",
     "w8a8_paged_prefill_workspace_bytes",
+    "w8a8_paged_decode_window",
+    "w8a8_paged_decode_window_workspace_bytes",
+    "w8a8_paged_prefill_window",
+    "w8a8_paged_prefill_window_workspace_bytes",
+    "w8a8_paged_tree",
+    "w8a8_paged_tree_workspace_bytes",
+    "w8a8_cache_accept",
+    "w8a8_token_logprobs",
+    "w8a8_token_logprobs_workspace_bytes",
 )
 
 _lock = threading.Lock()
@@ -147,6 +156,26 @@ _SIGNATURES = {
                                          _vp, _i64, _i64, _vp, _vp, _int, _f32, _vp, _i64, _i64,
                                          _i64, _i64, _i64, _i64, _i64, _vp, _i64, _vp]),
     "w8a8_paged_prefill_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64]),
+    "w8a8_paged_decode_window": (_int, [_vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
+                                        _vp, _i64, _i64, _vp, _i64, _i64, _int, _f32, _vp, _i64,
+                                        _i64, _i64, _i64, _i64, _i64, _vp, _i64, _vp]),
+    "w8a8_paged_decode_window_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64,
+                                                        _i64]),
+    "w8a8_paged_prefill_window": (_int, [_vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
+                                         _vp, _i64, _i64, _vp, _vp, _i64, _i64, _int, _int, _f32,
+                                         _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64,
+                                         _vp]),
+    "w8a8_paged_prefill_window_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64,
+                                                         _i64, _i64]),
+    "w8a8_paged_tree": (_int, [_vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp,
+                               _i64, _i64, _vp, _vp, _vp, _i64, _i64, _int, _int, _f32, _vp, _i64,
+                               _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _vp]),
+    "w8a8_paged_tree_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64]),
+    "w8a8_cache_accept": (_int, [_vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64,
+                                 _i64, _vp, _vp, _i64, _i64, _int, _i64, _i64, _i64, _vp]),
+    "w8a8_token_logprobs": (_int, [_vp, _i64, _int, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp,
+                                   _i64, _i64, _vp, _i64, _vp]),
+    "w8a8_token_logprobs_workspace_bytes": (_i64, [_i64, _i64, _i64, _int]),
 }
 
 

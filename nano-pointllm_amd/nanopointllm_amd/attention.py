@@ -11,8 +11,11 @@ The counterpart of the precomputed branch of ``PagedLlamaAttention.forward``
 * :func:`paged_decode` - attention of one new token per sequence, split over
   the cache's length where there are few sequences;
 * :func:`paged_prefill` - causal attention of prompts, or of chunks of them
-  behind a cached part, in a ragged batch;
-* :class:`PagedAttentionCore` - the three as the attention core that
+  behind a cached part, in a ragged batch; both also with a sliding window and
+  sinks, whose keys are the only ones read;
+* :func:`paged_tree` - attention of trees of drafted tokens (:func:`tree_masks`)
+  and :func:`paged_accept`, which keeps their accepted paths in the cache;
+* :class:`PagedAttentionCore` - these as the attention core that
   :class:`nanopointllm_amd.runner.W8A8LlamaRunner` calls, with
   :class:`PagedKVCache` and :class:`AttentionState`.
 
@@ -332,6 +335,37 @@ def _prefill_workspace(tokens: int, batch: int, heads: int, kv_heads: int, dim: 
                                                               dim, max_keys))
 
 
+@lru_cache(maxsize=1024)
+def _decode_window_workspace(batch: int, heads: int, kv_heads: int, dim: int, max_keys: int,
+                             window: int, sinks: int) -> int:
+    return int(_lib.load().w8a8_paged_decode_window_workspace_bytes(
+        batch, heads, kv_heads, dim, max_keys, window, sinks))
+
+
+@lru_cache(maxsize=1024)
+def _prefill_window_workspace(tokens: int, batch: int, heads: int, kv_heads: int, dim: int,
+                              max_keys: int, window: int, sinks: int) -> int:
+    return int(_lib.load().w8a8_paged_prefill_window_workspace_bytes(
+        tokens, batch, heads, kv_heads, dim, max_keys, window, sinks))
+
+
+@lru_cache(maxsize=1024)
+def _tree_workspace(tokens: int, batch: int, heads: int, kv_heads: int, dim: int,
+                    max_keys: int) -> int:
+    return int(_lib.load().w8a8_paged_tree_workspace_bytes(tokens, batch, heads, kv_heads, dim,
+                                                           max_keys))
+
+
+def _window(window: int | None, sinks: int) -> None:
+    if type(sinks) is not int or sinks < 0:
+        raise ValueError("sinks must be a whole number of at least 0")
+    if window is None:
+        if sinks:
+            raise ValueError("sinks need a window")
+    elif type(window) is not int or not 1 <= window < 1 << 62:
+        raise ValueError("window must be a whole number of at least 1, or None")
+
+
 def _queries(q: torch.Tensor) -> tuple[torch.Tensor, tuple[int, ...]]:
     """Query rows whose addresses the kernels' 16-byte loads take: a copy where
     q's are not (not by contiguous(), which returns a contiguous view at an odd
@@ -357,7 +391,8 @@ def _table(page_table: torch.Tensor, batch: int) -> tuple[torch.Tensor, int, int
 
 def paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                  page_table: torch.Tensor, lengths: torch.Tensor, *,
-                 scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+                 scale: float | None = None, window: int | None = None, sinks: int = 0,
+                 out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of one new token per sequence, ``q [batch, heads, head_dim]``,
     over the first ``lengths[b]`` keys of the cache (the new one is already in
     it).  ``page_table`` int32 ``[batch, n]`` names each sequence's pages,
@@ -366,11 +401,19 @@ def paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     multiple of the cache's heads, which consecutive queries share.  ``scale``
     defaults to ``head_dim ** -0.5``.  A NaN or infinite value among a row's
     keys makes the elements that it enters NaN or infinite, one behind its
-    length does nothing."""
+    length does nothing.
+
+    With a ``window`` a sequence's row sees its last ``window`` keys and its
+    first ``sinks`` only; the keys between are not read, and pages that hold no
+    others may be gone (their table entries are not used)."""
     index = _gpu(q, k_cache, v_cache, page_table, lengths, out)
     if index != torch._C._cuda_getDevice():
         with torch.cuda.device(index):
-            return paged_decode(q, k_cache, v_cache, page_table, lengths, scale=scale, out=out)
+            return paged_decode(q, k_cache, v_cache, page_table, lengths, scale=scale,
+                                window=window, sinks=sinks, out=out)
+    if window is not None or sinks:
+        return _decode_window(q, k_cache, v_cache, page_table, lengths, scale, window, sinks, out,
+                              index)
     code = _rows(q, "q")
     q, qs = _queries(q)
     b, h, d = q.shape
@@ -390,28 +433,87 @@ def paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     return out
 
 
+def _decode_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                   page_table: torch.Tensor, lengths: torch.Tensor, scale: float | None,
+                   window: int | None, sinks: int, out: torch.Tensor | None, index: int
+                   ) -> torch.Tensor:
+    _window(window, sinks)
+    code = _rows(q, "q")
+    q, qs = _queries(q)
+    b, h, d = q.shape
+    (pages, g, page_size, _), cs = _cache(k_cache, v_cache, q, d)
+    page_table, ld, width = _table(page_table, b)
+    lengths = _index(lengths, torch.int32, b, "lengths")
+    out = _out_like(out, q)
+    os = out.stride()
+    need = _decode_window_workspace(b, h, g, d, width * page_size, window, sinks)
+    ws = q.new_empty(((need + 1) // 2,)) if need > 0 else None
+    _lib.check(_lib.load().w8a8_paged_decode_window(
+        q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2],
+        pages, page_size, page_table.data_ptr(), ld, width, lengths.data_ptr(), window, sinks,
+        code, d ** -0.5 if scale is None else scale, out.data_ptr(), os[0], os[1], b, h, g, d,
+        None if ws is None else ws.data_ptr(), need, torch._C._cuda_getCurrentRawStream(index)),
+        "w8a8_paged_decode_window")
+    return out
+
+
 def paged_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                   page_table: torch.Tensor, lengths: torch.Tensor, q_starts: torch.Tensor, *,
-                  scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+                  scale: float | None = None, window: int | None = None, sinks: int = 0,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
     """Causal attention of prompts or prompt chunks in a ragged batch: rows
     ``q_starts[b] .. q_starts[b + 1] - 1`` of ``q [tokens, heads, head_dim]``
     (int32 ``[batch + 1]``, not decreasing) are the newest tokens of sequence
     ``b``, whose ``lengths[b]`` keys, theirs among them, are in the cache.  The
     last row sees all of them, each row before it one fewer; a row that sees
     none is zeros.  Rows of no sequence (a padded batch's) are zeros too, but
-    in a given ``out`` they keep what they hold.  Otherwise as
-    :func:`paged_decode`."""
-    return _prefill(q, k_cache, v_cache, page_table, lengths, q_starts, scale, out, out is None)
+    in a given ``out`` they keep what they hold.  With a ``window`` a row sees,
+    of these, its own key and the ``window - 1`` before it, and the sequence's
+    first ``sinks``.  Otherwise as :func:`paged_decode`."""
+    if window is not None or sinks:
+        _window(window, sinks)
+    return _prefill(q, k_cache, v_cache, page_table, lengths, q_starts, scale, out, out is None,
+                    window, sinks)
+
+
+def paged_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+               page_table: torch.Tensor, lengths: torch.Tensor, q_starts: torch.Tensor,
+               masks: torch.Tensor, *, scale: float | None = None,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of trees of drafted tokens: rows ``q_starts[b] .. q_starts[b +
+    1] - 1`` of ``q`` are the ``n`` drafted tokens of sequence ``b``, whose keys
+    are the last ``n`` of its ``lengths[b]`` in the cache.  Each row sees all
+    keys before those, and of the drafted ones key ``j`` where bit ``j % 64`` of
+    ``masks[row, j // 64]`` is set (int64 ``[tokens, words]``, see
+    :func:`tree_masks`; a row sees itself only if its own bit is set, and no key
+    past the words).  A row that sees no key is zeros.  Otherwise as
+    :func:`paged_prefill`."""
+    return _prefill(q, k_cache, v_cache, page_table, lengths, q_starts, scale, out, out is None,
+                    None, 0, masks)
+
+
+def _masks(masks: torch.Tensor, tokens: int) -> tuple[torch.Tensor, int, int]:
+    """(masks, their row stride, words per row)."""
+    shape = masks.shape
+    if masks.dtype != torch.int64 or len(shape) != 2 or shape[0] != tokens:
+        raise ValueError("masks must be int64 [tokens, words]")
+    if masks.stride(0) < shape[1] or masks.stride(1) != 1 and shape[1] > 1:
+        masks = masks.contiguous()
+    return masks, max(masks.stride(0), shape[1]), shape[1]
 
 
 def _prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
              page_table: torch.Tensor, lengths: torch.Tensor, q_starts: torch.Tensor,
-             scale: float | None, out: torch.Tensor | None, clear: bool) -> torch.Tensor:
-    """:func:`paged_prefill`; ``clear``: rows of no sequence become zeros."""
-    index = _gpu(q, k_cache, v_cache, page_table, lengths, q_starts, out)
+             scale: float | None, out: torch.Tensor | None, clear: bool,
+             window: int | None = None, sinks: int = 0, masks: torch.Tensor | None = None
+             ) -> torch.Tensor:
+    """:func:`paged_prefill` and, with masks, :func:`paged_tree`; ``clear``: rows
+    of no sequence become zeros."""
+    index = _gpu(q, k_cache, v_cache, page_table, lengths, q_starts, out, masks)
     if index != torch._C._cuda_getDevice():
         with torch.cuda.device(index):
-            return _prefill(q, k_cache, v_cache, page_table, lengths, q_starts, scale, out, clear)
+            return _prefill(q, k_cache, v_cache, page_table, lengths, q_starts, scale, out, clear,
+                            window, sinks, masks)
     code = _rows(q, "q")
     q, qs = _queries(q)
     t, h, d = q.shape
@@ -420,20 +522,96 @@ def _prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     page_table, ld, width = _table(page_table, b)
     lengths = _index(lengths, torch.int32, b, "lengths")
     q_starts = _index(q_starts, torch.int32, b + 1, "q_starts")
+    if masks is not None:
+        masks, ld_masks, words = _masks(masks, t)
     out = _out_like(out, q)
     os = out.stride()
-    need = _prefill_workspace(t, b, h, g, d, width * page_size)
+    if masks is not None:
+        need = _tree_workspace(t, b, h, g, d, width * page_size)
+    elif window is None:
+        need = _prefill_workspace(t, b, h, g, d, width * page_size)
+    else:
+        need = _prefill_window_workspace(t, b, h, g, d, width * page_size, window, sinks)
     ws = q.new_empty(((need + 1) // 2,)) if need > 0 else None
     if clear and b == 0:
         return out.zero_()
     lib = _lib.load()
-    _lib.check((lib.w8a8_paged_prefill_padded if clear else lib.w8a8_paged_prefill)(
-        q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2],
-        pages, page_size, page_table.data_ptr(), ld, width, lengths.data_ptr(),
-        q_starts.data_ptr(), code, d ** -0.5 if scale is None else scale, out.data_ptr(), os[0],
-        os[1], t, b, h, g, d, None if ws is None else ws.data_ptr(), need,
-        torch._C._cuda_getCurrentRawStream(index)), "w8a8_paged_prefill")
+    given = (q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1],
+             cs[2], pages, page_size, page_table.data_ptr(), ld, width, lengths.data_ptr(),
+             q_starts.data_ptr())
+    rest = (code, d ** -0.5 if scale is None else scale, out.data_ptr(), os[0], os[1], t, b, h, g,
+            d, None if ws is None else ws.data_ptr(), need,
+            torch._C._cuda_getCurrentRawStream(index))
+    if masks is not None:
+        status = lib.w8a8_paged_tree(*given, masks.data_ptr(), ld_masks, words, clear, *rest)
+    elif window is not None:
+        status = lib.w8a8_paged_prefill_window(*given, window, sinks, clear, *rest)
+    else:
+        status = (lib.w8a8_paged_prefill_padded if clear else lib.w8a8_paged_prefill)(
+            *given, *rest)
+    if status != _lib.OK:
+        _lib.check(status, "w8a8_paged_prefill" if masks is None else "w8a8_paged_tree")
     return out
+
+
+# ------------------------------------------------------------ drafted tokens
+def tree_masks(parents: Sequence[Sequence[int]], *, device: torch.device | str = "cuda"
+               ) -> torch.Tensor:
+    """The masks of :func:`paged_tree` for a batch of trees: ``parents[b][i]`` is
+    the parent of sequence ``b``'s drafted token ``i``, one of those before it
+    (a chain: ``i - 1``), or -1 for one that follows the cached tokens; each
+    token sees its ancestors and itself.  int64 ``[tokens, words]`` with as many
+    words as the longest tree needs."""
+    rows: list[int] = []
+    for tree in parents:
+        own: list[int] = []
+        for i, parent in enumerate(tree):
+            if not -1 <= parent < i:
+                raise ValueError("a drafted token's parent must be one before it, or -1")
+            own.append(1 << i | (own[parent] if parent >= 0 else 0))
+        rows += own
+    words = max(1, -(-max(map(len, parents), default=0) // 64))
+    low = (1 << 64) - 1
+    signed = [[((m >> 64 * w & low) ^ 1 << 63) - (1 << 63) for w in range(words)] for m in rows]
+    return torch.tensor(signed, dtype=torch.int64).reshape(len(rows), words).to(device)
+
+
+def paged_accept(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                 lengths: torch.Tensor, path: torch.Tensor) -> None:
+    """Keeps accepted drafted tokens in the cache, in place: the key and value of
+    sequence ``b``'s drafted token ``path[b, i]`` (int32 ``[batch, steps]``,
+    rising; -1 behind the path's end) go to place ``lengths[b] + i``, where
+    ``lengths[b]`` (int32) keys were cached before the drafted ones.  The caches
+    are one layer's, or ``[layers, pages, kv_heads, page_size, head_dim]``: all
+    layers in one launch (:meth:`PagedKVCache.accept`).  An entry below its
+    ``i`` moves nothing, as does a place outside the table or the cache.  The
+    pages of the drafted tokens belong to one sequence only."""
+    index = _gpu(k_cache, v_cache, page_table, lengths, path)
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            return paged_accept(k_cache, v_cache, page_table, lengths, path)
+    code = _CODES.get(k_cache.dtype)
+    if code is None or v_cache.dtype != k_cache.dtype:
+        raise ValueError("the cache must be float16 / bfloat16")
+    shape, strides, other = k_cache.shape, k_cache.stride(), v_cache.stride()
+    if len(shape) not in (4, 5) or shape != v_cache.shape:
+        raise ValueError("k_cache and v_cache must be [pages, kv_heads, page_size, head_dim] "
+                         "or [layers, ...] of these")
+    if strides[-1] != 1 or any(n > 1 and x != y for n, x, y in zip(shape, strides, other)):
+        raise ValueError("k_cache and v_cache must have equal strides and contiguous heads")
+    layers, ls = (shape[0], strides[0]) if len(shape) == 5 else (1, 0)
+    pages, g, page_size, d = shape[-4:]
+    b = lengths.shape[0] if lengths.dim() == 1 else -1
+    page_table, ld, width = _table(page_table, b)
+    lengths = _index(lengths, torch.int32, b, "lengths")
+    if path.dtype != torch.int32 or path.dim() != 2 or path.shape[0] != b:
+        raise ValueError("path must be int32 [batch, steps]")
+    path = path if path.is_contiguous() else path.contiguous()
+    steps = path.shape[1]
+    _lib.check(_lib.load().w8a8_cache_accept(
+        k_cache.data_ptr(), v_cache.data_ptr(), ls, *strides[-4:-1], layers, pages, page_size,
+        page_table.data_ptr(), ld, width, lengths.data_ptr(), path.data_ptr(), steps, steps, code,
+        b, g, d, torch._C._cuda_getCurrentRawStream(index)), "w8a8_cache_accept")
 
 
 # --------------------------------------------------------- the runner's core
@@ -457,6 +635,11 @@ class PagedKVCache:
                             device=device)
         self.k = [store[i, 0] for i in range(layers)]
         self.v = [store[i, 1] for i in range(layers)]
+        self._store = store
+
+    def accept(self, page_table: torch.Tensor, lengths: torch.Tensor, path: torch.Tensor) -> None:
+        """:func:`paged_accept` in every layer, one launch."""
+        paged_accept(self._store[:, 0], self._store[:, 1], page_table, lengths, path)
 
 
 @dataclass
@@ -467,7 +650,8 @@ class AttentionState:
     sequence its pages and its length with this step's tokens.  The first
     ``decode_rows`` rows are one new token each of the first ``decode_rows``
     sequences; the others are chunks, ``q_starts`` giving where each of the
-    remaining sequences' rows start, counted from the first of them."""
+    remaining sequences' rows start, counted from the first of them.  With
+    ``masks`` those chunks are trees of drafted tokens (:meth:`build_drafts`)."""
 
     positions: torch.Tensor            # int64 [rows]
     slots: torch.Tensor                # int64 [rows]
@@ -475,6 +659,36 @@ class AttentionState:
     lengths: torch.Tensor              # int32 [sequences]
     q_starts: torch.Tensor | None = None   # int32 [sequences - decode_rows + 1]
     decode_rows: int = 0
+    masks: torch.Tensor | None = None      # int64 [rows - decode_rows, words]
+
+    @classmethod
+    def build_drafts(cls, pages: Sequence[Sequence[int]], lengths: Sequence[int],
+                     parents: Sequence[Sequence[int]], page_size: int, *,
+                     device: torch.device | str = "cuda") -> "AttentionState":
+        """The state of a step that verifies a tree of drafted tokens per
+        sequence: sequence ``b``, which owns ``pages[b]`` in order and has
+        ``lengths[b]`` cached tokens, gets the drafted tokens whose parents are
+        ``parents[b]`` (:func:`tree_masks`).  Token ``i`` is stored at place
+        ``lengths[b] + i`` and turned to the position of its depth in the tree;
+        :meth:`PagedKVCache.accept` moves the accepted ones to their places."""
+        if not len(pages) == len(lengths) == len(parents):
+            raise ValueError("pages, lengths and parents must have one entry per sequence")
+        state = cls.build(pages, [n + len(tree) for n, tree in zip(lengths, parents)],
+                          [len(tree) for tree in parents], page_size, device=device)
+        masks = tree_masks(parents, device=device)
+        positions: list[int] = []
+        for n, tree in zip(lengths, parents):
+            own: list[int] = []
+            for parent in tree:
+                own.append(own[parent] + 1 if parent >= 0 else n)
+            positions += own
+        starts = [0]
+        for tree in parents:
+            starts.append(starts[-1] + len(tree))
+        state.positions = torch.tensor(positions, dtype=torch.int64, device=device)
+        state.q_starts = torch.tensor(starts, dtype=torch.int32, device=device)
+        state.decode_rows, state.masks = 0, masks
+        return state
 
     @classmethod
     def build(cls, pages: Sequence[Sequence[int]], lengths: Sequence[int],
@@ -520,30 +734,49 @@ class PagedAttentionCore:
     ``runner = W8A8LlamaRunner(model, PagedAttentionCore(cache, frequencies))``
     and ``runner(ids, attention_state=AttentionState.build(...))``; a decode
     step is captured with :class:`~nanopointllm_amd.runner.DecodeGraphBucket`
-    on a state whose tensors are then refilled in place between replays."""
+    on a state whose tensors are then refilled in place between replays.
+    ``window`` (one for all layers, or one or None for each) and ``sinks``
+    limit what a row sees as in :func:`paged_decode`; sequences keep their own
+    positions, sinks included."""
 
     def __init__(self, cache: PagedKVCache, frequencies: RotaryFrequencies, *,
-                 layout: str = "half", scale: float | None = None) -> None:
+                 layout: str = "half", scale: float | None = None,
+                 window: int | None | Sequence[int | None] = None, sinks: int = 0) -> None:
         _layout(layout)
         self.cache, self.frequencies = cache, frequencies
         self.layout, self.scale = layout, scale
+        if not isinstance(window, Sequence):
+            _window(window, sinks)
+        else:
+            window = list(window)
+            if len(window) != len(cache.k):
+                raise ValueError("window must be one for all layers, or one for each")
+            for w in window:
+                _window(w, sinks if w is not None else 0)
+            _window(max((w for w in window if w is not None), default=None), sinks)
+        self.window, self.sinks = window, sinks
 
     def __call__(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, layer_index: int,
                  state: AttentionState) -> torch.Tensor:
         k_cache, v_cache = self.cache.k[layer_index], self.cache.v[layer_index]
+        window = self.window[layer_index] if isinstance(self.window, list) else self.window
+        sinks = 0 if window is None else self.sinks
+        table, lengths, n = state.page_table, state.lengths, state.decode_rows
+        if state.masks is not None and window is not None:
+            raise ValueError("trees of drafted tokens run on layers without a window")
         q = rotary_store(q, k, v, state.positions, state.slots, self.frequencies.inv_freq,
                          k_cache, v_cache, layout=self.layout,
                          attention_factor=self.frequencies.attention_factor)
-        table, lengths, n = state.page_table, state.lengths, state.decode_rows
         if state.q_starts is None:
-            out = paged_decode(q, k_cache, v_cache, table, lengths, scale=self.scale)
+            out = paged_decode(q, k_cache, v_cache, table, lengths, scale=self.scale,
+                               window=window, sinks=sinks)
         elif n == 0:
-            out = paged_prefill(q, k_cache, v_cache, table, lengths, state.q_starts,
-                                scale=self.scale)
+            out = _prefill(q, k_cache, v_cache, table, lengths, state.q_starts, self.scale, None,
+                           True, window, sinks, state.masks)
         else:
             out = torch.empty_like(q)
             paged_decode(q[:n], k_cache, v_cache, table[:n], lengths[:n], scale=self.scale,
-                         out=out[:n])
+                         window=window, sinks=sinks, out=out[:n])
             _prefill(q[n:], k_cache, v_cache, table[n:], lengths[n:], state.q_starts,
-                     self.scale, out[n:], True)
+                     self.scale, out[n:], True, window, sinks, state.masks)
         return out.flatten(1)

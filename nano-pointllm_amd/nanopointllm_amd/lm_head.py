@@ -10,8 +10,14 @@ summation order, so a row's logits do not depend on the other rows of the
 batch).  ``DecodeLMHead`` wraps the module: decode batches take the kernel,
 larger batches keep the module's own GEMM (``F.linear``), as the reference
 does for prefill.
+
+``token_logprobs`` reads the logits once for the log probabilities of given
+tokens, the entropy of each row and its most probable tokens: what scores a
+prompt, or accepts drafted tokens.
 """
 from __future__ import annotations
+
+from typing import NamedTuple
 
 import torch
 import torch.nn.functional as F
@@ -98,3 +104,64 @@ class DecodeLMHead(nn.Module):
         if dense_gemv_supported(hidden, self.linear.weight, bias):
             return dense_gemv(hidden, self.linear.weight, bias)
         return F.linear(hidden, self.linear.weight, bias)
+
+
+MAX_TOP = 64
+MAX_VOCAB = 1 << 20
+_LOGIT_CODES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
+
+
+class TokenLogprobs(NamedTuple):
+    logprobs: torch.Tensor                  # float32, the tokens' shape
+    entropy: torch.Tensor                   # float32 [...], in nats
+    top_logprobs: torch.Tensor | None       # float32 [..., top], falling
+    top_tokens: torch.Tensor | None         # int64 [..., top]
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) -> TokenLogprobs:
+    """Log probabilities (natural, ``log_softmax``) of given ``tokens`` under
+    ``logits [..., vocab]`` (float16, bfloat16 or float32), with the entropy of
+    each row and its ``top`` (at most 64) most probable tokens.
+
+    ``tokens`` (int64) has the rows' shape ``[...]``, or ``[..., n]`` for n
+    tokens of each row; -1 (a padded place) gives 0, another number outside the
+    vocabulary NaN.  Among equal logits the lowest token comes first.  Sums and
+    results are binary32; a logit of -inf has probability 0, a row with +inf,
+    NaN or nothing above -inf gives NaN."""
+    device = _lib.require_cuda(logits, tokens)
+    code = _LOGIT_CODES.get(logits.dtype)
+    if code is None or logits.dim() < 1:
+        raise ValueError("logits must be float16, bfloat16 or float32 [..., vocab]")
+    shape, vocab = logits.shape[:-1], logits.shape[-1]
+    if not 1 <= vocab <= MAX_VOCAB:
+        raise ValueError(f"the vocabulary must have 1 to {MAX_VOCAB} tokens")
+    if tokens.dtype != torch.int64 or tokens.shape[:len(shape)] != shape \
+            or tokens.dim() > len(shape) + 1:
+        raise ValueError("tokens must be int64 of the rows' shape, or with one more axis")
+    if type(top) is not int or not 0 <= top <= min(MAX_TOP, vocab):
+        raise ValueError(f"top must be 0 to {MAX_TOP} and at most the vocabulary")
+    if device.index != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
+            return token_logprobs(logits, tokens, top=top)
+    x = logits.reshape(-1, vocab)
+    rows = x.shape[0]
+    if x.stride(1) != 1 and vocab > 1 or x.stride(0) < vocab and rows > 1:
+        x = x.contiguous()
+    per = tokens.shape[-1] if tokens.dim() > len(shape) else 1
+    tokens = tokens.contiguous()
+    logprobs = torch.empty(tokens.shape, device=device, dtype=torch.float32)
+    entropy = torch.empty(shape, device=device, dtype=torch.float32)
+    best = ids = None
+    if top:
+        best = torch.empty((*shape, top), device=device, dtype=torch.float32)
+        ids = torch.empty((*shape, top), device=device, dtype=torch.int64)
+    if rows == 0:
+        return TokenLogprobs(logprobs, entropy, best, ids)
+    lib = _lib.load()
+    need = lib.w8a8_token_logprobs_workspace_bytes(rows, vocab, top, code)
+    ws = torch.empty(need, device=device, dtype=torch.uint8) if need > 0 else None
+    _lib.check(lib.w8a8_token_logprobs(
+        x.data_ptr(), x.stride(0), code, tokens.data_ptr(), per, per, top, logprobs.data_ptr(),
+        entropy.data_ptr(), _lib.ptr(best), _lib.ptr(ids), rows, vocab, _lib.ptr(ws), need,
+        _lib.stream_handle(device)), "w8a8_token_logprobs")
+    return TokenLogprobs(logprobs, entropy, best, ids)

@@ -55,7 +55,7 @@ import torch.nn as nn
 
 from . import w8a8 as _w
 from .inject import inject_w8a8
-from .lm_head import DecodeLMHead
+from .lm_head import DecodeLMHead, TokenLogprobs, token_logprobs
 from .linear import W8A8Linear, W8A8MLP, W8A8PackedQKV, _norm_eps
 
 #: Most rows the GEMV kernels take (kGemvMaxRows).
@@ -244,6 +244,17 @@ class W8A8LlamaRunner(nn.Module):
         for layer in self.layers:
             hidden, residual = layer.forward_carry(hidden, residual, attention_state)
         return self.lm_head(self.final_norm(hidden, residual).view(shape))
+
+    @torch.no_grad()
+    def score(self, input_ids: torch.Tensor | None = None, *, tokens: torch.Tensor, top: int = 0,
+              inputs_embeds: torch.Tensor | None = None,
+              attention_state: Any = None) -> TokenLogprobs:
+        """One forward and, of its logits, the log probabilities of ``tokens``
+        (:func:`~nanopointllm_amd.lm_head.token_logprobs`; the logits' rows'
+        shape, or one more axis): a prompt's next tokens, or the drafted tokens
+        that may follow each node of a tree."""
+        logits = self(input_ids, inputs_embeds=inputs_embeds, attention_state=attention_state)
+        return token_logprobs(logits, tokens, top=top)
 
     def stream_route(self, rows: torch.Tensor) -> bool:
         """Whether a forward over ``rows`` takes :meth:`W8A8LlamaLayer.forward_stream`:
