@@ -25,13 +25,14 @@ bool aligned(const void* p, uintptr_t a) {
 }
 
 // A launch's threads are counted in 32 bits, a workgroup has up to 1024.
-constexpr int64_t kMaxRows = (int64_t{1} << 22) - 1;
+constexpr int64_t kMaxRows = (int64_t{1} << 22) - 1;   // and of workgroups
 constexpr int64_t kMaxGiven = int64_t{1} << 20;
 constexpr int64_t kMaxLd = int64_t{1} << 38;
 
-bool sizes_ok(int64_t rows, int64_t vocab, int64_t top) {
+bool sizes_ok(int64_t rows, int64_t vocab, int64_t top, int dtype) {
   return rows >= 0 && rows <= kMaxRows && vocab >= 1 && vocab <= kLogprobsMaxVocab && top >= 0 &&
-         top <= kLogprobsMaxTop && top <= vocab;
+         top <= kLogprobsMaxTop && top <= vocab &&
+         token_logprobs_workgroups(rows, vocab, dtype) <= kMaxRows;
 }
 
 }  // namespace
@@ -39,7 +40,8 @@ bool sizes_ok(int64_t rows, int64_t vocab, int64_t top) {
 extern "C" {
 
 int64_t w8a8_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int64_t top, int dtype) {
-  if (!sizes_ok(rows, vocab, top) || (dtype != kF32 && dtype != kF16 && dtype != kBF16)) return -1;
+  if ((dtype != kF32 && dtype != kF16 && dtype != kBF16) || !sizes_ok(rows, vocab, top, dtype))
+    return -1;
   return token_logprobs_workspace(rows, vocab, top, dtype);
 }
 
@@ -49,7 +51,7 @@ int w8a8_token_logprobs(const void* logits, int64_t ld_logits, int dtype, const 
                         int64_t vocab, void* workspace, int64_t workspace_bytes,
                         hipStream_t stream) {
   if (dtype != kF32 && dtype != kF16 && dtype != kBF16) return W8A8_ERR_DTYPE;
-  if (!sizes_ok(rows, vocab, top) || given < 0 || given > kMaxGiven) return W8A8_ERR_SHAPE;
+  if (!sizes_ok(rows, vocab, top, dtype) || given < 0 || given > kMaxGiven) return W8A8_ERR_SHAPE;
   if (ld_logits < 0 || ld_logits > kMaxLd || ld_tokens < 0 || ld_tokens > kMaxLd)
     return W8A8_ERR_SHAPE;
   if (rows == 0) return W8A8_OK;

@@ -5,114 +5,467 @@
 // log1p(R): a given token's log probability is (x - m) - log1p(R), the entropy
 // log1p(R) + sum (m - x) exp(x - m) / (1 + R), all terms of one sign, so that a
 // row that is nearly decided keeps its digits.
-#include "w8a8_internal.h"
+//
+// Design:
+//   * A workgroup holds a row, or a slice of a long one, in registers: the logits
+//     are read once.  The sums run while later loads are in flight, against a
+//     reference per thread that is the maximum so far or up to kSlack below.
+//   * The thread whose logit is the row's maximum leaves its sums: its wavefront
+//     adds its logits up again through LDS, with the maximum left out and counted.
+//   * Top tokens: the k-th largest of 256 groups' maxima bounds the k-th largest
+//     logit from below, and few logits reach it (k and some, rarely 2 k).  They go
+//     through LDS, in any order, and each counts those before it: its place.  Ties
+//     are broken by the token's number, so the order of arrival changes nothing.
+//     Where more than kMost reach the bound (a row of equal logits) the top tokens
+//     are found one by one.
+//   * Rows of more vectors than a workgroup holds are cut into equal slices, whose
+//     sums and top tokens a second launch joins.
+#include <algorithm>
+
+#include "attention_common.h"
 
 namespace w8a8 {
 
 namespace {
 
-constexpr int kThreads = 1024;
-constexpr int kWaves = kThreads / 64;
+constexpr int kMost = 1024;        // candidates that a workgroup ranks
+constexpr int kGroups = 256;       // maxima that the bound is taken from
+constexpr float kSlack = 8.0f;     // in powers of two
+constexpr float kLn2 = 0.693147180559945309417f;
+constexpr int kJoinThreads = 256;
 
-template <typename T> __device__ inline float logit(const void* x, int64_t i) {
+// What a slice leaves for the join.
+struct Part {
+  float top;     // its largest logit
+  float equal;   // how many are equal to it
+  float sum;     // sum of exp(x - top) over the others, 0 if top is -inf
+  float spread;  // sum of (top - x) exp(x - top)
+};
+
+template <typename T> constexpr int per_vector() { return 16 / sizeof(T); }
+
+// Element j of a vector.
+template <typename T> __device__ inline float element(const u32x4& v, int j) {
+  if constexpr (std::is_same<T, float>::value) {
+    return __uint_as_float(v[j]);
+  } else {
+    const uint32_t w = v[j >> 1];
+    return bits_to_f32<T>((j & 1) ? w >> 16 : w & 0xffffu);
+  }
+}
+template <typename T> __device__ inline uint32_t minus_infinity() {
   if constexpr (std::is_same<T, float>::value)
-    return static_cast<const float*>(x)[i];
+    return 0xff800000u;
+  else if constexpr (std::is_same<T, __half>::value)
+    return 0xfc00fc00u;
   else
-    return to_f32(static_cast<const T*>(x)[i]);
+    return 0xff80ff80u;
 }
 
-// The order of logits: by value, NaN above all, equal ones by their number.
-__device__ inline uint64_t rank_of(float x, int i) {
-  const uint32_t u = __float_as_uint(x + 0.0f);   // one zero
-  const uint32_t order = x != x ? ~0u : (u >> 31) ? ~u : u | 0x80000000u;
-  return static_cast<uint64_t>(order) << 32 | static_cast<uint32_t>(~i);
+// The order of logits as whole numbers: by value, one zero, NaN above all.
+__device__ inline uint32_t order_of(float x) {
+  const uint32_t u = __float_as_uint(x + 0.0f);
+  return x != x ? ~0u : (u >> 31) ? ~u : u | 0x80000000u;
+}
+__device__ inline float value_of(uint32_t order) {
+  return __uint_as_float((order >> 31) ? order & 0x7fffffffu : ~order);
+}
+// ... and of equal ones by the token's number.
+__device__ inline uint64_t rank_of(float x, int token) {
+  return static_cast<uint64_t>(order_of(x)) << 32 | ~static_cast<uint32_t>(token);
+}
+__device__ inline int token_of(uint64_t rank) {
+  return static_cast<int>(~static_cast<uint32_t>(rank));
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void logprobs_kernel(TokenLogprobs p) {
-  __shared__ float red[3][kWaves];
-  __shared__ uint64_t best[kWaves];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t row = blockIdx.x;
-  const T* x = static_cast<const T*>(p.logits) + row * p.ld;
-  float top = -INFINITY;
-  for (int i = threadIdx.x; i < p.vocab; i += kThreads) top = fmaxf(top, logit<T>(x, i));
-  for (int w = 1; w < 64; w <<= 1) top = fmaxf(top, __shfl_xor(top, w));
-  if (lane == 0) red[0][wave] = top;
-  __syncthreads();
-  for (int w = 0; w < kWaves; ++w) top = fmaxf(top, red[0][w]);
-  __syncthreads();
-  float sum = 0.0f, spread = 0.0f, equal = 0.0f;
-  for (int i = threadIdx.x; i < p.vocab; i += kThreads) {
-    const float d = logit<T>(x, i) - top;
-    const float e = expf(d);
-    if (d == 0.0f) {
-      equal += 1.0f;
-    } else {
-      sum += e;
-      spread -= e == 0.0f ? 0.0f : d * e;
-    }
-  }
+__device__ inline float wave_sum(float x) {
+#pragma unroll
+  for (int w = 1; w < 64; w <<= 1) x += __shfl_xor(x, w);
+  return x;
+}
+__device__ inline float wave_max(float x) {
+#pragma unroll
+  for (int w = 1; w < 64; w <<= 1) x = fmaxf(x, __shfl_xor(x, w));
+  return x;
+}
+__device__ inline uint64_t wave_max64(uint64_t x) {
+#pragma unroll
   for (int w = 1; w < 64; w <<= 1) {
-    sum += __shfl_xor(sum, w);
-    spread += __shfl_xor(spread, w);
-    equal += __shfl_xor(equal, w);
+    const uint64_t y = __shfl_xor(static_cast<unsigned long long>(x), w);
+    x = y > x ? y : x;
   }
-  if (lane == 0) {
-    red[0][wave] = sum;
-    red[1][wave] = spread;
-    red[2][wave] = equal;
+  return x;
+}
+
+// The k-th largest of 4 x 64 orders, to its upper 16 bits, rounded down.
+__device__ inline uint32_t kth_order(const uint32_t (&g)[4], int k) {
+  uint32_t t = 0;
+#pragma unroll 1
+  for (int bit = 31; bit >= 16; --bit) {
+    const uint32_t next = t | 1u << bit;
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) n += __popcll(__ballot(g[i] >= next));
+    if (n >= k) t = next;
   }
-  __syncthreads();
-  sum = spread = equal = 0.0f;
-  for (int w = 0; w < kWaves; ++w) {
-    sum += red[0][w];
-    spread += red[1][w];
-    equal += red[2][w];
-  }
+  return t;
+}
+
+// The results of a row whose logits are known but for the given tokens'.
+struct Row {
+  float top, norm, entropy;   // norm: log sum exp(x - top)
+  __device__ float logprob(float x) const { return (x - top) - norm; }
+};
+__device__ inline Row finish(float top, float equal, float sum, float spread) {
   const float rest = sum + (equal - 1.0f);
-  const float norm = equal == 0.0f ? NAN : log1pf(rest);
-  if (threadIdx.x == 0 && p.entropy != nullptr) p.entropy[row] = norm + spread / (1.0f + rest);
-  for (int i = threadIdx.x; i < p.given; i += kThreads) {
+  const float norm = top == -INFINITY ? NAN : log1pf(rest);
+  return Row{top, norm, norm + spread / (1.0f + rest)};
+}
+template <typename T>
+__device__ inline void write_given(const TokenLogprobs& p, int64_t row, const Row& r, int i,
+                                   int n) {
+  const T* x = static_cast<const T*>(p.logits) + row * p.ld;
+  for (; i < p.given; i += n) {
     const int64_t token = p.tokens[row * p.ld_tokens + i];
     float y = token == -1 ? 0.0f : NAN;
-    if (token >= 0 && token < p.vocab) y = (logit<T>(x, token) - top) - norm;
+    if (token >= 0 && token < p.vocab) y = r.logprob(to_f32(x[token]));
     p.logprobs[row * p.given + i] = y;
   }
-  uint64_t last = ~uint64_t{0};
-  for (int k = 0; k < p.top; ++k) {
-    uint64_t mine = 0;
-    for (int i = threadIdx.x; i < p.vocab; i += kThreads) {
-      const uint64_t r = rank_of(logit<T>(x, i), i);
-      if (r < last && r > mine) mine = r;
-    }
-    for (int w = 1; w < 64; w <<= 1) mine = max(mine, static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(mine), w)));
-    __syncthreads();
-    if (lane == 0) best[wave] = mine;
-    __syncthreads();
-    for (int w = 0; w < kWaves; ++w) mine = max(mine, best[w]);
-    last = mine;
-    if (threadIdx.x == 0) {
-      const int token = static_cast<int>(~static_cast<uint32_t>(mine));
-      p.top_tokens[row * p.top + k] = token;
-      p.top_logprobs[row * p.top + k] = (logit<T>(x, token) - top) - norm;
+}
+__device__ inline void write_top(const TokenLogprobs& p, int64_t row, const Row& r, int place,
+                                 uint64_t rank) {
+  p.top_tokens[row * p.top + place] = token_of(rank);
+  const uint32_t order = static_cast<uint32_t>(rank >> 32);
+  p.top_logprobs[row * p.top + place] = r.logprob(order == ~0u ? NAN : value_of(order));
+}
+
+// W wavefronts, NV vectors of 16 bytes a thread.  slices: workgroups of a row, of
+// `step` vectors each; parts and ranks are theirs if there are several.
+template <typename T, int W, int NV>
+__global__ __launch_bounds__(64 * W, NV > 8 ? 4 : NV > 4 ? 6 : 8) void logprobs_kernel(
+    TokenLogprobs p, int slices, int step, Part* parts, uint64_t* ranks) {
+  constexpr int E = per_vector<T>();
+  constexpr int N = 64 * W;
+  __shared__ u32x4 stage[W][NV];
+  __shared__ float tops[W];
+  __shared__ float sums[3][W];
+  __shared__ uint32_t group[kGroups];
+  __shared__ uint64_t found[kMost];
+  __shared__ uint64_t best[W];
+  __shared__ uint32_t bound;
+  __shared__ int count;
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t row = blockIdx.x / slices;
+  const int slice = blockIdx.x % slices;
+  const T* x = static_cast<const T*>(p.logits) + row * p.ld;
+  // Vectors are aligned: the first may begin before the row and the last end
+  // behind it; those two are read element by element.
+  const int skew = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+  const int v0 = slice * step;
+  const int v1 = min(v0 + step, (p.vocab + skew + E - 1) / E);
+  const int first_token = max(v0 * E - skew, 0);
+  const u32x4* vectors = reinterpret_cast<const u32x4*>(x - skew);
+
+  u32x4 raw[NV];
+#pragma unroll
+  for (int n = 0; n < NV; ++n) {
+    const int v = v0 + n * N + tid;
+    const uint32_t none = minus_infinity<T>();
+    raw[n] = u32x4{none, none, none, none};
+    if (v < v1 && v * E >= skew && (v + 1) * E <= p.vocab + skew) raw[n] = vectors[v];
+  }
+#pragma unroll
+  for (int n = 0; n < NV; ++n) {
+    const int v = v0 + n * N + tid;
+    if (v < v1 && (v * E < skew || (v + 1) * E > p.vocab + skew)) {
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const int token = v * E - skew + j;
+        if (token < 0 || token >= p.vocab) continue;
+        if constexpr (std::is_same<T, float>::value) {
+          raw[n][j] = __float_as_uint(x[token]);
+        } else {
+          const uint32_t b = reinterpret_cast<const uint16_t*>(x)[token];
+          const uint32_t w = raw[n][j >> 1];
+          raw[n][j >> 1] = (j & 1) ? (w & 0xffffu) | b << 16 : (w & 0xffff0000u) | b;
+        }
+      }
     }
   }
+  if (tid == 0) count = 0;
+
+  // sum = sum of 2^t, spread = sum of t 2^t with t = (x - ref) log2(e).
+  float top = -INFINITY, ref = 0.0f, sum = 0.0f, spread = 0.0f;
+#pragma unroll
+  for (int n = 0; n < NV; ++n) {
+    if (v0 + n * N + tid >= v1) continue;
+    float most = element<T>(raw[n], 0);
+#pragma unroll
+    for (int j = 1; j < E; ++j) most = fmaxf(most, element<T>(raw[n], j));
+    if ((most - ref) * kLog2e > kSlack || (top == -INFINITY && most > -INFINITY)) {
+      const float next = fminf(most, 3.40282347e38f);   // of infinities the sums are NaN
+      const float t = (ref - next) * kLog2e, f = exp2_hw(t);
+      const bool none = sum == 0.0f || f == 0.0f;
+      spread = none ? 0.0f : (spread + t * sum) * f;
+      sum = sum == 0.0f ? 0.0f : sum * f;
+      ref = next;
+    }
+    top = fmaxf(top, most);
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      const float t = (element<T>(raw[n], j) - ref) * kLog2e;
+      const float e = exp2_hw(t);
+      sum += e;
+      // A logit of -inf adds 0, one of NaN is in e.
+      spread = __builtin_fmaf(fmaxf(t, -200.0f), e, spread);
+    }
+  }
+
+  // The largest of the workgroup and of each group of threads.
+  {
+    float most = top;
+#pragma unroll
+    for (int w = 1; w < N / kGroups; w <<= 1) most = fmaxf(most, __shfl_xor(most, w));
+    if (p.top > 1 && tid % (N / kGroups) == 0) group[tid / (N / kGroups)] = order_of(most);
+    most = wave_max(most);
+    if (lane == 0) tops[wave] = most;
+  }
+  __syncthreads();
+  float peak = tops[0];
+#pragma unroll
+  for (int w = 1; w < W; ++w) peak = fmaxf(peak, tops[w]);
+  if (p.top > 1 && wave == 0) {
+    uint32_t g[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) g[i] = group[lane + 64 * i];
+    const uint32_t t = kth_order(g, p.top);
+    if (lane == 0) bound = t;
+  }
+
+  // One thread's logits, spread over its wavefront: f(logit, token) of each.
+  auto spread_out = [&](int from, auto f) __attribute__((always_inline)) {
+    __builtin_amdgcn_wave_barrier();
+    if (lane == from) {
+#pragma unroll
+      for (int n = 0; n < NV; ++n) stage[wave][n] = raw[n];
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    const T* values = reinterpret_cast<const T*>(stage[wave]);
+#pragma unroll
+    for (int i = 0; i < NV * E; i += 64) {
+      const int at = i + lane;
+      const int v = v0 + at / E * N + wave * 64 + from;
+      const int token = v * E - skew + at % E;
+      if (at < NV * E && v < v1 && token >= 0 && token < p.vocab) f(to_f32(values[at]), token);
+    }
+    __builtin_amdgcn_wave_barrier();
+  };
+
+  const float m = peak == -INFINITY ? 0.0f : peak;
+  float equal = 0.0f;
+  {
+    // From the thread's reference to the row's: t grows by (ref - m) log2(e).
+    const float t = (ref - m) * kLog2e, f = exp2_hw(t);
+    const bool nan = sum != sum;
+    spread = sum == 0.0f || f == 0.0f ? 0.0f : -(spread + t * sum) * f * kLn2;
+    sum *= f;
+    uint64_t holders = __ballot(top == peak && top > -INFINITY && !nan);
+    if (top == peak && top > -INFINITY && !nan) sum = spread = 0.0f;
+    while (holders != 0) {
+      const int from = __ffsll(static_cast<unsigned long long>(holders)) - 1;
+      holders &= holders - 1;
+      spread_out(from, [&](float y, int) {
+        const float d = y - m, e = exp2_hw(d * kLog2e);
+        if (d == 0.0f) {
+          equal += 1.0f;
+        } else {
+          sum += e;
+          spread -= fmaxf(d, -200.0f) * e;
+        }
+      });
+    }
+    const float s = wave_sum(sum), d = wave_sum(spread), n = wave_sum(equal);
+    if (lane == 0) {
+      sums[0][wave] = s;
+      sums[1][wave] = d;
+      sums[2][wave] = n;
+    }
+  }
+  const bool odd = sum != sum;   // the thread holds a NaN or an infinity
+  __syncthreads();
+  float all = 0.0f, wide = 0.0f, same = 0.0f;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    all += sums[0][w];
+    wide += sums[1][w];
+    same += sums[2][w];
+  }
+  const Row r = finish(peak, same, all, wide);
+  if (slices == 1) {
+    if (tid == 0 && p.entropy != nullptr) p.entropy[row] = r.entropy;
+    write_given<T>(p, row, r, tid, N);
+  } else if (tid == 0) {
+    parts[blockIdx.x] = Part{peak, same, all, wide};
+  }
+  if (p.top == 0) return;
+
+  // The bound's own order may be that of a NaN's bits below -inf.
+  const float least = p.top == 1 ? peak : bound <= 0x007fffffu ? -INFINITY : value_of(bound);
+  uint64_t holders = __ballot(!(top < least) || odd);
+  while (holders != 0) {
+    const int from = __ffsll(static_cast<unsigned long long>(holders)) - 1;
+    holders &= holders - 1;
+    spread_out(from, [&](float y, int token) {
+      // Of the tokens at -inf only the first `top` can be among the top ones.
+      if (y < least || (y == -INFINITY && token >= first_token + p.top)) return;
+      const int at = atomicAdd(&count, 1);
+      if (at < kMost) found[at] = rank_of(y, token);
+    });
+  }
+  __syncthreads();
+  auto write = [&](int place, uint64_t rank) {
+    if (slices == 1)
+      write_top(p, row, r, place, rank);
+    else
+      ranks[static_cast<int64_t>(blockIdx.x) * p.top + place] = rank;
+  };
+  const int n = count;
+  if (n <= kMost) {
+    for (int i = tid; i < n; i += N) {
+      const uint64_t mine = found[i];
+      int place = 0;
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) place += found[j] > mine;
+      if (place < p.top) write(place, mine);
+    }
+    for (int i = n + tid; i < p.top; i += N) write(i, 0);   // a short slice
+    return;
+  }
+  // Rare: the slice's logits are read again for each place.
+  uint64_t last = ~uint64_t{0};
+  const int last_token = min(v1 * E - skew, p.vocab);
+  for (int place = 0; place < p.top; ++place) {
+    uint64_t mine = 0;
+    for (int token = first_token + tid; token < last_token; token += N) {
+      const uint64_t rank = rank_of(to_f32(x[token]), token);
+      if (rank < last && rank > mine) mine = rank;
+    }
+    mine = wave_max64(mine);
+    if (lane == 0) best[wave] = mine;
+    __syncthreads();
+    mine = best[0];
+#pragma unroll
+    for (int w = 1; w < W; ++w) mine = best[w] > mine ? best[w] : mine;
+    __syncthreads();
+    last = mine;
+    if (tid == 0) write(place, mine);
+  }
+}
+
+// One workgroup per row: its slices' sums, given tokens and top tokens.
+template <typename T>
+__global__ __launch_bounds__(kJoinThreads) void logprobs_join_kernel(TokenLogprobs p, int slices,
+                                                                     const Part* parts,
+                                                                     const uint64_t* ranks) {
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x;
+  parts += row * slices;
+  ranks += row * slices * p.top;
+  float peak = -INFINITY;
+  for (int i = 0; i < slices; ++i) peak = fmaxf(peak, parts[i].top);
+  float equal = 0.0f, sum = 0.0f, spread = 0.0f;
+  for (int i = 0; i < slices; ++i) {
+    const Part s = parts[i];
+    if (s.top == peak) {
+      equal += s.equal;
+      sum += s.sum;
+      spread += s.spread;
+    } else {
+      const float d = peak - s.top, f = exp2_hw(-d * kLog2e);
+      const float part = (s.sum + s.equal) * f;
+      sum += part;
+      spread += s.spread * f + (part == 0.0f ? 0.0f : d * part);
+    }
+  }
+  const Row r = finish(peak, equal, sum, spread);
+  if (tid == 0 && p.entropy != nullptr) p.entropy[row] = r.entropy;
+  write_given<T>(p, row, r, tid, kJoinThreads);
+  // Each slice's ranks fall; 0 stands behind those of a short one.
+  for (int i = tid; i < slices * p.top; i += kJoinThreads) {
+    const uint64_t mine = ranks[i];
+    if (mine == 0) continue;
+    int place = 0;
+    for (int j = 0; j < slices * p.top && place < p.top; ++j) place += ranks[j] > mine;
+    if (place < p.top) write_top(p, row, r, place, mine);
+  }
+}
+
+// How a row is cut: slices of `step` vectors.
+struct Cut {
+  int slices, step;
+};
+constexpr int kMaxVectors = 16 * 64 * 16;
+Cut cut_of(int64_t vocab, int dtype) {
+  const int64_t e = dtype == kF32 ? 4 : 8;
+  const int64_t vectors = ceil_div(vocab + e - 1, e);   // at the worst alignment
+  const int64_t slices = ceil_div(vectors, kMaxVectors);
+  return Cut{static_cast<int>(slices), static_cast<int>(ceil_div(vectors, slices))};
+}
+int64_t parts_bytes(int64_t items) { return items * static_cast<int64_t>(sizeof(Part)); }
+
+template <typename T>
+hipError_t launch_t(const TokenLogprobs& p, const Cut& c, hipStream_t st) {
+  Part* parts = static_cast<Part*>(p.workspace);
+  uint64_t* ranks = reinterpret_cast<uint64_t*>(static_cast<char*>(p.workspace) +
+                                                parts_bytes(p.rows * c.slices));
+  const dim3 grid(static_cast<uint32_t>(p.rows * c.slices));
+  auto go = [&](auto waves, auto nv) {
+    constexpr int W = decltype(waves)::value, NV = decltype(nv)::value;
+    hipLaunchKernelGGL((logprobs_kernel<T, W, NV>), grid, dim3(64 * W), 0, st, p, c.slices, c.step,
+                       parts, ranks);
+  };
+  using std::integral_constant;
+  const integral_constant<int, 4> w4;
+  const integral_constant<int, 8> w8;
+  const integral_constant<int, 16> w16;
+  if (c.step <= 256)
+    go(w4, integral_constant<int, 1>{});
+  else if (c.step <= 1024)
+    go(w4, integral_constant<int, 4>{});
+  else if (c.step <= 4096)
+    go(w8, integral_constant<int, 8>{});
+  else if (c.step <= 8192)
+    go(w8, integral_constant<int, 16>{});
+  else
+    go(w16, integral_constant<int, 16>{});
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || c.slices == 1) return e;
+  hipLaunchKernelGGL((logprobs_join_kernel<T>), dim3(static_cast<uint32_t>(p.rows)),
+                     dim3(kJoinThreads), 0, st, p, c.slices, parts, ranks);
+  return hipGetLastError();
 }
 
 }  // namespace
 
-int64_t token_logprobs_workspace(int64_t, int64_t, int64_t, int) { return 0; }
+int64_t token_logprobs_workgroups(int64_t rows, int64_t vocab, int dtype) {
+  return rows * cut_of(vocab, dtype).slices;
+}
+
+int64_t token_logprobs_workspace(int64_t rows, int64_t vocab, int64_t top, int dtype) {
+  const Cut c = cut_of(vocab, dtype);
+  if (c.slices == 1) return 0;
+  return parts_bytes(rows * c.slices) + rows * c.slices * top * 8;
+}
 
 hipError_t launch_token_logprobs(const TokenLogprobs& p, int dtype, hipStream_t st) {
-  const dim3 grid(static_cast<uint32_t>(p.rows));
-  if (dtype == kF32)
-    hipLaunchKernelGGL((logprobs_kernel<float>), grid, dim3(kThreads), 0, st, p);
-  else if (dtype == kF16)
-    hipLaunchKernelGGL((logprobs_kernel<__half>), grid, dim3(kThreads), 0, st, p);
-  else
-    hipLaunchKernelGGL((logprobs_kernel<__hip_bfloat16>), grid, dim3(kThreads), 0, st, p);
-  return hipGetLastError();
+  const Cut c = cut_of(p.vocab, dtype);
+  if (dtype == kF32) return launch_t<float>(p, c, st);
+  if (dtype == kF16) return launch_t<__half>(p, c, st);
+  return launch_t<__hip_bfloat16>(p, c, st);
 }
 
 }  // namespace w8a8

@@ -353,6 +353,7 @@ struct TokenLogprobs {
   int64_t rows;
   int vocab, given, top;
 };
+int64_t token_logprobs_workgroups(int64_t rows, int64_t vocab, int dtype);
 int64_t token_logprobs_workspace(int64_t rows, int64_t vocab, int64_t top, int dtype);
 hipError_t launch_token_logprobs(const TokenLogprobs& p, int dtype, hipStream_t st);
 
