@@ -62,6 +62,23 @@ __device__ inline void split2(float p0, float p1, uint32_t& hi, uint32_t& lo) {
   }
 }
 
+// Two probabilities rounded to the 16-bit type, packed, and l plus the two
+// rounded values.
+template <typename T>
+__device__ inline uint32_t round2(float p0, float p1, float& l) {
+  if constexpr (std::is_same<T, __half>::value) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    const h2 v = __builtin_convertvector(f32x2{p0, p1}, h2);
+    l = __builtin_amdgcn_fdot2(v, h2{1, 1}, l, false);
+    return __builtin_bit_cast(uint32_t, v);
+  } else {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    const b2 v = __builtin_convertvector(f32x2{p0, p1}, b2);
+    l = __builtin_amdgcn_fdot2_f32_bf16(v, b2{1.0f, 1.0f}, l, false);
+    return __builtin_bit_cast(uint32_t, v);
+  }
+}
+
 // Inclusive sum over the wavefront's lanes (each step a DPP move: shifts by 1,
 // 2, 4 and 8 in rows of 16 lanes, then the rows' last lanes to the next ones).
 __device__ inline uint32_t scan64(uint32_t v) {

@@ -253,23 +253,6 @@ __device__ inline f32x16 mfma_32x32x16(u32x4 a, u32x4 b, f32x16 c) {
   }
 }
 
-// Two probabilities rounded to the 16-bit type, packed, and l plus the two
-// rounded values.
-template <typename T>
-__device__ inline uint32_t round2(float p0, float p1, float& l) {
-  if constexpr (std::is_same<T, __half>::value) {
-    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-    const h2 v = __builtin_convertvector(f32x2{p0, p1}, h2);
-    l = __builtin_amdgcn_fdot2(v, h2{1, 1}, l, false);
-    return __builtin_bit_cast(uint32_t, v);
-  } else {
-    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-    const b2 v = __builtin_convertvector(f32x2{p0, p1}, b2);
-    l = __builtin_amdgcn_fdot2_f32_bf16(v, b2{1.0f, 1.0f}, l, false);
-    return __builtin_bit_cast(uint32_t, v);
-  }
-}
-
 // 16 bytes per lane from the buffer into LDS at lds + 16 * lane; zeros from
 // past its range.
 __device__ inline void dma16(__amdgpu_buffer_rsrc_t r, char* lds, int offset) {
@@ -705,14 +688,18 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) void prefill_kernel
           }
         }
         const int left = seen - key0 - 4 * h;
-        const int from = low - key0 - 4 * h, sinks = p.sinks - key0 - 4 * h;
-        const uint32_t bits = S == Seen::kTree ? drafted_bits(key0 - cached) >> (4 * h) : 0;
+        // Seen::kWindow, Seen::kTree: bit k of the lane's keys k.
+        uint32_t bits = 0;
+        if constexpr (S == Seen::kTree) bits = drafted_bits(key0 - cached) >> (4 * h);
+        if constexpr (S == Seen::kWindow) {
+          auto below = [](int n) { return n >= kKeys ? ~0u : (1u << max(n, 0)) - 1u; };
+          bits = (~below(low - key0) | below(p.sinks - key0)) >> (4 * h);
+        }
 #pragma unroll
         for (int n = 0; n < 16; ++n) {
           const int k = 8 * (n >> 2) + (n & 3);
           bool there = k <= left && ((shown >> n) & 1);
-          if constexpr (S == Seen::kWindow) there = there && (k >= from || k < sinks);
-          if constexpr (S == Seen::kTree) there = there && ((bits >> k) & 1);
+          if constexpr (S != Seen::kCausal) there = there && ((bits >> k) & 1);
           s[n] = there ? s[n] : -INFINITY;
         }
       }

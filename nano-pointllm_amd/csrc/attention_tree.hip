@@ -1,16 +1,21 @@
-// Attention of trees of drafted tokens (attention_prefill.h): a sequence's rows
-// see all of its cached keys and, by a mask, each other's.
+// Attention of trees of drafted tokens: a sequence's rows see all of its cached keys
+// and, by a mask, each other's.  Few rows per sequence and key head run as
+// attention_drafts.hip, the others as a prompt's (attention_prefill.h).
 #include "attention_prefill.h"
 
 namespace w8a8 {
 
 int64_t paged_tree_workspace(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
                              int64_t head_dim, int64_t max_keys) {
+  if (small_trees(tokens, batch, q_heads, kv_heads, head_dim))
+    return small_trees_workspace(tokens, batch, q_heads, kv_heads, head_dim, max_keys);
   return workspace_of(tokens, batch, q_heads, kv_heads, head_dim, max_keys);
 }
 
 hipError_t launch_paged_tree(const PagedAttention& a, const uint64_t* masks, int64_t ld_masks,
                              int words, bool clear, int dtype, hipStream_t st) {
+  if (small_trees(a.tokens, a.batch, a.q_heads, a.kv_heads, a.head_dim))
+    return launch_small_trees(a, masks, ld_masks, words, clear, dtype, st);
   PrefillParams p{};
   p.masks = masks;
   p.ld_masks = ld_masks;

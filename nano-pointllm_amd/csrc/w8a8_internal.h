@@ -310,6 +310,13 @@ hipError_t launch_paged_prefill_window(const PagedAttention& p, int window, int 
 // its mask, bit j % 64 of masks[row * ld_masks + j / 64] (none from 64 words on).
 int64_t paged_tree_workspace(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
                              int64_t head_dim, int64_t max_keys);
+// Whether a call of these sizes runs as attention_drafts.hip, and its parts.
+bool small_trees(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                 int64_t head_dim);
+int64_t small_trees_workspace(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                              int64_t head_dim, int64_t max_keys);
+hipError_t launch_small_trees(const PagedAttention& p, const uint64_t* masks, int64_t ld_masks,
+                              int words, bool clear, int dtype, hipStream_t st);
 hipError_t launch_paged_tree(const PagedAttention& p, const uint64_t* masks, int64_t ld_masks,
                              int words, bool clear, int dtype, hipStream_t st);
 

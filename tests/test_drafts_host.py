@@ -142,7 +142,10 @@ def test_workspaces():
                       lib.w8a8_paged_tree_workspace_bytes)
     assert dec(1, 4, 3, 64, 100, 5, 0) == -1 and dec(1, 4, 2, 64, 100, 0, 0) == -1
     assert pre(5, 1, 4, 2, 264, 100, 5, 0) == -1 and pre(5, 1, 4, 2, 64, 100, 5, -1) == -1
-    assert tree(-1, 1, 4, 2, 64, 100) == -1
+    assert tree(-1, 1, 4, 2, 64, 100) == -1 and tree(5, 1, 4, 2, 60, 100) == -1
+    assert tree(5, 1, 4, 2, 64, -1) == -1 and tree(5, 1, 4, 2, 64, 1 << 32) == -1
+    assert tree(0, 0, 4, 2, 64, 64) == 0 < tree(300, 1, 8, 2, 64, 1 << 14)
+    assert tree(5, 1, 4, 2, 64, 128) == 0 < tree(5, 1, 4, 2, 64, 1 << 14)
     # By what is seen, not by the table's width; all of it for a wide window.
     assert dec(1, 32, 8, 128, 1 << 17, 100, 4) == 0 < dec(1, 32, 8, 128, 1 << 17, 1 << 16, 4)
     assert dec(1, 32, 8, 128, 1 << 17, 1 << 17, 4) == \
