@@ -146,7 +146,7 @@ __global__ __launch_bounds__(64 * W, NV > 8 ? 4 : NV > 4 ? 6 : 8) void logprobs_
     TokenLogprobs p, int slices, int step, Part* parts, uint64_t* ranks) {
   constexpr int E = per_vector<T>();
   constexpr int N = 64 * W;
-  __shared__ u32x4 stage[W][NV];
+  __shared__ u32x4 stage[W][NV + 1];
   __shared__ float tops[W];
   __shared__ float sums[3][W];
   __shared__ uint32_t group[kGroups];
@@ -160,47 +160,53 @@ __global__ __launch_bounds__(64 * W, NV > 8 ? 4 : NV > 4 ? 6 : 8) void logprobs_
   const int64_t row = blockIdx.x / slices;
   const int slice = blockIdx.x % slices;
   const T* x = static_cast<const T*>(p.logits) + row * p.ld;
-  // Vectors are aligned: the first may begin before the row and the last end
-  // behind it; those two are read element by element.
+  // Vectors are aligned: of the row's first and last one a part may lie outside.
+  // Those two are read element by element, by the first slice's threads 0 and 1.
   const int skew = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
-  const int v0 = slice * step;
-  const int v1 = min(v0 + step, (p.vocab + skew + E - 1) / E);
-  const int first_token = max(v0 * E - skew, 0);
+  const int full0 = skew > 0 ? 1 : 0, full1 = (p.vocab + skew) / E;   // whole ones
+  const int v0 = full0 + slice * step, v1 = min(v0 + step, full1);
+  const int first_token = slice == 0 ? 0 : v0 * E - skew;
   const u32x4* vectors = reinterpret_cast<const u32x4*>(x - skew);
+  // The token of element j of the thread's vector n (below 0: none).
+  const int lone = slice > 0 ? -1 : tid == 0 && skew > 0 ? 0
+                                : tid == 1 && full1 >= full0 && full1 * E < p.vocab + skew ? full1
+                                                                                          : -1;
+  auto token_at = [&](int thread_lone, int thread, int n, int j) {
+    return (n == NV ? thread_lone : v0 + n * N + thread) * E - skew + j;
+  };
 
-  u32x4 raw[NV];
-#pragma unroll
-  for (int n = 0; n < NV; ++n) {
-    const int v = v0 + n * N + tid;
+  u32x4 raw[NV + 1];
+  {
     const uint32_t none = minus_infinity<T>();
-    raw[n] = u32x4{none, none, none, none};
-    if (v < v1 && v * E >= skew && (v + 1) * E <= p.vocab + skew) raw[n] = vectors[v];
+    raw[NV] = u32x4{none, none, none, none};
   }
+  if (lone >= 0) {
 #pragma unroll
-  for (int n = 0; n < NV; ++n) {
-    const int v = v0 + n * N + tid;
-    if (v < v1 && (v * E < skew || (v + 1) * E > p.vocab + skew)) {
-#pragma unroll
-      for (int j = 0; j < E; ++j) {
-        const int token = v * E - skew + j;
-        if (token < 0 || token >= p.vocab) continue;
-        if constexpr (std::is_same<T, float>::value) {
-          raw[n][j] = __float_as_uint(x[token]);
-        } else {
-          const uint32_t b = reinterpret_cast<const uint16_t*>(x)[token];
-          const uint32_t w = raw[n][j >> 1];
-          raw[n][j >> 1] = (j & 1) ? (w & 0xffffu) | b << 16 : (w & 0xffff0000u) | b;
-        }
+    for (int j = 0; j < E; ++j) {
+      const int token = lone * E - skew + j;
+      if (token < 0 || token >= p.vocab) continue;
+      if constexpr (std::is_same<T, float>::value) {
+        raw[NV][j] = __float_as_uint(x[token]);
+      } else {
+        const uint32_t b = reinterpret_cast<const uint16_t*>(x)[token];
+        const uint32_t w = raw[NV][j >> 1];
+        raw[NV][j >> 1] = (j & 1) ? (w & 0xffffu) | b << 16 : (w & 0xffff0000u) | b;
       }
     }
+  }
+  // Every thread loads every vector, one behind the slice's end its last: without
+  // branches the first are used while the others are in flight.
+  if (v0 < v1) {
+#pragma unroll
+    for (int n = 0; n < NV; ++n) raw[n] = vectors[min(v0 + n * N + tid, v1 - 1)];
   }
   if (tid == 0) count = 0;
 
   // sum = sum of 2^t, spread = sum of t 2^t with t = (x - ref) log2(e).
   float top = -INFINITY, ref = 0.0f, sum = 0.0f, spread = 0.0f;
 #pragma unroll
-  for (int n = 0; n < NV; ++n) {
-    if (v0 + n * N + tid >= v1) continue;
+  for (int n = 0; n <= NV; ++n) {
+    if (n == NV ? lone < 0 : v0 + n * N + tid >= v1) continue;
     float most = element<T>(raw[n], 0);
 #pragma unroll
     for (int j = 1; j < E; ++j) most = fmaxf(most, element<T>(raw[n], j));
@@ -249,18 +255,19 @@ __global__ __launch_bounds__(64 * W, NV > 8 ? 4 : NV > 4 ? 6 : 8) void logprobs_
     __builtin_amdgcn_wave_barrier();
     if (lane == from) {
 #pragma unroll
-      for (int n = 0; n < NV; ++n) stage[wave][n] = raw[n];
+      for (int n = 0; n <= NV; ++n) stage[wave][n] = raw[n];
     }
+    const int its = __builtin_amdgcn_readlane(lone, from);
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     const T* values = reinterpret_cast<const T*>(stage[wave]);
 #pragma unroll
-    for (int i = 0; i < NV * E; i += 64) {
-      const int at = i + lane;
-      const int v = v0 + at / E * N + wave * 64 + from;
-      const int token = v * E - skew + at % E;
-      if (at < NV * E && v < v1 && token >= 0 && token < p.vocab) f(to_f32(values[at]), token);
+    for (int i = 0; i < (NV + 1) * E; i += 64) {
+      const int at = i + lane, n = at / E;
+      if (at >= (NV + 1) * E || (n == NV ? its < 0 : v0 + n * N + wave * 64 + from >= v1)) continue;
+      const int token = token_at(its, wave * 64 + from, n, at % E);
+      if (token >= 0 && token < p.vocab) f(to_f32(values[at]), token);
     }
     __builtin_amdgcn_wave_barrier();
   };
@@ -347,10 +354,13 @@ __global__ __launch_bounds__(64 * W, NV > 8 ? 4 : NV > 4 ? 6 : 8) void logprobs_
   }
   // Rare: the slice's logits are read again for each place.
   uint64_t last = ~uint64_t{0};
-  const int last_token = min(v1 * E - skew, p.vocab);
+  const int last_token = slices == 1 ? p.vocab : max(v1 * E - skew, first_token);
+  // The first of several slices has the row's last tokens too.
+  const int more = slices > 1 && slice == 0 ? p.vocab - (full1 * E - skew) : 0;
   for (int place = 0; place < p.top; ++place) {
     uint64_t mine = 0;
-    for (int token = first_token + tid; token < last_token; token += N) {
+    for (int i = first_token + tid; i < last_token + more; i += N) {
+      const int token = i < last_token ? i : i - last_token + full1 * E - skew;
       const uint64_t rank = rank_of(to_f32(x[token]), token);
       if (rank < last && rank > mine) mine = rank;
     }
@@ -411,7 +421,7 @@ struct Cut {
 constexpr int kMaxVectors = 16 * 64 * 16;
 Cut cut_of(int64_t vocab, int dtype) {
   const int64_t e = dtype == kF32 ? 4 : 8;
-  const int64_t vectors = ceil_div(vocab + e - 1, e);   // at the worst alignment
+  const int64_t vectors = std::max<int64_t>(vocab / e, 1);   // whole ones at most
   const int64_t slices = ceil_div(vectors, kMaxVectors);
   return Cut{static_cast<int>(slices), static_cast<int>(ceil_div(vectors, slices))};
 }

@@ -412,8 +412,7 @@ def paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
             return paged_decode(q, k_cache, v_cache, page_table, lengths, scale=scale,
                                 window=window, sinks=sinks, out=out)
     if window is not None or sinks:
-        return _decode_window(q, k_cache, v_cache, page_table, lengths, scale, window, sinks, out,
-                              index)
+        _window(window, sinks)
     code = _rows(q, "q")
     q, qs = _queries(q)
     b, h, d = q.shape
@@ -422,6 +421,16 @@ def paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     lengths = _index(lengths, torch.int32, b, "lengths")
     out = _out_like(out, q)
     os = out.stride()
+    if window is not None:
+        need = _decode_window_workspace(b, h, g, d, width * page_size, window, sinks)
+        ws = q.new_empty(((need + 1) // 2,)) if need > 0 else None
+        _lib.check(_lib.load().w8a8_paged_decode_window(
+            q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1],
+            cs[2], pages, page_size, page_table.data_ptr(), ld, width, lengths.data_ptr(), window,
+            sinks, code, d ** -0.5 if scale is None else scale, out.data_ptr(), os[0], os[1], b, h,
+            g, d, None if ws is None else ws.data_ptr(), need,
+            torch._C._cuda_getCurrentRawStream(index)), "w8a8_paged_decode_window")
+        return out
     need = _decode_workspace(b, h, g, d, width * page_size)
     ws = q.new_empty(((need + 1) // 2,)) if need > 0 else None
     _lib.check(_lib.load().w8a8_paged_decode(
@@ -430,30 +439,6 @@ def paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
         d ** -0.5 if scale is None else scale, out.data_ptr(), os[0], os[1], b, h, g, d,
         None if ws is None else ws.data_ptr(), need, torch._C._cuda_getCurrentRawStream(index)),
         "w8a8_paged_decode")
-    return out
-
-
-def _decode_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
-                   page_table: torch.Tensor, lengths: torch.Tensor, scale: float | None,
-                   window: int | None, sinks: int, out: torch.Tensor | None, index: int
-                   ) -> torch.Tensor:
-    _window(window, sinks)
-    code = _rows(q, "q")
-    q, qs = _queries(q)
-    b, h, d = q.shape
-    (pages, g, page_size, _), cs = _cache(k_cache, v_cache, q, d)
-    page_table, ld, width = _table(page_table, b)
-    lengths = _index(lengths, torch.int32, b, "lengths")
-    out = _out_like(out, q)
-    os = out.stride()
-    need = _decode_window_workspace(b, h, g, d, width * page_size, window, sinks)
-    ws = q.new_empty(((need + 1) // 2,)) if need > 0 else None
-    _lib.check(_lib.load().w8a8_paged_decode_window(
-        q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2],
-        pages, page_size, page_table.data_ptr(), ld, width, lengths.data_ptr(), window, sinks,
-        code, d ** -0.5 if scale is None else scale, out.data_ptr(), os[0], os[1], b, h, g, d,
-        None if ws is None else ws.data_ptr(), need, torch._C._cuda_getCurrentRawStream(index)),
-        "w8a8_paged_decode_window")
     return out
 
 
@@ -597,7 +582,8 @@ def paged_accept(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch
     if len(shape) not in (4, 5) or shape != v_cache.shape:
         raise ValueError("k_cache and v_cache must be [pages, kv_heads, page_size, head_dim] "
                          "or [layers, ...] of these")
-    if strides[-1] != 1 or any(n > 1 and x != y for n, x, y in zip(shape, strides, other)):
+    if strides[-1] != 1 or strides != other and any(
+            n > 1 and x != y for n, x, y in zip(shape, strides, other)):
         raise ValueError("k_cache and v_cache must have equal strides and contiguous heads")
     layers, ls = (shape[0], strides[0]) if len(shape) == 5 else (1, 0)
     pages, g, page_size, d = shape[-4:]

@@ -17,6 +17,7 @@ prompt, or accepts drafted tokens.
 """
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import NamedTuple
 
 import torch
@@ -111,6 +112,11 @@ MAX_VOCAB = 1 << 20
 _LOGIT_CODES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
 
 
+@lru_cache(maxsize=1024)
+def _logprobs_workspace(rows: int, vocab: int, top: int, code: int) -> int:
+    return int(_lib.load().w8a8_token_logprobs_workspace_bytes(rows, vocab, top, code))
+
+
 class TokenLogprobs(NamedTuple):
     logprobs: torch.Tensor                  # float32, the tokens' shape
     entropy: torch.Tensor                   # float32 [...], in nats
@@ -128,40 +134,49 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) 
     vocabulary NaN.  Among equal logits the lowest token comes first.  Sums and
     results are binary32; a logit of -inf has probability 0, a row with +inf,
     NaN or nothing above -inf gives NaN."""
-    device = _lib.require_cuda(logits, tokens)
+    # A decode step scores its rows eagerly, bounded by the host: each attribute is
+    # read once, sizes of workspaces are kept by call.
+    index = logits.get_device()
+    if index < 0 or tokens.get_device() != index:
+        _lib.require_cuda(logits, tokens)    # raises, naming the reason
     code = _LOGIT_CODES.get(logits.dtype)
-    if code is None or logits.dim() < 1:
+    axes = logits.dim() - 1
+    if code is None or axes < 0:
         raise ValueError("logits must be float16, bfloat16 or float32 [..., vocab]")
     shape, vocab = logits.shape[:-1], logits.shape[-1]
     if not 1 <= vocab <= MAX_VOCAB:
         raise ValueError(f"the vocabulary must have 1 to {MAX_VOCAB} tokens")
-    if tokens.dtype != torch.int64 or tokens.shape[:len(shape)] != shape \
-            or tokens.dim() > len(shape) + 1:
+    given = tokens.shape
+    if tokens.dtype != torch.int64 or given[:axes] != shape or len(given) > axes + 1:
         raise ValueError("tokens must be int64 of the rows' shape, or with one more axis")
     if type(top) is not int or not 0 <= top <= min(MAX_TOP, vocab):
         raise ValueError(f"top must be 0 to {MAX_TOP} and at most the vocabulary")
-    if device.index != torch._C._cuda_getDevice():
-        with torch.cuda.device(device):
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
             return token_logprobs(logits, tokens, top=top)
-    x = logits.reshape(-1, vocab)
+    x = logits if axes == 1 else logits.reshape(-1, vocab)
     rows = x.shape[0]
-    if x.stride(1) != 1 and vocab > 1 or x.stride(0) < vocab and rows > 1:
-        x = x.contiguous()
-    per = tokens.shape[-1] if tokens.dim() > len(shape) else 1
-    tokens = tokens.contiguous()
-    logprobs = torch.empty(tokens.shape, device=device, dtype=torch.float32)
-    entropy = torch.empty(shape, device=device, dtype=torch.float32)
+    ld, step = x.stride()
+    if step != 1 and vocab > 1 or ld < vocab and rows > 1:
+        x, ld = x.contiguous(), vocab
+    elif rows == 1:
+        ld = vocab
+    per = given[-1] if len(given) > axes else 1
+    if not tokens.is_contiguous():
+        tokens = tokens.contiguous()
+    logprobs = logits.new_empty(given, dtype=torch.float32)
+    entropy = logits.new_empty(shape, dtype=torch.float32)
     best = ids = None
     if top:
-        best = torch.empty((*shape, top), device=device, dtype=torch.float32)
-        ids = torch.empty((*shape, top), device=device, dtype=torch.int64)
+        best = logits.new_empty((*shape, top), dtype=torch.float32)
+        ids = logits.new_empty((*shape, top), dtype=torch.int64)
     if rows == 0:
         return TokenLogprobs(logprobs, entropy, best, ids)
-    lib = _lib.load()
-    need = lib.w8a8_token_logprobs_workspace_bytes(rows, vocab, top, code)
-    ws = torch.empty(need, device=device, dtype=torch.uint8) if need > 0 else None
-    _lib.check(lib.w8a8_token_logprobs(
-        x.data_ptr(), x.stride(0), code, tokens.data_ptr(), per, per, top, logprobs.data_ptr(),
-        entropy.data_ptr(), _lib.ptr(best), _lib.ptr(ids), rows, vocab, _lib.ptr(ws), need,
-        _lib.stream_handle(device)), "w8a8_token_logprobs")
+    need = _logprobs_workspace(rows, vocab, top, code)
+    ws = logits.new_empty(need, dtype=torch.uint8) if need > 0 else None
+    _lib.check(_lib.load().w8a8_token_logprobs(
+        x.data_ptr(), ld, code, tokens.data_ptr(), per, per, top, logprobs.data_ptr(),
+        entropy.data_ptr(), best.data_ptr() if top else None, ids.data_ptr() if top else None, rows,
+        vocab, None if ws is None else ws.data_ptr(), need,
+        torch._C._cuda_getCurrentRawStream(index)), "w8a8_token_logprobs")
     return TokenLogprobs(logprobs, entropy, best, ids)
