@@ -691,7 +691,7 @@ int w8a8_cache_accept(void* k_cache, void* v_cache, int64_t cache_stride_layer,
  * largest).  All results are binary32 from binary32 sums; -inf logits have
  * probability 0, a row with +inf, NaN or nothing above -inf gives NaN.
  * A term exp(x[j] - max) below 2^-126 counts as 0.  rows < 2^22 (2^17 where the
- * vocabulary passes 2^16), vocab <= 2^20; outputs are contiguous and overlap
+ * vocabulary passes 2^15), vocab <= 2^20; outputs are contiguous and overlap
  * nothing.
  * Workspace: w8a8_token_logprobs_workspace_bytes(rows, vocab, top, dtype) bytes,
  * 16-byte aligned; no state survives the call.

@@ -12,7 +12,7 @@
 //     reference per thread that is the maximum so far or up to kSlack below.
 //   * The thread whose logit is the row's maximum leaves its sums: its wavefront
 //     adds its logits up again through LDS, with the maximum left out and counted.
-//   * Top tokens: the k-th largest of 256 groups' maxima bounds the k-th largest
+//   * Top tokens: the k-th largest of 128 groups' maxima bounds the k-th largest
 //     logit from below, and few logits reach it (k and some, rarely 2 k).  They go
 //     through LDS, in any order, and each counts those before it: its place.  Ties
 //     are broken by the token's number, so the order of arrival changes nothing.
@@ -29,10 +29,14 @@ namespace w8a8 {
 namespace {
 
 constexpr int kMost = 1024;        // candidates that a workgroup ranks
-constexpr int kGroups = 256;       // maxima that the bound is taken from
+constexpr int kGroups = 128;       // maxima that the bound is taken from
+constexpr int kFewHolders = 4;     // threads of a wavefront whose logits are spread over it
+constexpr int kRankers = 8;        // threads that count those before one of many candidates
+constexpr int kFew = 24;
 constexpr float kSlack = 8.0f;     // in powers of two
 constexpr float kLn2 = 0.693147180559945309417f;
 constexpr int kJoinThreads = 256;
+constexpr int kMaxSlices = 32;
 
 // What a slice leaves for the join.
 struct Part {
@@ -97,18 +101,43 @@ __device__ inline uint64_t wave_max64(uint64_t x) {
   return x;
 }
 
-// The k-th largest of 4 x 64 orders, to its upper 16 bits, rounded down.
-__device__ inline uint32_t kth_order(const uint32_t (&g)[4], int k) {
+// The k-th largest of kGroups orders, to its upper 16 bits, rounded down.
+__device__ inline uint32_t kth_order(const uint32_t (&g)[kGroups / 64], int k) {
   uint32_t t = 0;
 #pragma unroll 1
   for (int bit = 31; bit >= 16; --bit) {
     const uint32_t next = t | 1u << bit;
     int n = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) n += __popcll(__ballot(g[i] >= next));
+    for (int i = 0; i < kGroups / 64; ++i) n += __popcll(__ballot(g[i] >= next));
     if (n >= k) t = next;
   }
   return t;
+}
+
+// f(place, rank) of each of n different ranks in LDS: its place among them, by counting
+// those before it; of many, by several threads each.
+template <typename F>
+__device__ inline void rank_all(const uint64_t* ranks, int n, int tid, int threads, F f) {
+  if (n <= kFew) {
+    if (tid >= n) return;
+    const uint64_t mine = ranks[tid];
+    int place = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) place += ranks[j] > mine;
+    f(place, mine);
+    return;
+  }
+  const int part = tid % kRankers;
+  for (int i = tid / kRankers; i < n; i += threads / kRankers) {
+    const uint64_t mine = ranks[i];
+    int place = 0;
+#pragma unroll 4
+    for (int j = part; j < n; j += kRankers) place += ranks[j] > mine;
+#pragma unroll
+    for (int w = 1; w < kRankers; w <<= 1) place += __shfl_xor(place, w);
+    if (part == 0) f(place, mine);
+  }
 }
 
 // The results of a row whose logits are known but for the given tokens'.
@@ -243,9 +272,9 @@ __global__ __launch_bounds__(64 * W, NV > 8 ? 4 : NV > 4 ? 6 : 8) void logprobs_
 #pragma unroll
   for (int w = 1; w < W; ++w) peak = fmaxf(peak, tops[w]);
   if (p.top > 1 && wave == 0) {
-    uint32_t g[4];
+    uint32_t g[kGroups / 64];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) g[i] = group[lane + 64 * i];
+    for (int i = 0; i < kGroups / 64; ++i) g[i] = group[lane + 64 * i];
     const uint32_t t = kth_order(g, p.top);
     if (lane == 0) bound = t;
   }
@@ -322,16 +351,35 @@ __global__ __launch_bounds__(64 * W, NV > 8 ? 4 : NV > 4 ? 6 : 8) void logprobs_
 
   // The bound's own order may be that of a NaN's bits below -inf.
   const float least = p.top == 1 ? peak : bound <= 0x007fffffu ? -INFINITY : value_of(bound);
-  uint64_t holders = __ballot(!(top < least) || odd);
-  while (holders != 0) {
-    const int from = __ffsll(static_cast<unsigned long long>(holders)) - 1;
-    holders &= holders - 1;
-    spread_out(from, [&](float y, int token) {
-      // Of the tokens at -inf only the first `top` can be among the top ones.
-      if (y < least || (y == -INFINITY && token >= first_token + p.top)) return;
-      const int at = atomicAdd(&count, 1);
-      if (at < kMost) found[at] = rank_of(y, token);
-    });
+  // Of the tokens at -inf only the first `top` can be among the top ones.
+  auto offer = [&](float y, int token) {
+    if (y < least || (y == -INFINITY && token >= first_token + p.top)) return;
+    const int at = atomicAdd(&count, 1);
+    if (at < kMost) found[at] = rank_of(y, token);
+  };
+  const bool holds = !(top < least) || odd;
+  uint64_t holders = __ballot(holds);
+  if (__popcll(holders) <= kFewHolders) {
+    while (holders != 0) {
+      const int from = __ffsll(static_cast<unsigned long long>(holders)) - 1;
+      holders &= holders - 1;
+      spread_out(from, offer);
+    }
+  } else if (holds) {
+    // Each looks through its own, a vector at a time.
+#pragma unroll
+    for (int n = 0; n <= NV; ++n) {
+      if (n == NV ? lone < 0 : v0 + n * N + tid >= v1) continue;
+      bool any = false;
+#pragma unroll
+      for (int j = 0; j < E; ++j) any = any || !(element<T>(raw[n], j) < least);
+      if (!any) continue;
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const int token = token_at(lone, tid, n, j);
+        if (token >= 0 && token < p.vocab) offer(element<T>(raw[n], j), token);
+      }
+    }
   }
   __syncthreads();
   auto write = [&](int place, uint64_t rank) {
@@ -342,13 +390,9 @@ __global__ __launch_bounds__(64 * W, NV > 8 ? 4 : NV > 4 ? 6 : 8) void logprobs_
   };
   const int n = count;
   if (n <= kMost) {
-    for (int i = tid; i < n; i += N) {
-      const uint64_t mine = found[i];
-      int place = 0;
-#pragma unroll 4
-      for (int j = 0; j < n; ++j) place += found[j] > mine;
-      if (place < p.top) write(place, mine);
-    }
+    rank_all(found, n, tid, N, [&](int place, uint64_t rank) {
+      if (place < p.top) write(place, rank);
+    });
     for (int i = n + tid; i < p.top; i += N) write(i, 0);   // a short slice
     return;
   }
@@ -404,25 +448,34 @@ __global__ __launch_bounds__(kJoinThreads) void logprobs_join_kernel(TokenLogpro
   const Row r = finish(peak, equal, sum, spread);
   if (tid == 0 && p.entropy != nullptr) p.entropy[row] = r.entropy;
   write_given<T>(p, row, r, tid, kJoinThreads);
-  // Each slice's ranks fall; 0 stands behind those of a short one.
-  for (int i = tid; i < slices * p.top; i += kJoinThreads) {
-    const uint64_t mine = ranks[i];
-    if (mine == 0) continue;
-    int place = 0;
-    for (int j = 0; j < slices * p.top && place < p.top; ++j) place += ranks[j] > mine;
-    if (place < p.top) write_top(p, row, r, place, mine);
-  }
+  if (p.top == 0) return;
+  // 0 stands behind the ranks of a short slice.
+  __shared__ uint64_t all[kMaxSlices * kLogprobsMaxTop];
+  const int n = slices * p.top;
+  for (int i = tid; i < n; i += kJoinThreads) all[i] = ranks[i];
+  __syncthreads();
+  rank_all(all, n, tid, kJoinThreads, [&](int place, uint64_t rank) {
+    if (place < p.top && rank != 0) write_top(p, row, r, place, rank);
+  });
 }
 
-// How a row is cut: slices of `step` vectors.
+// How a row is cut: slices of `step` vectors.  A workgroup of 16 wavefronts holds
+// 16384 vectors but has its CU to itself, so that nothing covers its loads: rows that
+// need so many are cut in two, for two workgroups on a CU, once there are two rows
+// per CU (1024 rows of 128256 bfloat16 logits: 61 against 70 us, with 20 top tokens
+// 79 against 84; 256 rows: 21 against 19, 29 against 24), and so is any row that is
+// cut at all (8 rows of 262144: 12 against 16 us).
 struct Cut {
   int slices, step;
 };
-constexpr int kMaxVectors = 16 * 64 * 16;
-Cut cut_of(int64_t vocab, int dtype) {
-  const int64_t e = dtype == kF32 ? 4 : 8;
-  const int64_t vectors = std::max<int64_t>(vocab / e, 1);   // whole ones at most
-  const int64_t slices = ceil_div(vectors, kMaxVectors);
+constexpr int kMostVectors = 16 * 64 * 16;
+constexpr int kShared = 8 * 64 * 16;   // of a workgroup that shares its CU
+constexpr int64_t kManyRows = 512;
+static_assert(kLogprobsMaxVocab / 4 / kShared <= kMaxSlices);
+Cut cut_of(int64_t rows, int64_t vocab, int dtype) {
+  const int64_t vectors = std::max<int64_t>(vocab / (dtype == kF32 ? 4 : 8), 1);   // whole ones
+  const bool alone = vectors <= kMostVectors && rows <= kManyRows;
+  const int64_t slices = ceil_div(vectors, alone ? kMostVectors : kShared);
   return Cut{static_cast<int>(slices), static_cast<int>(ceil_div(vectors, slices))};
 }
 int64_t parts_bytes(int64_t items) { return items * static_cast<int64_t>(sizeof(Part)); }
@@ -462,17 +515,17 @@ hipError_t launch_t(const TokenLogprobs& p, const Cut& c, hipStream_t st) {
 }  // namespace
 
 int64_t token_logprobs_workgroups(int64_t rows, int64_t vocab, int dtype) {
-  return rows * cut_of(vocab, dtype).slices;
+  return rows * cut_of(rows, vocab, dtype).slices;
 }
 
 int64_t token_logprobs_workspace(int64_t rows, int64_t vocab, int64_t top, int dtype) {
-  const Cut c = cut_of(vocab, dtype);
+  const Cut c = cut_of(rows, vocab, dtype);
   if (c.slices == 1) return 0;
   return parts_bytes(rows * c.slices) + rows * c.slices * top * 8;
 }
 
 hipError_t launch_token_logprobs(const TokenLogprobs& p, int dtype, hipStream_t st) {
-  const Cut c = cut_of(p.vocab, dtype);
+  const Cut c = cut_of(p.rows, p.vocab, dtype);
   if (dtype == kF32) return launch_t<float>(p, c, st);
   if (dtype == kF16) return launch_t<__half>(p, c, st);
   return launch_t<__hip_bfloat16>(p, c, st);
