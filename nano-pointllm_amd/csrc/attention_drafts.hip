@@ -57,6 +57,7 @@ struct TreeParams {
   int group;               // query heads per key head
   bool whole;              // no sequence is cut
   bool clear;              // rows of no sequence become zeros
+  int items;               // that the workspace has room for
   float* part_o;           // [items x kv_heads, rows of a block, head_dim]
   f32x2* part_rl;          // [items x kv_heads, rows of a block]
 };
@@ -256,6 +257,7 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 2 : 1) void tree_kernel(TreeParams
     if (p.clear) clear_rows(p, kvh, slot - x.start, gridDim.x / a.kv_heads - x.start);
     return;
   }
+  if (slot >= p.items) return;   // starts that decrease: more rows than the batch has
   const int keys = x.keys, cached = x.keys - x.count;
   const int t0 = static_cast<int>(static_cast<int64_t>(x.tiles) * x.piece / x.pieces);
   const int t1 = static_cast<int>(static_cast<int64_t>(x.tiles) * (x.piece + 1) / x.pieces);
@@ -591,7 +593,8 @@ __global__ __launch_bounds__(kJoinThreads) void tree_join_kernel(TreeParams p) {
   const int lane = threadIdx.x % 64, c = lane % C, first = lane / C;
   const int in = blockIdx.y * G + threadIdx.x / 64;
   const int n = x.pieces, row = x.block * R + in;
-  if (x.seq < 0 || n <= 1 || row >= x.count * p.group) return;
+  if (x.seq < 0 || n <= 1 || row >= x.count * p.group || x.first + (x.block + 1) * n > p.items)
+    return;
   const int64_t step = static_cast<int64_t>(a.kv_heads) * R;
   const int64_t at = static_cast<int64_t>(x.first + x.block * n) * step + kvh * R + in;
   float top = -INFINITY;
@@ -710,6 +713,7 @@ hipError_t launch_small_trees(const PagedAttention& a, const uint64_t* masks, in
   p.clear = clear;
   const Plan x = plan_of(a.tokens, a.batch, p.group, a.kv_heads, a.max_keys);
   p.whole = x.whole;
+  p.items = static_cast<int>(x.items);
   char* ws = static_cast<char*>(a.workspace);
   p.part_rl = reinterpret_cast<f32x2*>(ws);
   p.part_o = reinterpret_cast<float*>(ws + pairs_bytes(x.items * a.kv_heads * x.rows));

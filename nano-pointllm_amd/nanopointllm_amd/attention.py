@@ -507,35 +507,55 @@ def _prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     page_table, ld, width = _table(page_table, b)
     lengths = _index(lengths, torch.int32, b, "lengths")
     q_starts = _index(q_starts, torch.int32, b + 1, "q_starts")
-    if masks is not None:
-        masks, ld_masks, words = _masks(masks, t)
     out = _out_like(out, q)
     os = out.stride()
-    if masks is not None:
-        need = _tree_workspace(t, b, h, g, d, width * page_size)
-    elif window is None:
-        need = _prefill_workspace(t, b, h, g, d, width * page_size)
-    else:
-        need = _prefill_window_workspace(t, b, h, g, d, width * page_size, window, sinks)
+    if masks is not None or window is not None:
+        return _prefill_masked(q, k_cache, v_cache, page_table, lengths, q_starts, scale, out,
+                               clear, window, sinks, masks, ld, width, code, index)
+    need = _prefill_workspace(t, b, h, g, d, width * page_size)
     ws = q.new_empty(((need + 1) // 2,)) if need > 0 else None
     if clear and b == 0:
         return out.zero_()
     lib = _lib.load()
+    _lib.check((lib.w8a8_paged_prefill_padded if clear else lib.w8a8_paged_prefill)(
+        q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2],
+        pages, page_size, page_table.data_ptr(), ld, width, lengths.data_ptr(),
+        q_starts.data_ptr(), code, d ** -0.5 if scale is None else scale, out.data_ptr(), os[0],
+        os[1], t, b, h, g, d, None if ws is None else ws.data_ptr(), need,
+        torch._C._cuda_getCurrentRawStream(index)), "w8a8_paged_prefill")
+    return out
+
+
+def _prefill_masked(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                    page_table: torch.Tensor, lengths: torch.Tensor, q_starts: torch.Tensor,
+                    scale: float | None, out: torch.Tensor, clear: bool, window: int | None,
+                    sinks: int, masks: torch.Tensor | None, ld: int, width: int, code: int,
+                    index: int) -> torch.Tensor:
+    """The windowed and the tree call of :func:`_prefill`, whose arguments are
+    checked."""
+    (t, h, d), (pages, g, page_size, _), b = q.shape, k_cache.shape, lengths.shape[0]
+    qs, cs, os = q.stride(), k_cache.stride(), out.stride()
+    if masks is not None:
+        masks, ld_masks, words = _masks(masks, t)
+        need = _tree_workspace(t, b, h, g, d, width * page_size)
+    else:
+        need = _prefill_window_workspace(t, b, h, g, d, width * page_size, window, sinks)
+    if clear and b == 0:
+        return out.zero_()
+    ws = q.new_empty(((need + 1) // 2,)) if need > 0 else None
     given = (q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1],
              cs[2], pages, page_size, page_table.data_ptr(), ld, width, lengths.data_ptr(),
              q_starts.data_ptr())
-    rest = (code, d ** -0.5 if scale is None else scale, out.data_ptr(), os[0], os[1], t, b, h, g,
-            d, None if ws is None else ws.data_ptr(), need,
+    rest = (clear, code, d ** -0.5 if scale is None else scale, out.data_ptr(), os[0], os[1], t, b,
+            h, g, d, None if ws is None else ws.data_ptr(), need,
             torch._C._cuda_getCurrentRawStream(index))
+    lib = _lib.load()
     if masks is not None:
-        status = lib.w8a8_paged_tree(*given, masks.data_ptr(), ld_masks, words, clear, *rest)
-    elif window is not None:
-        status = lib.w8a8_paged_prefill_window(*given, window, sinks, clear, *rest)
+        _lib.check(lib.w8a8_paged_tree(*given, masks.data_ptr(), ld_masks, words, *rest),
+                   "w8a8_paged_tree")
     else:
-        status = (lib.w8a8_paged_prefill_padded if clear else lib.w8a8_paged_prefill)(
-            *given, *rest)
-    if status != _lib.OK:
-        _lib.check(status, "w8a8_paged_prefill" if masks is None else "w8a8_paged_tree")
+        _lib.check(lib.w8a8_paged_prefill_window(*given, window, sinks, *rest),
+                   "w8a8_paged_prefill_window")
     return out
 
 
@@ -748,8 +768,9 @@ class PagedAttentionCore:
         window = self.window[layer_index] if isinstance(self.window, list) else self.window
         sinks = 0 if window is None else self.sinks
         table, lengths, n = state.page_table, state.lengths, state.decode_rows
-        if state.masks is not None and window is not None:
-            raise ValueError("trees of drafted tokens run on layers without a window")
+        if state.masks is not None and (window is not None or state.q_starts is None):
+            raise ValueError("trees of drafted tokens run on layers without a window" if window
+                             else "masks need the q_starts of their trees")
         q = rotary_store(q, k, v, state.positions, state.slots, self.frequencies.inv_freq,
                          k_cache, v_cache, layout=self.layout,
                          attention_factor=self.frequencies.attention_factor)

@@ -133,7 +133,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) 
     tokens of each row; -1 (a padded place) gives 0, another number outside the
     vocabulary NaN.  Among equal logits the lowest token comes first.  Sums and
     results are binary32; a logit of -inf has probability 0, a row with +inf,
-    NaN or nothing above -inf gives NaN."""
+    NaN or nothing above -inf gives NaN.  One kernel for rows of up to 131072
+    16-bit logits (65536 binary32), two for longer ones; no autograd."""
     # A decode step scores its rows eagerly, bounded by the host: each attribute is
     # read once, sizes of workspaces are kept by call.
     index = logits.get_device()

@@ -68,6 +68,9 @@ def test_windows_refused():
     q = torch.zeros(1, 1, 64, dtype=torch.float16)
     with pytest.raises(ValueError, match="without a window"):
         core(q, q, q, 1, state)
+    state.q_starts = None
+    with pytest.raises(ValueError, match="q_starts"):
+        core(q, q, q, 0, state)
     with pytest.raises(ValueError, match="sinks"):
         A.paged_prefill(q, *[None] * 5, sinks=1)
 

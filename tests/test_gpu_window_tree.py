@@ -385,3 +385,17 @@ def test_captured_steps_on_two_streams(cuda):
         got = step()
     side.synchronize()
     assert torch.equal(got, want)
+
+
+def test_starts_that_decrease_stay_inside(cuda):
+    """Not a batch that the call allows: two sequences have the same rows.  Each
+    row is one of theirs."""
+    G.note("decreasing starts")
+    lengths = [700, 650, 600, 640]
+    for dtype in DTYPES:
+        k, v, table = G.paged(2, lengths, 2, 64, 16, dtype, cuda, poison=False)
+        q = G.randn(G.gen_of(4), 40, 4, 64, dtype=dtype, device=cuda)
+        n, starts = i32(lengths, cuda), i32([0, 40, 0, 40, 20], cuda)
+        masks = torch.full((40, 1), -1, dtype=torch.int64, device=cuda)
+        out = A.paged_tree(q, k, v, table, n, starts, masks)
+        assert torch.isfinite(out).all()
