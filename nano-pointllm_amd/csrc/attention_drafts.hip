@@ -4,22 +4,35 @@
 // Mathematics.  As attention_decode.hip: S^T = K Q^T, P = 2^(S^T c - r), O^T = V^T P,
 // l = sum P, with the rows as columns; a masked key's score is -inf.
 //
-// Bound by memory: every key and value is read once per workgroup's rows.
+// Bound by memory: every key and value is read once per workgroup's 16 W rows, for up
+// to 64 rows.  4 trees of 64 behind 4032 keys of 32 heads (268 MB): 52 us and a join of
+// 5, 5.2 TB/s; one of 64 behind 16320: 51 us in all.  8 of 25 to 64 behind 630 to 1590
+// keys (169 MB) are 256 workgroups, of which the longest walks 26 steps: 39 us.  A
+// small call is bound by its launches: 26 rows of 32 heads behind 601 keys take 11 us
+// and the join 4.
 //
 // Design:
 //   * A workgroup takes 16 rows per wavefront of one key head, and a piece of the
 //     sequence's keys.  Units of 32 keys and values pass through a ring of kStages
 //     buffers in LDS, filled by LDS-DMA buffer loads straight from the pages, so that
-//     up to 48 KiB per workgroup are in flight without a register.  16-byte chunks
-//     are permuted by key (in the source address), which leaves the reads of both
-//     operands without bank conflicts.
+//     64 KiB per workgroup are in flight without a register (a wavefront that loads
+//     its keys itself, as decode does, has no room for 32 rows and the next keys: 54
+//     us for the 8 trees).  16-byte chunks are permuted by key (in the source
+//     address), which leaves the reads of both operands without bank conflicts.
+//   * Two sets of wavefronts (kParts) take every other unit for the same rows, and add
+//     up their sums at the end: alone on its SIMD a wavefront waits for each unit's
+//     operands, scores and sums in turn (8 trees: 43 us; one of 64 behind 16320 keys:
+//     57).
 //   * The scores' registers are the second product's operand as they are: its inner
 //     index is summed over, so the values are read (transposing) in the key order
 //     that the scores have.
 //   * Only the units that hold drafted keys have masks: 32 bits per row, loaded a unit
 //     ahead.
-//   * Work is cut by the keys there are, on the device, and joined in a second launch
-//     in a fixed order; batches that fill the card, and short tables, are not cut.
+//   * Work is cut by the keys there are, on the device, into kSlots workgroups and a
+//     few, one per CU (512: 66 instead of 57 us for the 4 trees), and joined in a
+//     second launch in a fixed order.  Batches that give every CU a workgroup are not
+//     cut while their tables are short (the 8 trees cut: 54 us), nor are short
+//     sequences.
 //   * Keys behind the sequence and of unknown pages arrive as zeros and are masked.  A
 //     masked key's probability is 0, but 0 times an infinite or NaN value is NaN: a
 //     row whose sums are not finite is computed again key by key.
@@ -38,14 +51,15 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef const int32_t __attribute__((address_space(4))) const_i32;   // scalar loads
 
 constexpr int kTile = 32;          // keys of a unit
-constexpr int kStages = 4;
+constexpr int kParts = 2;          // wavefronts of the same rows, on every other unit
+constexpr int kStages = 3;
 constexpr int kOutside = 0x7ffffff0;   // a buffer offset past every range
 constexpr int kBufferWord3 = 0x00020000;
 constexpr int kMinTiles = 4;       // least units of a workgroup of several
 constexpr int kWholeTiles = 10;    // sequences up to here are not cut
 constexpr int64_t kCus = 256;
 constexpr int64_t kWholeKeys = 2048;
-constexpr int kSlots = 512;        // workgroups aimed at
+constexpr int kSlots = 256;        // workgroups aimed at
 constexpr int kJoinThreads = 256;
 constexpr int kJoinAhead = 8;
 
@@ -227,10 +241,10 @@ template <int DP> __device__ inline int swizzle_v(int key) {
   return DP == 64 ? ((key >> 1) & 1) << 2 | ((key >> 2) & 3) : (key & 3) << 2 | ((key >> 2) & 3);
 }
 
-// DP: head_dim rounded up to 64 or 128.  W: wavefronts, of 16 rows each.  DMA: pages of
-// at least 8 keys; else each chunk is copied through registers.
+// DP: head_dim rounded up to 64 or 128.  W: wavefronts of each part, of 16 rows each.
+// DMA: pages of at least 8 keys; else each chunk is copied through registers.
 template <typename T, int DP, int W, bool DMA>
-__global__ __launch_bounds__(64 * W, W == 4 ? 2 : 1) void tree_kernel(TreeParams p) {
+__global__ __launch_bounds__(64 * W * kParts, W == 4 ? 2 : 1) void tree_kernel(TreeParams p) {
   constexpr int KS = DP / 32;               // first product: steps over the head
   constexpr int DV = DP / 16;               // second product: row tiles of O^T
   constexpr int R = 16 * W;
@@ -243,12 +257,14 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 2 : 1) void tree_kernel(TreeParams
   constexpr bool SPLIT = W <= 2;
   // Arrays of their own, so that the compiler sees that one is read while loads into
   // the others are in flight.
-  __shared__ __align__(16) char k0[UB], k1[UB], k2[UB], k3[UB], v0[UB], v1[UB], v2[UB], v3[UB];
-  __shared__ int odd_pages[W];
+  constexpr int SB = UB * kParts;           // a unit of each part
+  __shared__ __align__(16) char k0[SB], k1[SB], k2[SB], v0[SB], v1[SB], v2[SB];
+  __shared__ int odd_pages[W * kParts];
 
   const PagedAttention& a = p.a;
   const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int all_waves = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = all_waves % W, part_no = all_waves / W;
   const int r = lane & 15, g = lane >> 4;
   const int kvh = blockIdx.x % a.kv_heads;
   const int slot = blockIdx.x / a.kv_heads;
@@ -309,8 +325,8 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 2 : 1) void tree_kernel(TreeParams
 #pragma unroll
     for (int i = 0; i < GN; ++i) {
       const int key = t * kTile + first_key + 8 * i;
-      char* to_k = kd + (wave * GN + i) * GL * 1024;
-      char* to_v = vd + (wave * GN + i) * GL * 1024;
+      char* to_k = kd + part_no * UB + (wave * GN + i) * GL * 1024;
+      char* to_v = vd + part_no * UB + (wave * GN + i) * GL * 1024;
       if constexpr (DMA) {
         const int left = t < t1 ? keys - key : 0;
         const int page = __builtin_amdgcn_readfirstlane(e.page[i]);
@@ -365,21 +381,21 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 2 : 1) void tree_kernel(TreeParams
   const float sc = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * kLog2e;
 
   if (t0 < t1) {
-    copy(t0, lookup(t0), k0, v0);
-    copy(t0 + 1, lookup(t0 + 1), k1, v1);
-    copy(t0 + 2, lookup(t0 + 2), k2, v2);
-    Entries ahead = lookup(t0 + 3);
+    const int tf = t0 + part_no;   // the part's first unit
+    copy(tf, lookup(tf), k0, v0);
+    copy(tf + kParts, lookup(tf + kParts), k1, v1);
+    Entries ahead = lookup(tf + 2 * kParts);
 
     // Whether a page of these keys is unknown: then every unit looks its keys up.
     int odd = 0;
     {
       const int n = ((min(t1 * kTile, keys) - 1) >> a.page_shift) + 1;
-      for (int i = (t0 * kTile >> a.page_shift) + threadIdx.x; i < n; i += 64 * W) {
+      for (int i = (t0 * kTile >> a.page_shift) + threadIdx.x; i < n; i += 64 * W * kParts) {
         const int page = a.table[x.seq * a.ld_table + i];
         odd |= page < 0 || page >= pages;
       }
       const bool any = __any(odd);
-      if (lane == 0) odd_pages[wave] = any;
+      if (lane == 0) odd_pages[all_waves] = any;
     }
     u32x4 qf[KS];
     {
@@ -409,7 +425,7 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 2 : 1) void tree_kernel(TreeParams
       if (word >= 0 && word < p.words) words[0] = mask_row[word];
       if (word + 1 < p.words) words[1] = mask_row[word + 1];
     };
-    if (masked(t0)) load_mask(t0);
+    if (tf < t1 && masked(tf)) load_mask(tf);
 
     int read_k[2][KS], read_v[2];
 #pragma unroll
@@ -436,15 +452,17 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 2 : 1) void tree_kernel(TreeParams
 
     auto unit = [&](int t, char* kt, char* vt, char* kfree, char* vfree)
         __attribute__((always_inline)) {
+      kt += part_no * UB;
+      vt += part_no * UB;
       arrived();
-      if (t == t0) {
+      if (t == tf) {
 #pragma unroll
-        for (int w = 0; w < W; ++w) odd |= odd_pages[w];
+        for (int w = 0; w < W * kParts; ++w) odd |= odd_pages[w];
         odd = __builtin_amdgcn_readfirstlane(odd);
       }
-      copy(t + kStages - 1, ahead, kfree, vfree);
-      ahead = lookup(t + kStages);
-      if (!works) return;
+      copy(t + (kStages - 1) * kParts, ahead, kfree, vfree);
+      ahead = lookup(t + kStages * kParts);
+      if (!works || t >= t1) return;
       // All operands are read ahead, the values' while the scores become
       // probabilities.
       u32x4 kf[KS][2], vf[DV];
@@ -483,7 +501,7 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 2 : 1) void tree_kernel(TreeParams
           s[i >> 2][i & 3] =
               (bits >> ((i < 4 ? 0 : 16) + (i & 3))) & 1 ? s[i >> 2][i & 3] : -INFINITY;
       }
-      if (t + 1 < t1 && masked(t + 1)) load_mask(t + 1);
+      if (t + kParts < t1 && masked(t + kParts)) load_mask(t + kParts);
       float top = s[0][0];
 #pragma unroll
       for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i >> 2][i & 3]);
@@ -525,19 +543,47 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 2 : 1) void tree_kernel(TreeParams
         for (int d = 0; d < DV; ++d) o[d] = mfma_16x16x32<T>(vf[d], lo, o[d]);
       }
     };
-    int t = t0;
+    // Both parts take as many steps, for their barriers.
+    int t = tf;
+    const int end = t1 + part_no;
     while (true) {
-      unit(t, k0, v0, k3, v3);
-      if (++t >= t1) break;
+      unit(t, k0, v0, k2, v2);
+      if ((t += kParts) >= end) break;
       unit(t, k1, v1, k0, v0);
-      if (++t >= t1) break;
+      if ((t += kParts) >= end) break;
       unit(t, k2, v2, k1, v1);
-      if (++t >= t1) break;
-      unit(t, k3, v3, k2, v2);
-      if (++t >= t1) break;
+      if ((t += kParts) >= end) break;
     }
-    // No load into LDS outlives the workgroup.
+    // No load into LDS outlives the workgroup, nor meets what follows.
     __builtin_amdgcn_s_waitcnt(0x0f70);
+
+    // The second part's sums to the first, lane by lane.
+    __shared__ f32x2 rl[W][64];
+    __syncthreads();
+    if (part_no > 0) {
+#pragma unroll
+      for (int d = 0; d < DV; ++d)
+        *reinterpret_cast<f32x4*>((d < DV / 2 ? k0 : k1) +
+                                  ((wave * (DV / 2) + d % (DV / 2)) * 64 + lane) * 16) = o[d];
+      rl[wave][lane] = f32x2{ref, l};
+    }
+    __syncthreads();
+    if (part_no > 0) return;
+    const f32x2 other = rl[wave][lane];
+    const float next = fmaxf(ref, other[0]);
+    const float base = next == -INFINITY ? 0.0f : next;
+    const float f0 = exp2_hw(ref - base), f1 = exp2_hw(other[0] - base);
+    ref = next;
+    l = l * f0 + other[1] * f1;
+#pragma unroll
+    for (int d = 0; d < DV; ++d) {
+      const f32x4 y =
+          *reinterpret_cast<const f32x4*>((d < DV / 2 ? k0 : k1) +
+                                          ((wave * (DV / 2) + d % (DV / 2)) * 64 + lane) * 16);
+      o[d] = o[d] * f0 + y * f1;
+    }
+  } else if (part_no > 0) {
+    return;
   }
   if (!works) return;
 
@@ -668,9 +714,9 @@ hipError_t launch_w(const TreeParams& p, const Plan& x, hipStream_t st) {
   // To clear rows, a workgroup per key head without an item.
   const dim3 grid(static_cast<uint32_t>((x.items + (p.clear ? 1 : 0)) * heads));
   if (p.a.page_shift >= 3 && (p.a.c_tok << p.a.page_shift) < (int64_t{1} << 30))
-    hipLaunchKernelGGL((tree_kernel<T, DP, W, true>), grid, dim3(64 * W), 0, st, p);
+    hipLaunchKernelGGL((tree_kernel<T, DP, W, true>), grid, dim3(64 * W * kParts), 0, st, p);
   else
-    hipLaunchKernelGGL((tree_kernel<T, DP, W, false>), grid, dim3(64 * W), 0, st, p);
+    hipLaunchKernelGGL((tree_kernel<T, DP, W, false>), grid, dim3(64 * W * kParts), 0, st, p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || x.whole) return e;
   hipLaunchKernelGGL((tree_join_kernel<T, DP, 16 * W>),
@@ -687,6 +733,9 @@ template <typename T> hipError_t launch_t(const TreeParams& p, const Plan& x, hi
 
 }  // namespace
 
+// More rows than that have few keys per operation: they run as a prompt's, 128 rows to
+// a key (4 trees of 33 to 45 tokens, 32 heads over 8, behind 32768: 147 us, here 209; 8
+// of 48 behind 4048: 64 and 102; one of 64 behind 32704: 84 and 75).
 bool small_trees(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
                  int64_t head_dim) {
   const int64_t rows = tokens * (q_heads / kv_heads);
