@@ -37,6 +37,11 @@
 //     decides, by the table's width: of one wider than the sequences' lengths the
 //     joining launch may find nothing to do, and short sequences are cut that a
 //     narrow table would leave whole (kWholeKeys).
+//   * With a window and sinks (WINDOW) a sequence's tiles are those that hold a seen
+//     key, the sinks' and then the window's; the keys of the first and last of them that
+//     are not seen are masked like keys behind the length.  64 sequences of 229 to 8190
+//     keys of 8 heads, a window of 1024 (258 MB): 44 us, 5.9 TB/s; one of 131071 with a
+//     window of 4096: 8.0 us and 5.6 to join them.
 #include <algorithm>
 #include <type_traits>
 

@@ -6,6 +6,13 @@
 // log1p(R) + sum (m - x) exp(x - m) / (1 + R), all terms of one sign, so that a
 // row that is nearly decided keeps its digits.
 //
+// Bound by memory where there are rows for every CU: 2048 rows of 32003 binary32 logits
+// (262 MB) take 46 to 50 us, 5.2 to 5.7 TB/s.  16-bit logits are close to the vector
+// units' bound, about ten instructions an element, four cycles each and sixteen for the
+// exponential: 1024 rows of 128256 bfloat16 logits 61 us, 4.3 TB/s.  A few rows are bound
+// by one workgroup's way through them: 8 of 32003 take 6.5 us, with 5 top tokens 8.4, 20
+// 11, 64 16.
+//
 // Design:
 //   * A workgroup holds a row, or a slice of a long one, in registers: the logits
 //     are read once.  The sums run while later loads are in flight, against a
@@ -14,7 +21,9 @@
 //     adds its logits up again through LDS, with the maximum left out and counted.
 //   * Top tokens: the k-th largest of 128 groups' maxima bounds the k-th largest
 //     logit from below, and few logits reach it (k and some, rarely 2 k).  They go
-//     through LDS, in any order, and each counts those before it: its place.  Ties
+//     through LDS, in any order, and each counts those before it: its place (k rounds
+//     of the largest that is left, over the whole row, took 1 ms for 256 rows of
+//     128256 and k = 20, this 4 us).  Ties
 //     are broken by the token's number, so the order of arrival changes nothing.
 //     Where more than kMost reach the bound (a row of equal logits) the top tokens
 //     are found one by one.

@@ -18,7 +18,9 @@ Public surface:
   ``LightweightLlamaRunner`` on the W8A8 modules, capturable in a HIP graph.
 * :mod:`nanopointllm_amd.attention` - the runner's attention core: rotary
   positions, a paged key-value cache and attention over it, for prompts and
-  for single tokens.
+  for single tokens, with windows and sinks, and for trees of drafted tokens.
+* :mod:`nanopointllm_amd.lm_head` - the LM head at decode batches, and log
+  probabilities of given tokens with entropy and top tokens.
 * :mod:`nanopointllm_amd.calibration` - activation range collection, QDQ
   hooks, weight fake-quant and SmoothQuant smoothing.
 * :mod:`nanopointllm_amd.integer_epilogues` - the int32 -> int8
