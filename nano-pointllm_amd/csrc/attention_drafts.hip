@@ -72,6 +72,7 @@ struct TreeParams {
   bool whole;              // no sequence is cut
   bool clear;              // rows of no sequence become zeros
   int items;               // that the workspace has room for
+  int resident;            // workgroups that the card holds at a time
   float* part_o;           // [items x kv_heads, rows of a block, head_dim]
   f32x2* part_rl;          // [items x kv_heads, rows of a block]
 };
@@ -109,6 +110,9 @@ __device__ inline Item find_item(const TreeParams& p, int rows, int at, bool joi
     }
     return s;
   };
+  auto pieces_of = [](uint32_t tiles, uint32_t cut) {
+    return tiles <= kWholeTiles ? 1u : (tiles + cut - 1) / cut;
+  };
   const Seq first = read(lane);
   uint32_t cut = INT32_MAX;
   if (!p.whole) {
@@ -124,13 +128,34 @@ __device__ inline Item find_item(const TreeParams& p, int rows, int at, bool joi
           lane_value(scan64(static_cast<uint32_t>(min(share, uint64_t{1} << 25))), 63));
     }
     total = (total * a.kv_heads + kSlots - 1) / kSlots;
-    if (!much) cut = static_cast<uint32_t>(max(int64_t{kMinTiles}, min(total, int64_t{1} << 30)));
+    if (!much) {
+      cut = static_cast<uint32_t>(max(int64_t{kMinTiles}, min(total, int64_t{1} << 30)));
+      // Pieces rounded up may be more workgroups than the card holds, of which the last
+      // few would run by themselves: larger ones then, up to twice (3 trees of 40 behind
+      // 5960 keys of 32 heads: 59 us, else 83; 2 of 24 behind 9258 of 40 heads of 80: 66
+      // and 92; where lengths are uneven it may cost, 5 of 12 to 40 behind 3606 to 8960:
+      // 157 and 137).
+      const uint32_t least = cut;
+      for (int i = 0;; ++i) {
+        int64_t all = 0;
+        for (int b0 = 0; b0 < a.batch; b0 += 64) {
+          const Seq s = b0 == 0 ? first : read(b0 + lane);
+          all += static_cast<uint32_t>(lane_value(
+              scan64(pieces_of(s.tiles, cut) * static_cast<uint32_t>(s.blocks)), 63));
+        }
+        if (all * a.kv_heads <= p.resident) break;
+        if (i == 3) {
+          cut = least;
+          break;
+        }
+        cut += (cut + 3) / 4;
+      }
+    }
   }
   int items = 0, blocks = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
     const Seq s = b0 == 0 ? first : read(b0 + lane);
-    const uint32_t tiles = s.tiles;
-    const int pieces = tiles <= kWholeTiles ? 1 : static_cast<int>((tiles + cut - 1) / cut);
+    const int pieces = static_cast<int>(pieces_of(s.tiles, cut));
     const uint32_t own = pieces * s.blocks;
     const uint32_t upto = scan64(own);
     const uint32_t upto_blocks = scan64(s.blocks);
@@ -763,6 +788,7 @@ hipError_t launch_small_trees(const PagedAttention& a, const uint64_t* masks, in
   const Plan x = plan_of(a.tokens, a.batch, p.group, a.kv_heads, a.max_keys);
   p.whole = x.whole;
   p.items = static_cast<int>(x.items);
+  p.resident = static_cast<int>(a.head_dim <= 64 ? 3 * kCus : kCus);   // by their LDS
   char* ws = static_cast<char*>(a.workspace);
   p.part_rl = reinterpret_cast<f32x2*>(ws);
   p.part_o = reinterpret_cast<float*>(ws + pairs_bytes(x.items * a.kv_heads * x.rows));

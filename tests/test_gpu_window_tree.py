@@ -206,6 +206,14 @@ TREES = [
     (16, 16, 128, 16, [16, 7, 12], [1500, 1111, 64]), (32, 4, 64, 16, [2, 2, 1], [700, 33, 1]),
     (8, 1, 64, 16, [1 + 7 * i % 41 for i in range(70)], [50 + 11 * i % 60 for i in range(70)]),
     (200, 1, 64, 16, [3, 0, 70], [40, 9, 70]), (2, 2, 64, 8, [300], [305]),
+    # 33 to 64 rows, cut and whole, narrow heads, pages copied through registers
+    (3, 3, 64, 16, [40, 64, 33], [2500, 700, 40]), (4, 2, 80, 8, [32, 20], [3000, 1501]),
+    (2, 2, 128, 4, [50, 64, 7], [1000, 65, 640]), (2, 2, 96, 2, [9, 14], [600, 700]),
+    (64, 64, 64, 32, [36, 64, 40, 50], [500, 64, 333, 600]),
+    # more sequences than a wavefront has lanes, cut and whole
+    (2, 2, 64, 16, [i % 4 for i in range(90)], [i % 4 + 13 * i % 700 for i in range(90)]),
+    (4, 4, 128, 64, [1 + i % 9 for i in range(130)], [9 + 7 * i % 300 for i in range(130)]),
+    (4, 2, 128, 16, [5, 17, 1], [20000, 9000, 70]),
 ]
 
 
