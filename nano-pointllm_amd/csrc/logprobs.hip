@@ -42,6 +42,7 @@ constexpr int kGroups = 128;       // maxima that the bound is taken from
 constexpr int kFewHolders = 4;     // threads of a wavefront whose logits are spread over it
 constexpr int kRankers = 8;        // threads that count those before one of many candidates
 constexpr int kFew = 24;
+constexpr int kMany = 256;         // candidates that are thinned out before they are ranked
 constexpr float kSlack = 8.0f;     // in powers of two
 constexpr float kLn2 = 0.693147180559945309417f;
 constexpr int kJoinThreads = 256;
@@ -397,7 +398,44 @@ __global__ __launch_bounds__(64 * W, NV > 8 ? 4 : NV > 4 ? 6 : 8) void logprobs_
     else
       ranks[static_cast<int64_t>(blockIdx.x) * p.top + place] = rank;
   };
-  const int n = count;
+  int n = count;
+  if (n > kMany && n <= kMost) {
+    // Few groups hold a logit, or many logits are equal: the candidates from the
+    // top-th largest rank on, found bit by bit, are `top` exactly.
+    if (wave == 0) {
+      uint64_t mine[kMost / 64];
+#pragma unroll
+      for (int i = 0; i < kMost / 64; ++i) mine[i] = lane + 64 * i < n ? found[lane + 64 * i] : 0;
+      // Bits that are the same in all of them are known.
+      const uint64_t any = found[0];
+      uint64_t differ = 0;
+#pragma unroll
+      for (int i = 0; i < kMost / 64; ++i) differ |= lane + 64 * i < n ? mine[i] ^ any : 0;
+#pragma unroll
+      for (int w = 1; w < 64; w <<= 1)
+        differ |= __shfl_xor(static_cast<unsigned long long>(differ), w);
+      uint64_t t = any & ~differ;
+#pragma unroll 1
+      for (int bit = 63; bit >= 0; --bit) {
+        if (!((differ >> bit) & 1)) continue;
+        // Above this bit t is the rank's own, below it the least with the known bits.
+        const uint64_t next = (t | uint64_t{1} << bit) & (~uint64_t{0} << bit);
+        int reach = 0;
+#pragma unroll
+        for (int i = 0; i < kMost / 64; ++i) reach += __popcll(__ballot(mine[i] >= next));
+        if (reach >= p.top) t |= uint64_t{1} << bit;
+      }
+      uint32_t kept = 0;
+#pragma unroll
+      for (int i = 0; i < kMost / 64; ++i) {
+        const uint64_t in = __ballot(mine[i] >= t);
+        if (mine[i] >= t) found[kept + __popcll(in & ((uint64_t{1} << lane) - 1))] = mine[i];
+        kept += __popcll(in);
+      }
+    }
+    n = p.top;
+    __syncthreads();
+  }
   if (n <= kMost) {
     rank_all(found, n, tid, N, [&](int place, uint64_t rank) {
       if (place < p.top) write(place, rank);

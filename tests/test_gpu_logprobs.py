@@ -79,6 +79,8 @@ SHAPES = [
     (1, 50257, 0, 1), (2, 65536, 0, 20), (2, 65537, 0, 3), (3, 128256, 4, 20),
     (1, 131073, 0, 64), (2, 262144, 0, 10), (1, 1 << 20, 2, 64), (700, 300, 0, 4),
     (2500, 40, 0, 0), (300, 4097, 2, 2),
+    # few groups of threads hold a logit: hundreds of candidates
+    (67, 1004, 0, 64), (3, 700, 2, 64), (5, 520, 0, 40), (2, 420, 0, 64),
 ]
 
 
@@ -118,7 +120,7 @@ def test_rows_at_any_alignment(cuda, offset, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("vocab", [40, 5000, 70000, 300000])
+@pytest.mark.parametrize("vocab", [40, 600, 1000, 5000, 70000, 300000])
 def test_ties_and_special_rows(cuda, vocab, dtype):
     """Equal logits (the lowest token first), zeros of both signs, fewer finite
     logits than asked for, rising and falling rows, NaN, infinities, and rows of
