@@ -357,7 +357,7 @@ def _tree_workspace(tokens: int, batch: int, heads: int, kv_heads: int, dim: int
 
 
 def _window(window: int | None, sinks: int) -> None:
-    if type(sinks) is not int or sinks < 0:
+    if type(sinks) is not int or not 0 <= sinks < 1 << 62:
         raise ValueError("sinks must be a whole number of at least 0")
     if window is None:
         if sinks:

@@ -55,6 +55,14 @@ def test_state_of_drafts():
 
 
 # ------------------------------------------------------- refusals in Python
+@pytest.mark.parametrize("window,sinks", [(8, 2 ** 64), (8, 2 ** 64 + 3), (2 ** 64 + 8, 2)])
+def test_numbers_past_64_bits_are_refused(window, sinks):
+    """Not cut to their lower bits."""
+    cache = A.PagedKVCache(1, 1, 1, 64, device="cpu")
+    with pytest.raises(ValueError, match="sinks" if sinks > 8 else "window"):
+        A.PagedAttentionCore(cache, None, window=window, sinks=sinks)
+
+
 def test_windows_refused():
     cache = A.PagedKVCache(2, 1, 1, 64, device="cpu")
     for window, sinks, message in ((0, 0, "window"), (-3, 0, "window"), (2.0, 0, "window"),

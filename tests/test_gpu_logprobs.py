@@ -192,3 +192,29 @@ def test_captured_and_on_another_stream(cuda):
         got = L.token_logprobs(x, tokens, top=7)
     side.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_empty_calls(cuda):
+    G.note("logprobs empty")
+    x = torch.zeros(0, 50, device=cuda)
+    out = L.token_logprobs(x, torch.zeros(0, dtype=torch.int64, device=cuda), top=2)
+    assert out.logprobs.shape == out.entropy.shape == (0,) and out.top_tokens.shape == (0, 2)
+    x = rows_of(1, 3, 50, torch.float16, cuda)
+    out = L.token_logprobs(x, torch.zeros(3, 0, dtype=torch.int64, device=cuda), top=2)
+    assert out.logprobs.shape == (3, 0)
+    want = L.token_logprobs(x, torch.zeros(3, dtype=torch.int64, device=cuda), top=2)
+    assert all(torch.equal(a, b) for a, b in zip(out[1:], want[1:]))
+
+
+@pytest.mark.parametrize("vocab", [5000, 200000])
+def test_offsets_past_32_bits(cuda, vocab):
+    """Rows 2^31 logits apart, the last more than 2^32 behind the first."""
+    G.note(f"logprobs far rows {vocab}")
+    apart = (1 << 31) + 24
+    store = torch.empty(2 * apart + vocab, dtype=torch.bfloat16, device=cuda)
+    x = store.as_strided((3, vocab), (apart, 1))
+    near = rows_of(4, 3, vocab, torch.bfloat16, cuda)
+    x.copy_(near)
+    tokens = torch.randint(0, vocab, (3, 4), generator=G.gen_of(1)).to(cuda)
+    got, want = (L.token_logprobs(y, tokens, top=9) for y in (x, near))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -407,3 +407,143 @@ def test_starts_that_decrease_stay_inside(cuda):
         masks = torch.full((40, 1), -1, dtype=torch.int64, device=cuda)
         out = A.paged_tree(q, k, v, table, n, starts, masks)
         assert torch.isfinite(out).all()
+
+
+# few rows of a sequence, in one piece and in several; many rows
+NEW = [[9, 3], [40, 1], [200, 30]]
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 2.0])
+@pytest.mark.parametrize("new", NEW)
+def test_given_scales(cuda, new, scale):
+    G.note(f"scale {scale} {new}")
+    lengths, dtype = [900, 230], torch.float16
+    k, v, table = G.paged(5, lengths, 2, 64, 16, dtype, cuda)
+    n, starts = i32(lengths, cuda), i32([0, new[0], sum(new)], cuda)
+    q = G.randn(G.gen_of(1), sum(new), 4, 64, dtype=dtype, device=cuda)
+    masks = A.tree_masks(random_trees(3, new), device=cuda)
+    out = A.paged_tree(q, k, v, table, n, starts, masks, scale=scale)
+    check(out, q, k, v, table, n, starts, lambda b, c, t: O.tree_sight(
+        masks[int(starts[b]):int(starts[b + 1])].cpu(), t), scale=scale)
+
+    def sight(b, rows, total):
+        return O.window_sight(rows, total, 77, 3)
+
+    out = A.paged_prefill(q, k, v, table, n, starts, scale=scale, window=77, sinks=3)
+    check(out, q, k, v, table, n, starts, sight, scale=scale)
+    out = A.paged_decode(q[:2], k, v, table, n, scale=scale, window=77, sinks=3)
+    check(out, q[:2], k, v, table, n, torch.arange(3), sight, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new", NEW)
+def test_sharp_and_flat_rows(cuda, new, dtype):
+    """Scores hundreds apart, all equal, a first key far above or far below the
+    rest, and a drafted key that takes all where it is seen."""
+    G.note(f"sharp trees {new} {dtype}")
+    lengths = [900, 230]
+    k, v, table = G.paged(9, lengths, 1, 64, 16, dtype, cuda, poison=False)
+    q = G.randn(G.gen_of(3), sum(new), 4, 64, dtype=dtype, device=cuda)
+    first = k[table[0, 0].long(), 0, 0]
+    first *= 8.0
+    place = lengths[0] - new[0] + 1
+    drafted = k[table[0, place // 16].long(), 0, place % 16]
+    drafted *= 8.0
+    q[0] *= 60.0
+    q[1], q[2], q[3], q[4] = 0.0, first * 0.5, -first * 0.5, drafted * 0.5
+    q[5], q[6] = drafted * 0.5, -drafted * 0.5
+    n, starts = i32(lengths, cuda), i32([0, new[0], sum(new)], cuda)
+    masks = A.tree_masks(random_trees(3, new), device=cuda)
+    masks[4] |= 2
+    masks[5] &= ~2
+    out = A.paged_tree(q, k, v, table, n, starts, masks)
+    check(out, q, k, v, table, n, starts, lambda b, c, t: O.tree_sight(
+        masks[int(starts[b]):int(starts[b + 1])].cpu(), t))
+    out = A.paged_prefill(q, k, v, table, n, starts, window=100, sinks=1)
+    check(out, q, k, v, table, n, starts, lambda b, c, t: O.window_sight(c, t, 100, 1))
+
+
+@pytest.mark.parametrize("new", NEW)
+def test_lengths_past_the_table_are_cut(cuda, new):
+    G.note(f"long lengths {new}")
+    k, v, table = G.paged(7, [640, 640], 2, 64, 16, torch.float16, cuda)
+    table = table[:, :40]
+    q = G.randn(G.gen_of(2), sum(new), 4, 64, dtype=torch.float16, device=cuda)
+    masks = A.tree_masks(random_trees(3, new), device=cuda)
+    starts = i32([0, new[0], sum(new)], cuda)
+    for given, cut in ([2 ** 31 - 1, -5], [640, 0]), ([10 ** 9, 641], [640, 640]):
+        n, m = i32(given, cuda), i32(cut, cuda)
+        out = A.paged_tree(q, k, v, table, n, starts, masks)
+        assert torch.equal(out, A.paged_tree(q, k, v, table, m, starts, masks))
+        check(out, q, k, v, table, m, starts, lambda b, c, t: O.tree_sight(
+            masks[int(starts[b]):int(starts[b + 1])].cpu(), t))
+        assert torch.equal(A.paged_prefill(q, k, v, table, n, starts, window=70, sinks=2),
+                           A.paged_prefill(q, k, v, table, m, starts, window=70, sinks=2))
+        assert torch.equal(A.paged_decode(q[:2], k, v, table, n, window=70, sinks=2),
+                           A.paged_decode(q[:2], k, v, table, m, window=70, sinks=2))
+
+
+def test_empty_calls(cuda):
+    G.note("empty")
+    k, v, table = G.paged(7, [64], 2, 64, 16, torch.float16, cuda)
+    none = torch.empty(0, 4, 64, dtype=torch.float16, device=cuda)
+    no_rows = torch.zeros(0, 1, dtype=torch.int64, device=cuda)
+    no_seqs, n, zero = i32([], cuda), i32([64], cuda), i32([0, 0], cuda)
+    assert A.paged_decode(none, k, v, table[:0], no_seqs, window=3, sinks=1).shape == none.shape
+    assert A.paged_prefill(none, k, v, table, n, zero, window=3, sinks=1).shape == none.shape
+    assert A.paged_tree(none, k, v, table, n, zero, no_rows).shape == none.shape
+    kept = k.clone(), v.clone()
+    A.paged_accept(k, v, table[:0], no_seqs, torch.zeros(0, 3, dtype=torch.int32, device=cuda))
+    A.paged_accept(k, v, table, n, torch.zeros(1, 0, dtype=torch.int32, device=cuda))
+    A.paged_accept(k, v, table[:, :0], n, i32([[1, 2]], cuda))
+    A.paged_accept(k[:0], v[:0], table, n, i32([[1, 2]], cuda))
+    for now, then in zip((k, v), kept):
+        assert torch.equal(now.view(torch.int16), then.view(torch.int16))
+    # Rows of no sequence, no page, no sequence.
+    q = torch.ones(3, 4, 64, dtype=torch.float16, device=cuda)
+    masks = torch.full((3, 1), -1, dtype=torch.int64, device=cuda)
+    for rows, seqs, pages in ((zero, n, table), (i32([0, 3], cuda), n, table[:, :0]),
+                              (i32([0], cuda), no_seqs, table[:0])):
+        assert (A.paged_tree(q, k, v, pages, seqs, rows, masks) == 0).all()
+        assert (A.paged_prefill(q, k, v, pages, seqs, rows, window=2) == 0).all()
+    assert (A.paged_tree(q, k[:0], v[:0], table, n, i32([0, 3], cuda), masks) == 0).all()
+
+
+def test_offsets_past_32_bits(cuda):
+    """Pages more than 2^32 elements into the cache, and layers as far apart."""
+    G.note("far pages")
+    g, page, d, dtype = 2, 64, 128, torch.bfloat16
+    pages = (1 << 32) // (g * page * d) + 40
+    store = torch.empty(1, 2, pages, g, page, d, dtype=dtype, device=cuda)
+    k, v = store[0]
+    lengths, r = [150, 70], G.gen_of(5)
+    table = i32([[pages - 1, 3, pages - 30], [pages - 7, pages - 2, -1]], cuda)
+    at = table.flatten()[:5].long()
+    for c in (k, v):
+        c[at] = G.randn(r, 5, g, page, d, dtype=dtype, device=cuda)
+    small = i32([[0, 1, 2], [3, 4, -1]], cuda)
+    ks, vs, n = k[at], v[at], i32(lengths, cuda)
+    for new in ([20, 9], [140, 60]):
+        q = G.randn(r, sum(new), 4, d, dtype=dtype, device=cuda)
+        starts = i32([0, new[0], sum(new)], cuda)
+        masks = A.tree_masks(random_trees(3, new), device=cuda)
+        assert torch.equal(A.paged_tree(q, k, v, table, n, starts, masks),
+                           A.paged_tree(q, ks, vs, small, n, starts, masks))
+        assert torch.equal(A.paged_prefill(q, k, v, table, n, starts, window=30, sinks=2),
+                           A.paged_prefill(q, ks, vs, small, n, starts, window=30, sinks=2))
+        assert torch.equal(A.paged_decode(q[:2], k, v, table, n, window=30, sinks=2),
+                           A.paged_decode(q[:2], ks, vs, small, n, window=30, sinks=2))
+    before, path = i32([100, 62], cuda), i32([[3, 30, 49], [0, 5, -1]], cuda)
+    A.paged_accept(store[:, 0], store[:, 1], table, before, path)
+    A.paged_accept(ks, vs, small, before, path)
+    assert torch.equal(k[at], ks) and torch.equal(v[at], vs)
+    # One page per layer, the layers far apart.
+    layers = store.flatten()[:2 << 32].view(2, 1 << 32)[:, :2 * g * page * d]
+    layers = layers.view(2, 2, 1, g, page, d)
+    layers.copy_(G.randn(r, *layers.shape, dtype=dtype, device=cuda))
+    near = layers.contiguous()
+    assert layers.stride(0) == 1 << 32 and near.stride(0) < 1 << 32
+    for c in (layers, near):
+        A.paged_accept(c[:, 0], c[:, 1], i32([[0]], cuda), i32([9], cuda), i32([[2, 5]], cuda))
+    assert torch.equal(layers, near) and not torch.equal(near[1, 0, 0, :, 9], near[1, 0, 0, :, 10])
+    assert torch.equal(near[1, 0, 0, :, 9], near[1, 0, 0, :, 11])
