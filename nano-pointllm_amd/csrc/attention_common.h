@@ -79,6 +79,12 @@ __device__ inline uint32_t round2(float p0, float p1, float& l) {
   }
 }
 
+// s where bit k of bits is set, else -inf: two instructions.
+__device__ inline float shown_or_minus_infinity(float s, uint32_t bits, int k) {
+  const uint32_t m = static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(bits), k, 1));
+  return __uint_as_float((__float_as_uint(s) & m) | (0xff800000u & ~m));
+}
+
 // Inclusive sum over the wavefront's lanes (each step a DPP move: shifts by 1,
 // 2, 4 and 8 in rows of 16 lanes, then the rows' last lanes to the next ones).
 __device__ inline uint32_t scan64(uint32_t v) {

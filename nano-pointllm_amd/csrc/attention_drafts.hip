@@ -524,7 +524,7 @@ __global__ __launch_bounds__(64 * W * kParts, W == 4 ? 2 : 1) void tree_kernel(T
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           s[i >> 2][i & 3] =
-              (bits >> ((i < 4 ? 0 : 16) + (i & 3))) & 1 ? s[i >> 2][i & 3] : -INFINITY;
+              shown_or_minus_infinity(s[i >> 2][i & 3], bits, (i < 4 ? 0 : 16) + (i & 3));
       }
       if (t + kParts < t1 && masked(t + kParts)) load_mask(t + kParts);
       float top = s[0][0];

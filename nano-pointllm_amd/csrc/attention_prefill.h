@@ -677,31 +677,24 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) void prefill_kernel
       const int key0 = units.key(i);
       const bool left_out = S == Seen::kWindow && key0 < low_last && key0 + kKeys > p.sinks;
       if (key0 + kKeys - 1 > seen_first || left_out || odd != 0) {
-        uint32_t shown = 0xffffu;
+        // Bit k: the lane's key k is seen.
+        auto below = [](int n) { return n >= kKeys ? ~0u : (1u << max(n, 0)) - 1u; };
+        uint32_t bits = below(seen - key0 + 1);
+        if constexpr (S == Seen::kTree) bits &= drafted_bits(key0 - cached);
+        if constexpr (S == Seen::kWindow) bits &= ~below(low - key0) | below(p.sinks - key0);
+        bits >>= 4 * h;
         if (odd != 0) {
 #pragma unroll 1
           for (int n = 0; n < 16; ++n) {
             const int key = key0 + 8 * (n >> 2) + 4 * h + (n & 3);
             int page = 0;
             if (key < at.keys) page = a.table[at.seq * a.ld_table + (key >> a.page_shift)];
-            if (page < 0 || page >= pages) shown &= ~(1u << n);
+            if (page < 0 || page >= pages) bits &= ~(1u << (8 * (n >> 2) + (n & 3)));
           }
         }
-        const int left = seen - key0 - 4 * h;
-        // Seen::kWindow, Seen::kTree: bit k of the lane's keys k.
-        uint32_t bits = 0;
-        if constexpr (S == Seen::kTree) bits = drafted_bits(key0 - cached) >> (4 * h);
-        if constexpr (S == Seen::kWindow) {
-          auto below = [](int n) { return n >= kKeys ? ~0u : (1u << max(n, 0)) - 1u; };
-          bits = (~below(low - key0) | below(p.sinks - key0)) >> (4 * h);
-        }
 #pragma unroll
-        for (int n = 0; n < 16; ++n) {
-          const int k = 8 * (n >> 2) + (n & 3);
-          bool there = k <= left && ((shown >> n) & 1);
-          if constexpr (S != Seen::kCausal) there = there && ((bits >> k) & 1);
-          s[n] = there ? s[n] : -INFINITY;
-        }
+        for (int n = 0; n < 16; ++n)
+          s[n] = shown_or_minus_infinity(s[n], bits, 8 * (n >> 2) + (n & 3));
       }
       float top = s[0];
 #pragma unroll
