@@ -38,7 +38,9 @@
 //     are: its inner index is summed over, so the values are read (transposing
 //     ds_read_b64_tr_b16) in the key order that the scores have.
 //   * Masks are formed for the units that a row of the wavefront sees in part,
-//     the last ones; the others have none.
+//     the last ones; the others have none.  They are a word of bits, of which each
+//     score takes its own in two instructions (compared one by one: 560 tokens with a
+//     window of 256 keys 21.7 instead of 18.7 us, without one 21.2 instead of 20.1).
 //   * Few rows far into a long cache are cut over its length: each piece
 //     leaves (O, r, l) in the workspace and prefill_join_kernel adds them up.
 //     Whether there may be pieces the host decides by the table's width: 560

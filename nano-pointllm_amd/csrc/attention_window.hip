@@ -5,8 +5,9 @@
 // Bound as a prompt without a window: 16384 tokens of 32 heads over 8 with a window of
 // 4096 take 0.99 to 1.04 ms (0.93 to 0.98 PFLOP/s of what is seen), 5 of the 131 units
 // of a row tile with masks.  A short prompt is one row tile's units in a row: 560 tokens
-// of 32 heads take 13.9 us with a window of 32 keys, 17.2 with 128, 21.3 with 256, and
-// 20.7 with one of 559.
+// of 32 heads take 12.5 us with a window of 32 keys, 14.9 with 128, 17.8 with 256, and
+// 19.7 with one of 559; 10 of the 13 units of a window of 256 have masks, which cost
+// about 0.25 us each on top of a unit's 0.55.
 #include "attention_prefill.h"
 
 namespace w8a8 {
