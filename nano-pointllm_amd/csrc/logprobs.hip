@@ -318,7 +318,7 @@ __global__ __launch_bounds__(64 * W, NV > 8 ? 4 : NV > 4 ? 6 : 8) void logprobs_
     const float t = (ref - m) * kLog2e, f = exp2_hw(t);
     const bool nan = sum != sum;
     spread = sum == 0.0f || f == 0.0f ? 0.0f : -(spread + t * sum) * f * kLn2;
-    sum *= f;
+    sum = sum == 0.0f ? 0.0f : sum * f;   // f may be infinite for a thread without logits
     uint64_t holders = __ballot(top == peak && top > -INFINITY && !nan);
     if (top == peak && top > -INFINITY && !nan) sum = spread = 0.0f;
     while (holders != 0) {

@@ -218,3 +218,19 @@ def test_offsets_past_32_bits(cuda, vocab):
     tokens = torch.randint(0, vocab, (3, 4), generator=G.gen_of(1)).to(cuda)
     got, want = (L.token_logprobs(y, tokens, top=9) for y in (x, near))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab,top", [(3, 40, 3), (4, 1300, 20), (5, 32003, 5), (3, 140003, 64),
+                                            (2, 300000, 0)])
+def test_rows_far_from_zero(cuda, rows, vocab, top, dtype):
+    """All of a row's logits far below or above zero, with and without masked
+    tokens, where some threads have none."""
+    G.note(f"logprobs far {rows} {vocab} {top} {dtype}")
+    g = G.gen_of(vocab)
+    tokens = torch.randint(0, vocab, (rows,), generator=g)
+    for shift in (-90.0, -700.0, -60000.0, 700.0, 60000.0):
+        x = (torch.randn(rows, vocab, generator=g) + shift).to(dtype)
+        x[0, 3:] = -math.inf
+        x[1] = x[1, 0]
+        check(L.token_logprobs(x.to(cuda), tokens.to(cuda), top=top), x, tokens, top)
