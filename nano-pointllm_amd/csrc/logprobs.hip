@@ -18,15 +18,20 @@
 //     are read once.  The sums run while later loads are in flight, against a
 //     reference per thread that is the maximum so far or up to kSlack below.
 //   * The thread whose logit is the row's maximum leaves its sums: its wavefront
-//     adds its logits up again through LDS, with the maximum left out and counted.
+//     adds its logits up again through LDS, with the maximum left out and counted
+//     (of many such threads each reads its own again: 2048 rows of 32003 zeros 238
+//     instead of 488 us).
 //   * Top tokens: the k-th largest of 128 groups' maxima bounds the k-th largest
 //     logit from below, and few logits reach it (k and some, rarely 2 k).  They go
 //     through LDS, in any order, and each counts those before it: its place (k rounds
 //     of the largest that is left, over the whole row, took 1 ms for 256 rows of
 //     128256 and k = 20, this 4 us).  Ties
 //     are broken by the token's number, so the order of arrival changes nothing.
-//     Where more than kMost reach the bound (a row of equal logits) the top tokens
-//     are found one by one.
+//     Where more than kMost reach the bound (equal logits, masked ones at the type's
+//     lowest value) the maxima of all threads give a better one, and of logits equal
+//     to that the first tokens are counted off: 256 rows of 128256 zeros, 20 top
+//     tokens, 106 us (one by one, as what is left after that is found, 1060), 8 rows of
+//     32003 of which all but 3 are masked, 64 top tokens, 41 us (780).
 //   * Rows of more vectors than a workgroup holds are cut into equal slices, whose
 //     sums and top tokens a second launch joins.
 #include <algorithm>
@@ -111,15 +116,15 @@ __device__ inline uint64_t wave_max64(uint64_t x) {
   return x;
 }
 
-// The k-th largest of kGroups orders, to its upper 16 bits, rounded down.
-__device__ inline uint32_t kth_order(const uint32_t (&g)[kGroups / 64], int k) {
+// The k-th largest of 64 M orders, to its bits from LOW on, rounded down.
+template <int LOW, int M> __device__ inline uint32_t kth_order(const uint32_t (&g)[M], int k) {
   uint32_t t = 0;
 #pragma unroll 1
-  for (int bit = 31; bit >= 16; --bit) {
+  for (int bit = 31; bit >= LOW; --bit) {
     const uint32_t next = t | 1u << bit;
     int n = 0;
 #pragma unroll
-    for (int i = 0; i < kGroups / 64; ++i) n += __popcll(__ballot(g[i] >= next));
+    for (int i = 0; i < M; ++i) n += __popcll(__ballot(g[i] >= next));
     if (n >= k) t = next;
   }
   return t;
@@ -285,7 +290,7 @@ __global__ __launch_bounds__(64 * W, NV > 8 ? 4 : NV > 4 ? 6 : 8) void logprobs_
     uint32_t g[kGroups / 64];
 #pragma unroll
     for (int i = 0; i < kGroups / 64; ++i) g[i] = group[lane + 64 * i];
-    const uint32_t t = kth_order(g, p.top);
+    const uint32_t t = kth_order<16>(g, p.top);
     if (lane == 0) bound = t;
   }
 
@@ -311,6 +316,27 @@ __global__ __launch_bounds__(64 * W, NV > 8 ? 4 : NV > 4 ? 6 : 8) void logprobs_
     __builtin_amdgcn_wave_barrier();
   };
 
+  // The thread's logits from memory again, f(logit, token) of each in vectors of which
+  // one is wanted (in a loop that keeps no registers for them).
+  auto each_again = [&](auto wanted, auto f) __attribute__((always_inline)) {
+    auto look = [&](int vector) {
+#pragma unroll 1
+      for (int j = 0; j < E; ++j) {
+        const int token = vector * E - skew + j;
+        if (token >= 0 && token < p.vocab) f(to_f32(x[token]), token);
+      }
+    };
+#pragma unroll 1
+    for (int i = v0 + tid; i < v1; i += N) {
+      const u32x4 v = vectors[i];
+      bool any = false;
+#pragma unroll
+      for (int j = 0; j < E; ++j) any = any || wanted(element<T>(v, j));
+      if (any) look(i);
+    }
+    if (lone >= 0) look(lone);
+  };
+
   const float m = peak == -INFINITY ? 0.0f : peak;
   float equal = 0.0f;
   {
@@ -319,20 +345,27 @@ __global__ __launch_bounds__(64 * W, NV > 8 ? 4 : NV > 4 ? 6 : 8) void logprobs_
     const bool nan = sum != sum;
     spread = sum == 0.0f || f == 0.0f ? 0.0f : -(spread + t * sum) * f * kLn2;
     sum = sum == 0.0f ? 0.0f : sum * f;   // f may be infinite for a thread without logits
-    uint64_t holders = __ballot(top == peak && top > -INFINITY && !nan);
-    if (top == peak && top > -INFINITY && !nan) sum = spread = 0.0f;
-    while (holders != 0) {
-      const int from = __ffsll(static_cast<unsigned long long>(holders)) - 1;
-      holders &= holders - 1;
-      spread_out(from, [&](float y, int) {
-        const float d = y - m, e = exp2_hw(d * kLog2e);
-        if (d == 0.0f) {
-          equal += 1.0f;
-        } else {
-          sum += e;
-          spread -= fmaxf(d, -200.0f) * e;
-        }
-      });
+    const bool holds = top == peak && top > -INFINITY && !nan;
+    uint64_t holders = __ballot(holds);
+    if (holds) sum = spread = 0.0f;
+    auto add = [&](float y, int) {
+      const float d = y - m, e = exp2_hw(d * kLog2e);
+      if (d == 0.0f) {
+        equal += 1.0f;
+      } else {
+        sum += e;
+        spread -= fmaxf(d, -200.0f) * e;
+      }
+    };
+    if (__popcll(holders) > kFewHolders) {
+      // Many equal ones: each reads its own again.
+      if (holds) each_again([](float) { return true; }, add);
+    } else {
+      while (holders != 0) {
+        const int from = __ffsll(static_cast<unsigned long long>(holders)) - 1;
+        holders &= holders - 1;
+        spread_out(from, add);
+      }
     }
     const float s = wave_sum(sum), d = wave_sum(spread), n = wave_sum(equal);
     if (lane == 0) {
@@ -360,10 +393,12 @@ __global__ __launch_bounds__(64 * W, NV > 8 ? 4 : NV > 4 ? 6 : 8) void logprobs_
   if (p.top == 0) return;
 
   // The bound's own order may be that of a NaN's bits below -inf.
-  const float least = p.top == 1 ? peak : bound <= 0x007fffffu ? -INFINITY : value_of(bound);
+  float least = p.top == 1 ? peak : bound <= 0x007fffffu ? -INFINITY : value_of(bound);
   // Of the tokens at -inf only the first `top` can be among the top ones.
+  bool above = false;   // and those at the bound are none
+  auto below = [&](float y) { return y < least || (above && y == least); };
   auto offer = [&](float y, int token) {
-    if (y < least || (y == -INFINITY && token >= first_token + p.top)) return;
+    if (below(y) || (y == -INFINITY && token >= first_token + p.top)) return;
     const int at = atomicAdd(&count, 1);
     if (at < kMost) found[at] = rank_of(y, token);
   };
@@ -399,6 +434,57 @@ __global__ __launch_bounds__(64 * W, NV > 8 ? 4 : NV > 4 ? 6 : 8) void logprobs_
       ranks[static_cast<int64_t>(blockIdx.x) * p.top + place] = rank;
   };
   int n = count;
+  const int last_token = slices == 1 ? p.vocab : max(v1 * E - skew, first_token);
+  // The first of several slices has the row's last tokens too.
+  const int more = slices > 1 && slice == 0 ? p.vocab - (full1 * E - skew) : 0;
+  auto nth_token = [&](int i) { return i < last_token ? i : i - last_token + full1 * E - skew; };
+  // Rare: too many candidates, where few groups hold a logit or masked logits are the
+  // type's lowest value.  Those from the top-th largest maximum of a thread on, then,
+  // where too many are equal to that, those above it and its first tokens.  The slice
+  // is read again (kept in registers for this, it does not fit them).
+  for (int round = 1; n > kMost && round <= 2; ++round) {
+    __syncthreads();
+    if (round == 1) {
+      uint32_t* maxima = reinterpret_cast<uint32_t*>(found);
+      maxima[tid] = order_of(top);
+      __syncthreads();
+      if (wave == 0) {
+        uint32_t g[W];
+#pragma unroll
+        for (int i = 0; i < W; ++i) g[i] = maxima[lane + 64 * i];
+        const uint32_t t = kth_order<0>(g, p.top);
+        if (lane == 0) bound = t;
+      }
+    }
+    if (tid == 0) count = 0;
+    __syncthreads();
+    least = value_of(bound);
+    above = round == 2;
+    // (No more than that they are too many is to be known.)
+    if (!below(top) || odd)
+      each_again([&](float y) { return !below(y) && *static_cast<volatile int*>(&count) <= kMost; },
+                 offer);
+    __syncthreads();
+    n = count;
+  }
+  if (above && n < p.top) {
+    for (int i0 = first_token; n < p.top && i0 < last_token + more; i0 += N) {
+      const int i = i0 + tid, token = nth_token(i);
+      const bool equal = i < last_token + more && to_f32(x[token]) == least;
+      const uint64_t in = __ballot(equal);
+      if (lane == 0) best[wave] = __popcll(in);
+      __syncthreads();
+      int at = n + __popcll(in & ((uint64_t{1} << lane) - 1)), upto = n;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        if (w < wave) at += static_cast<int>(best[w]);
+        upto += static_cast<int>(best[w]);
+      }
+      if (equal && at < p.top) found[at] = rank_of(least, token);
+      n = min(upto, p.top);
+      __syncthreads();
+    }
+  }
   if (n > kMany && n <= kMost) {
     // Few groups hold a logit, or many logits are equal: the candidates from the
     // top-th largest rank on, found bit by bit, are `top` exactly.
@@ -445,13 +531,10 @@ __global__ __launch_bounds__(64 * W, NV > 8 ? 4 : NV > 4 ? 6 : 8) void logprobs_
   }
   // Rare: the slice's logits are read again for each place.
   uint64_t last = ~uint64_t{0};
-  const int last_token = slices == 1 ? p.vocab : max(v1 * E - skew, first_token);
-  // The first of several slices has the row's last tokens too.
-  const int more = slices > 1 && slice == 0 ? p.vocab - (full1 * E - skew) : 0;
   for (int place = 0; place < p.top; ++place) {
     uint64_t mine = 0;
     for (int i = first_token + tid; i < last_token + more; i += N) {
-      const int token = i < last_token ? i : i - last_token + full1 * E - skew;
+      const int token = nth_token(i);
       const uint64_t rank = rank_of(to_f32(x[token]), token);
       if (rank < last && rank > mine) mine = rank;
     }

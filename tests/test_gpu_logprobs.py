@@ -221,6 +221,41 @@ def test_offsets_past_32_bits(cuda, vocab):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab,top,skew", [(1300, 20, 0), (32003, 5, 1), (32003, 64, 3),
+                                            (140003, 33, 5), (262144, 64, 0), (50001, 1, 7)])
+def test_thousands_of_equal_or_close_tokens(cuda, vocab, top, skew, dtype):
+    """More candidates than are ranked: rows of one value, masks of the type's
+    lowest value that leave fewer tokens than are asked for, tokens allowed in one
+    short range only, runs of equal ones at either end, and values of which
+    thousands are equal."""
+    G.note(f"logprobs ties {vocab} {top} {skew} {dtype}")
+    g = G.gen_of(vocab + top)
+    low = torch.finfo(dtype).min
+    x = torch.full((12, vocab), low, dtype=dtype)
+    x[0] = 0.0
+    x[1] = -3.5
+    few = torch.randperm(vocab, generator=g)[:3]
+    x[2, few] = torch.tensor([1.0, 3.0, 2.0], dtype=dtype)
+    x[3, [0, vocab - 1]] = 1.0
+    x[5, vocab // 3:vocab // 3 + 1200] = torch.randn(1200, generator=g).to(dtype)[:vocab - vocab // 3]
+    x[6:9] = -math.inf
+    x[6, vocab // 3:vocab // 3 + 1200] = x[5, vocab // 3:vocab // 3 + 1200]
+    x[7, -1200:] = 1.0
+    x[7, vocab // 2] = 4.0
+    x[8, :1200] = -1.0
+    x[8, -3:] = 0.0
+    x[9] = torch.randint(0, 3, (vocab,), generator=g).to(dtype)
+    x[10] = torch.randint(0, 3, (vocab,), generator=g).to(dtype)
+    x[10, few] = 7.0
+    x[11] = torch.arange(vocab).div(2000, rounding_mode="floor").to(dtype)
+    wide = torch.full((12, vocab + 8), math.nan, dtype=dtype, device=cuda)
+    y = wide[:, skew:skew + vocab]
+    y.copy_(x)
+    tokens = torch.randint(0, vocab, (12,), generator=g)
+    check(L.token_logprobs(y, tokens.to(cuda), top=top), x, tokens, top)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,vocab,top", [(3, 40, 3), (4, 1300, 20), (5, 32003, 5), (3, 140003, 64),
                                             (2, 300000, 0)])
 def test_rows_far_from_zero(cuda, rows, vocab, top, dtype):
