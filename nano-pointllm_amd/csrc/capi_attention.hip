@@ -77,23 +77,36 @@ inline i128 cache_bytes(const Cache& c) {
               i128(c.page_size - 1) * c.c_tok + c.dim);
 }
 
-// Whether no two rows of the cache, or of `layers` of them at a stride, share an
-// element: each stride covers the extent of the axes with smaller strides.
-inline bool cache_distinct(const Cache& c, int64_t c_layer = 0, int64_t layers = 1) {
-  int64_t stride[4] = {c_layer, c.c_page, c.c_head, c.c_tok};
-  int64_t count[4] = {layers, c.pages, c.heads, c.page_size};
+// The axes of a cache, or of `layers` of them at a stride, that have more than one
+// row, largest stride first.
+struct Axis {
+  int64_t stride, count;
+  i128 inner;   // elements that the axes of smaller strides and a row span
+};
+struct Axes {
+  Axis axis[4];
+  int n;
+};
+inline Axes axes_of(const Cache& c, int64_t c_layer, int64_t layers) {
+  Axes x{{{c_layer, layers, 0}, {c.c_page, c.pages, 0}, {c.c_head, c.heads, 0},
+          {c.c_tok, c.page_size, 0}}, 4};
+  x.n = static_cast<int>(std::remove_if(x.axis, x.axis + 4,
+                                        [](const Axis& a) { return a.count <= 1; }) - x.axis);
+  std::sort(x.axis, x.axis + x.n, [](const Axis& a, const Axis& b) { return a.stride > b.stride; });
   i128 extent = c.dim;
-  bool used[4] = {};
-  for (int n = 0; n < 4; ++n) {
-    int best = -1;
-    for (int i = 0; i < 4; ++i)
-      if (!used[i] && (best < 0 || stride[i] < stride[best])) best = i;
-    used[best] = true;
-    if (count[best] > 1) {
-      if (stride[best] < extent) return false;
-      extent += i128(count[best] - 1) * stride[best];
-    }
+  for (int i = x.n - 1; i >= 0; --i) {
+    x.axis[i].inner = extent;
+    extent += i128(x.axis[i].count - 1) * x.axis[i].stride;
   }
+  return x;
+}
+
+// Whether no two rows share an element: each stride covers the extent of the axes
+// with smaller strides.
+inline bool cache_distinct(const Cache& c, int64_t c_layer = 0, int64_t layers = 1) {
+  const Axes x = axes_of(c, c_layer, layers);
+  for (int i = 0; i < x.n; ++i)
+    if (x.axis[i].stride < x.axis[i].inner) return false;
   return true;
 }
 
@@ -103,17 +116,29 @@ inline bool clear_of(const Rows& r, const void* cache, const Cache& c) {
   return a0 + bytes_of(r) <= b0 || b0 + cache_bytes(c) <= a0;
 }
 
-// Whether k and v share no element: apart, or each inside the other's gaps
-// between layers (one tensor [layers, 2, ...]).
-inline bool caches_apart(const void* k, const void* v, const Cache& c, int64_t stride,
+// Whether a row of one cache and one of another of the same axes, `bytes` behind it,
+// share an element: whether differences d of their indexes bring bytes - sum of
+// 2 d stride to less than a row's length.  The strides cover what is inside them
+// (cache_distinct), so on every axis only the two d around the quotient can.
+inline bool rows_meet(const Axes& x, int i, i128 bytes, int64_t dim) {
+  if (i == x.n) return bytes > -2 * i128(dim) && bytes < 2 * i128(dim);
+  const Axis& a = x.axis[i];
+  const i128 step = 2 * i128(a.stride), d0 = bytes / step - (bytes % step < 0 ? 1 : 0);
+  for (i128 d = d0; d <= d0 + 1; ++d) {
+    const i128 rest = bytes - d * step;
+    if (d > -a.count && d < a.count && rest > -2 * a.inner && rest < 2 * a.inner &&
+        rows_meet(x, i + 1, rest, dim))
+      return true;
+  }
+  return false;
+}
+
+// Whether k and v, whose rows do not share elements among themselves, share none:
+// apart, or side by side within layers, pages, heads or tokens.
+inline bool caches_apart(const void* k, const void* v, const Cache& c, int64_t c_layer,
                          int64_t layers) {
   const i128 a = i128(reinterpret_cast<uintptr_t>(k)), b = i128(reinterpret_cast<uintptr_t>(v));
-  const i128 one = cache_bytes(c), all = one + 2 * i128(layers - 1) * stride;
-  if (a + all <= b || b + all <= a) return true;
-  if (layers == 1) return false;
-  const i128 step = 2 * i128(stride);
-  const i128 off = (((b - a) % step) + step) % step;
-  return off >= one && off + one <= step;
+  return !rows_meet(axes_of(c, c_layer, layers), 0, b - a, c.dim);
 }
 
 // log2 of a power of two up to 2^20, or -1.

@@ -588,7 +588,8 @@ def paged_accept(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch
     rising; -1 behind the path's end) go to place ``lengths[b] + i``, where
     ``lengths[b]`` (int32) keys were cached before the drafted ones.  The caches
     are one layer's, or ``[layers, pages, kv_heads, page_size, head_dim]``: all
-    layers in one launch (:meth:`PagedKVCache.accept`).  An entry below its
+    layers in one launch (:meth:`PagedKVCache.accept`); keys and values may be
+    views of one tensor, in any order of its axes.  An entry below its
     ``i`` moves nothing, as does a place outside the table or the cache.  The
     pages of the drafted tokens belong to one sequence only."""
     index = _gpu(k_cache, v_cache, page_table, lengths, path)
