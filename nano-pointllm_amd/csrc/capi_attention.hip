@@ -655,9 +655,11 @@ int w8a8_cache_accept(void* k_cache, void* v_cache, int64_t cache_stride_layer,
   if (!cache_distinct(c, cache_stride_layer, layers) ||
       !caches_apart(k_cache, v_cache, c, cache_stride_layer, layers))
     return W8A8_ERR_OVERLAP;
-  for (const auto& in : {std::pair<const void*, i128>{page_table, 4 * i128(batch) * ld_table},
-                         {lengths, 4 * i128(batch)},
-                         {path, 4 * i128(batch) * ld_path}}) {
+  // Up to the last row's last entry: what is behind it may be another tensor's.
+  for (const auto& in :
+       {std::pair<const void*, i128>{page_table, 4 * (i128(batch - 1) * ld_table + table_pages)},
+        {lengths, 4 * i128(batch)},
+        {path, 4 * (i128(batch - 1) * ld_path + path_length)}}) {
     const i128 a0 = i128(reinterpret_cast<uintptr_t>(in.first));
     for (const void* cache : {k_cache, v_cache}) {
       const i128 b0 = i128(reinterpret_cast<uintptr_t>(cache));

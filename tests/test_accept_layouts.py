@@ -96,3 +96,36 @@ def test_accepted_paths_in_every_order_of_axes(cuda, layers):
     assert torch.equal(store[:, 0].cpu(), want[0][0]) and torch.equal(store[:, 1].cpu(), want[1][0])
     with pytest.raises(Exception, match="overlap"):
         A.paged_accept(store[:, 0], store[:, 0], table, n, path)
+
+
+@no_gpu
+def test_tables_that_end_where_a_cache_begins():
+    """The last columns of a wide table or path: their last row ends with its own
+    entries, a whole row further would be inside the cache."""
+    n, ld, b = 4, 1000, 3
+    last = 4 * ((b - 1) * ld + n)
+    for cache in (H.KC, H.VC):
+        assert H._accept(table=cache - last, ld=ld, n=n, b=b) == _lib.ERR_HIP
+        assert H._accept(table=cache - last + 4, ld=ld, n=n, b=b) == _lib.ERR_OVERLAP
+        assert H._accept(path=cache - last, ld_path=ld, steps=n, b=b) == _lib.ERR_HIP
+        assert H._accept(path=cache - last + 4, ld_path=ld, steps=n, b=b) == _lib.ERR_OVERLAP
+        assert H._accept(lengths=cache - 4 * b, b=b) == _lib.ERR_HIP
+        assert H._accept(lengths=cache - 4 * b + 4, b=b) == _lib.ERR_OVERLAP
+
+
+@pytest.mark.gpu
+def test_accepted_paths_with_a_table_right_before_the_cache(cuda):
+    """Table and caches in one allocation, the table the last columns of a wide one."""
+    g, d, page, pages, ld, b = 2, 16, 4, 5, 1000, 2
+    cells = pages * g * page * d
+    room = torch.zeros(ld * 4 + 4 * cells, dtype=torch.uint8, device=cuda)
+    table = room[:ld * 4].view(torch.int32).as_strided((b, 3), (ld - 3, 1), 0)
+    table.copy_(torch.tensor([[3, 0, -1], [4, 1, 2]], dtype=torch.int32))
+    assert table.data_ptr() + 4 * ((b - 1) * (ld - 3) + 3) == room.data_ptr() + ld * 4
+    caches = room[ld * 4:].view(torch.float16).view(2, pages, g, page, d)
+    caches.copy_(torch.randn(caches.shape, generator=torch.Generator().manual_seed(1)))
+    n = torch.tensor([1, 5], dtype=torch.int32, device=cuda)
+    path = torch.tensor([[0, 2, 6], [1, 3, -1]], dtype=torch.int32, device=cuda)
+    want = [O.accept(c, table, n.cpu(), path.cpu()) for c in caches]
+    A.paged_accept(caches[0], caches[1], table, n, path)
+    assert torch.equal(caches[0].cpu(), want[0]) and torch.equal(caches[1].cpu(), want[1])
