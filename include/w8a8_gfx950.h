@@ -670,8 +670,9 @@ int64_t w8a8_paged_tree_workspace_bytes(int64_t tokens, int64_t batch, int64_t q
  * entries rise; one below i (behind the path's end: -1) moves nothing, and
  * neither does a place past the table or in a page outside [0, pages).  The pages
  * of places from lengths[b] on belong to one sequence only.  batch <= 65535,
- * layers <= 32767; k and v share no element, but may be views of one tensor, side
- * by side within layers, pages, heads or tokens ([pages, 2, ...]).
+ * layers <= 32767 and 2 layers x batch x ceil(kv_heads head_dim / 2048) < 2^24; k
+ * and v share no element, but may be views of one tensor, side by side within
+ * layers, pages, heads or tokens ([pages, 2, ...]).
  */
 int w8a8_cache_accept(void* k_cache, void* v_cache, int64_t cache_stride_layer,
                       int64_t cache_stride_page, int64_t cache_stride_head,

@@ -60,12 +60,21 @@ __global__ __launch_bounds__(kThreads) void accept_kernel(CacheAccept p) {
   }
 }
 
+// Workgroups of one layer's keys, for one sequence.
+int64_t groups_of(int64_t kv_heads, int64_t head_dim) {
+  return ceil_div(kv_heads * (head_dim / 8), kThreads);
+}
+
 }  // namespace
 
+int64_t cache_accept_workgroups(int64_t layers, int64_t batch, int64_t kv_heads,
+                                int64_t head_dim) {
+  return groups_of(kv_heads, head_dim) * 2 * layers * batch;
+}
+
 hipError_t launch_cache_accept(const CacheAccept& p, hipStream_t st) {
-  const int64_t threads = int64_t{p.kv_heads} * (p.head_dim / 8);
   hipLaunchKernelGGL(accept_kernel,
-                     dim3(static_cast<uint32_t>(ceil_div(threads, kThreads)), 2 * p.layers,
+                     dim3(static_cast<uint32_t>(groups_of(p.kv_heads, p.head_dim)), 2 * p.layers,
                           p.batch),
                      dim3(kThreads), 0, st, p);
   return hipGetLastError();

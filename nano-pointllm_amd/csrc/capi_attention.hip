@@ -632,7 +632,8 @@ int w8a8_cache_accept(void* k_cache, void* v_cache, int64_t cache_stride_layer,
                 page_size,         kv_heads,          head_dim};
   if (head_dim <= 0 || head_dim % 8 || head_dim > kAttentionMaxDim || kv_heads <= 0 ||
       kv_heads > kMaxHeads || batch < 0 || batch > kMaxGridYZ || layers < 0 ||
-      layers > kMaxGridYZ / 2)
+      layers > kMaxGridYZ / 2 ||
+      cache_accept_workgroups(layers, batch, kv_heads, head_dim) > kMaxBlocks)
     return W8A8_ERR_SHAPE;
   const int rc = check_cache(c, 8);
   if (rc != W8A8_OK) return rc;

@@ -340,6 +340,8 @@ struct CacheAccept {
   int max_keys;
   int layers, batch, kv_heads, head_dim;
 };
+// Workgroups of 256 threads of a call.
+int64_t cache_accept_workgroups(int64_t layers, int64_t batch, int64_t kv_heads, int64_t head_dim);
 hipError_t launch_cache_accept(const CacheAccept& p, hipStream_t st);
 
 // Log probabilities of given tokens from logits [rows, vocab] (logprobs.hip),

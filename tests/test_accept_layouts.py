@@ -98,6 +98,21 @@ def test_accepted_paths_in_every_order_of_axes(cuda, layers):
         A.paged_accept(store[:, 0], store[:, 0], table, n, path)
 
 
+def test_launches_past_32_bits_of_threads_are_refused():
+    """2^24 workgroups of 256 threads; with no page a call that is taken does
+    nothing."""
+    def call(**kw):
+        return H._accept(pages=0, cl=1 << 30, cs=(1 << 20, 1 << 10, 64), **kw)
+
+    assert call(b=65535, layers=64, g=32, d=128) == _lib.OK
+    assert call(b=65535, layers=65, g=32, d=128) == _lib.ERR_SHAPE
+    assert call(b=65535, layers=128, g=8, d=128) == _lib.OK
+    assert call(b=65535, layers=129, g=8, d=128) == _lib.ERR_SHAPE
+    assert call(b=65535, layers=64, g=33, d=128) == _lib.ERR_SHAPE
+    assert call(b=1, layers=32767, g=4096, d=256) == _lib.ERR_SHAPE
+    assert call(b=65535, layers=32767, g=1, d=8) == _lib.ERR_SHAPE
+
+
 @no_gpu
 def test_tables_that_end_where_a_cache_begins():
     """The last columns of a wide table or path: their last row ends with its own
