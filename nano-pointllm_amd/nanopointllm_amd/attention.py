@@ -744,7 +744,8 @@ class PagedAttentionCore:
     on a state whose tensors are then refilled in place between replays.
     ``window`` (one for all layers, or one or None for each) and ``sinks``
     limit what a row sees as in :func:`paged_decode`; sequences keep their own
-    positions, sinks included."""
+    positions, sinks included.  Where any layer has a window, trees of drafted
+    tokens are refused, by each layer before it stores anything."""
 
     def __init__(self, cache: PagedKVCache, frequencies: RotaryFrequencies, *,
                  layout: str = "half", scale: float | None = None,
@@ -769,9 +770,13 @@ class PagedAttentionCore:
         window = self.window[layer_index] if isinstance(self.window, list) else self.window
         sinks = 0 if window is None else self.sinks
         table, lengths, n = state.page_table, state.lengths, state.decode_rows
-        if state.masks is not None and (window is not None or state.q_starts is None):
-            raise ValueError("trees of drafted tokens run on layers without a window" if window
-                             else "masks need the q_starts of their trees")
+        if state.masks is not None:
+            if state.q_starts is None:
+                raise ValueError("masks need the q_starts of their trees")
+            # Of all layers, so that none has stored a step that a later one refuses.
+            windows = self.window if isinstance(self.window, list) else [self.window]
+            if any(w is not None for w in windows):
+                raise ValueError("trees of drafted tokens run on stacks without a window")
         q = rotary_store(q, k, v, state.positions, state.slots, self.frequencies.inv_freq,
                          k_cache, v_cache, layout=self.layout,
                          attention_factor=self.frequencies.attention_factor)
