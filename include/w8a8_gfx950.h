@@ -695,6 +695,8 @@ int w8a8_cache_accept(void* k_cache, void* v_cache, int64_t cache_stride_layer,
  * A term exp(x[j] - max) below 2^-126 counts as 0.  rows < 2^22 (2^17 where the
  * vocabulary passes 2^15), vocab <= 2^20; outputs are contiguous and overlap
  * nothing.
+ * How many workgroups a row is cut into, and with it the order of its sums, goes by
+ * the vocabulary, the type and whether there are more than 512 rows, nothing else.
  * Workspace: w8a8_token_logprobs_workspace_bytes(rows, vocab, top, dtype) bytes,
  * 16-byte aligned; no state survives the call.
  */

@@ -133,8 +133,12 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) 
     tokens of each row; -1 (a padded place) gives 0, another number outside the
     vocabulary NaN.  Among equal logits the lowest token comes first.  Sums and
     results are binary32; a logit of -inf has probability 0, a row with +inf,
-    NaN or nothing above -inf gives NaN.  One kernel for rows of up to 131072
-    16-bit logits (65536 binary32), two for longer ones; no autograd."""
+    NaN or nothing above -inf gives NaN.  No autograd.
+
+    Rows of up to 131072 16-bit logits (65536 binary32), in calls of more than 512
+    rows half of that, take one kernel; longer ones are cut and joined by a second.
+    A row's last bits may differ between the two, and so between calls of up to and
+    of more than 512 rows; otherwise they do not depend on the other rows."""
     # A decode step scores its rows eagerly, bounded by the host: each attribute is
     # read once, sizes of workspaces are kept by call.
     index = logits.get_device()
