@@ -644,9 +644,11 @@ int64_t w8a8_paged_prefill_window_workspace_bytes(int64_t tokens, int64_t batch,
  * of masks[row * ld_masks + j / 64] is set (its own among them only if its bit
  * is); key j of 64 * mask_words or more is not seen.  A row that sees no key is
  * zeros; clear_rows nonzero: so are rows of no sequence, else they are left as
- * they were.  Otherwise as w8a8_paged_prefill (heads of at most 128 with up to 32 rows,
- * tokens x q_heads / kv_heads, per sequence on average as w8a8_paged_decode: their
- * probabilities are not rounded to 16 bits).  Workspace: w8a8_paged_tree_workspace_bytes.
+ * they were.  Otherwise as w8a8_paged_prefill, whose probabilities are rounded to
+ * 16 bits; where the call's rows are at most 64 per sequence on average (tokens x
+ * q_heads / kv_heads <= 64 x batch) and its heads at most 128 as w8a8_paged_decode:
+ * they are not.  A tree's last bits therefore depend on the sizes of the trees it is
+ * called with.  Workspace: w8a8_paged_tree_workspace_bytes.
  */
 int w8a8_paged_tree(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_cache,
                     const void* v_cache, int64_t cache_stride_page, int64_t cache_stride_head,

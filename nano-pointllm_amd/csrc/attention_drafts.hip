@@ -2,7 +2,13 @@
 // up to 64 rows (token, query head) of a sequence and key head on average.
 //
 // Mathematics.  As attention_decode.hip: S^T = K Q^T, P = 2^(S^T c - r), O^T = V^T P,
-// l = sum P, with the rows as columns; a masked key's score is -inf.
+// l = sum P, with the rows as columns; a masked key's score is -inf.  P enters the
+// second product as two 16-bit parts (split2), so that the result's own rounding is
+// the only one that shows: rounded once, in O and l alike, it leaves 1.4 times that
+// error (of the norm 2.9e-4 and 2.1e-4 in binary16, 2.3e-3 and 1.7e-3 in bfloat16), and
+// the second part's products cost little next to the loads: 8 trees of 25 to 64 35.2
+// instead of 34.6 us, 4 of 64 behind 4032 59.8 and 59.4, 32 of 30 to 60 72 and 68, heads
+// of 64 55.6 and 52.4.
 //
 // Bound by memory: every key and value is read once per workgroup's 16 W rows, for up
 // to 64 rows.  4 trees of 64 behind 4032 keys of 32 heads (268 MB): 52 us and a join of
@@ -277,9 +283,6 @@ __global__ __launch_bounds__(64 * W * kParts, W == 4 ? 2 : 1) void tree_kernel(T
   constexpr int UB = kTile * RB;            // bytes of a unit of one operand
   constexpr int GN = kTile / 8 / W;         // groups of 8 keys that a wavefront copies
   constexpr int GL = 8 * RB / 1024;         // loads of a group and operand
-  // Few rows leave the matrix unit time for probabilities in two parts (split2);
-  // of many they are rounded once, in both products' sums alike.
-  constexpr bool SPLIT = W <= 2;
   // Arrays of their own, so that the compiler sees that one is read while loads into
   // the others are in flight.
   constexpr int SB = UB * kParts;           // a unit of each part
@@ -549,24 +552,19 @@ __global__ __launch_bounds__(64 * W * kParts, W == 4 ? 2 : 1) void tree_kernel(T
       float w[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) w[i] = exp2_hw(__builtin_fmaf(s[i >> 2][i & 3], sc, base));
-      if constexpr (SPLIT) l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+      l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
       u32x4 hi, lo;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        uint32_t y, z = 0;
-        if constexpr (SPLIT)
-          split2<T>(w[2 * i], w[2 * i + 1], y, z);
-        else
-          y = round2<T>(w[2 * i], w[2 * i + 1], l);
+        uint32_t y, z;
+        split2<T>(w[2 * i], w[2 * i + 1], y, z);
         hi[i] = y;
         lo[i] = z;
       }
 #pragma unroll
       for (int d = 0; d < DV; ++d) o[d] = mfma_16x16x32<T>(vf[d], hi, o[d]);
-      if constexpr (SPLIT) {
 #pragma unroll
-        for (int d = 0; d < DV; ++d) o[d] = mfma_16x16x32<T>(vf[d], lo, o[d]);
-      }
+      for (int d = 0; d < DV; ++d) o[d] = mfma_16x16x32<T>(vf[d], lo, o[d]);
     };
     // Both parts take as many steps, for their barriers.
     int t = tf;

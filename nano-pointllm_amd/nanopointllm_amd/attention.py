@@ -471,8 +471,13 @@ def paged_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     keys before those, and of the drafted ones key ``j`` where bit ``j % 64`` of
     ``masks[row, j // 64]`` is set (int64 ``[tokens, words]``, see
     :func:`tree_masks`; a row sees itself only if its own bit is set, and no key
-    past the words).  A row that sees no key is zeros.  Otherwise as
-    :func:`paged_prefill`."""
+    past the words).  A row that sees no key is zeros.
+
+    Trees of at most 64 rows (tokens x query heads of a key head) per sequence, on
+    the call's average, and heads of at most 128 have :func:`paged_decode`'s
+    arithmetic, others :func:`paged_prefill`'s, whose probabilities are rounded to
+    the rows' type: a tree's last bits, and how fast it runs, depend on the trees
+    that it is called with.  Otherwise as :func:`paged_prefill`."""
     return _prefill(q, k_cache, v_cache, page_table, lengths, q_starts, scale, out, out is None,
                     None, 0, masks)
 
