@@ -10,6 +10,8 @@ values that nearly cancel make e |out| and r small: a single rounding, e = 2^-11
 """
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -47,3 +49,40 @@ def test_probabilities_keep_two_parts(cuda, h, g, d, page, new, cached, dtype):
     err = (out.double().cpu() - want).abs()
     bad = ~(err <= tol)
     assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} off, worst {float((err / tol).max())}"
+
+
+@pytest.mark.parametrize("dtype", G.DTYPES)
+@pytest.mark.parametrize("cached,n", [(100, 50), (700, 64), (0, 40)])
+def test_values_that_only_some_of_many_rows_see(cuda, cached, n, dtype):
+    """An infinity and a NaN among the drafted values, and an infinite and a NaN key
+    that no row sees: they reach the rows that see them, and no others, in one piece
+    and in several."""
+    G.note(f"tree parts special values {cached} {n} {dtype}")
+    h = g = 2
+    d, page = 64, 16
+    k, v, table = G.paged(8, [cached + n], g, d, page, dtype, cuda)
+
+    def row(cache, node):
+        at = cached + node
+        return cache[int(table[0, at // page]), :, at % page]
+
+    row(v, 5)[:, 3], row(v, 5)[:, 7] = math.inf, math.nan
+    row(k, 9)[:, 1], row(k, 11)[:, 2] = math.inf, math.nan
+    row(v, 9)[:], row(v, 11)[:] = math.nan, -math.inf
+    masks = A.tree_masks([[-1, 0, 1, 2, 3] + [4 if i % 2 else i - 1 for i in range(5, n)]],
+                         device="cpu")
+    masks &= ~(1 << 9 | 1 << 11)
+    q = G.randn(G.gen_of(2), n, h, d, dtype=dtype, device=cuda)
+    lengths = torch.tensor([cached + n], dtype=torch.int32, device=cuda)
+    starts = torch.tensor([0, n], dtype=torch.int32, device=cuda)
+    out = A.paged_tree(q, k, v, table, lengths, starts, masks.to(cuda))
+    sees = O.tree_sight(masks, cached + n)[:, cached + 5].to(cuda)
+    assert 0 < int(sees.sum()) < n
+    assert (out[sees][..., 3] == math.inf).all() and out[sees][..., 7].isnan().all()
+    assert torch.isfinite(out[~sees]).all()
+    keep = [i for i in range(d) if i not in (3, 7)]
+    assert torch.isfinite(out[..., keep]).all()
+    # The others to the bit what they are without those values.
+    row(v, 5)[:, 3], row(v, 5)[:, 7] = 0.25, -0.5
+    want = A.paged_tree(q, k, v, table, lengths, starts, masks.to(cuda))
+    assert torch.isfinite(want).all() and torch.equal(out[~sees], want[~sees])
