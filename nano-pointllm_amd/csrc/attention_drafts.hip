@@ -11,11 +11,12 @@
 // of 64 55.6 and 52.4.
 //
 // Bound by memory: every key and value is read once per workgroup's 16 W rows, for up
-// to 64 rows.  4 trees of 64 behind 4032 keys of 32 heads (268 MB): 52 us and a join of
-// 5, 5.2 TB/s; one of 64 behind 16320: 51 us in all.  8 of 25 to 64 behind 630 to 1590
-// keys (169 MB) are 256 workgroups, of which the longest walks 26 steps: 39 us.  A
-// small call is bound by its launches: 26 rows of 32 heads behind 601 keys take 11 us
-// and the join 4.
+// to 64 rows.  4 trees of 64 behind 4032 keys of 32 heads (268 MB): 50 us and a join of
+// 12, 5.4 TB/s; one of 64 behind 16320: 50 us and a join of 5, back to back 52.5.  8 of
+// 25 to 64 behind 630 to 1590 keys (169 MB) are 256 workgroups, of which the longest
+// walks 26 steps: 35 to 40 us.  A small call is bound by its launches: 26 rows of 32
+// heads behind 601 keys take 9 us and the join 4.  The comparisons below were made
+// while more than 32 rows rounded P once.
 //
 // Design:
 //   * A workgroup takes 16 rows per wavefront of one key head, and a piece of the
@@ -757,8 +758,8 @@ template <typename T> hipError_t launch_t(const TreeParams& p, const Plan& x, hi
 }  // namespace
 
 // More rows than that have few keys per operation: they run as a prompt's, 128 rows to
-// a key (4 trees of 33 to 45 tokens, 32 heads over 8, behind 32768: 147 us, here 209; 8
-// of 48 behind 4048: 64 and 102; one of 64 behind 32704: 84 and 75).
+// a key (4 trees of 33 to 45 tokens, 32 heads over 8, behind 32768: 148 us, here 220; 8
+// of 48 behind 4048: 58 and 77; one of 64 behind 32704: 81 and 77).
 bool small_trees(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
                  int64_t head_dim) {
   const int64_t rows = tokens * (q_heads / kv_heads);

@@ -3,11 +3,13 @@
 // between the two are neither read nor computed, nor are their pages looked up.
 //
 // Bound as a prompt without a window: 16384 tokens of 32 heads over 8 with a window of
-// 4096 take 0.99 to 1.04 ms (0.93 to 0.98 PFLOP/s of what is seen), 5 of the 131 units
-// of a row tile with masks.  A short prompt is one row tile's units in a row: 560 tokens
-// of 32 heads take 12.5 us with a window of 32 keys, 14.9 with 128, 17.8 with 256, and
-// 19.7 with one of 559; 10 of the 13 units of a window of 256 have masks, which cost
-// about 0.25 us each on top of a unit's 0.55.
+// 4096 take 0.99 to 1.05 ms (0.92 to 0.98 PFLOP/s of what is seen) once the clock has
+// settled, up to 1.18 ms in the first dozen launches after idle time; 5 of the 131
+// units of a row tile have masks.  A short prompt is one row tile's units in a row: 560
+// tokens of 32 heads take 11.4 us with a window of one key, 12.4 with 32, 15.1 with 128,
+// 17.9 with 256, and 19.3 with one of 559 (calls in a captured graph; back to back 0.2
+// more, as a trace's durations 0.6 more); 10 of the 13 units of a window of 256 have
+// masks, which cost about 0.25 us each on top of a unit's 0.55.
 #include "attention_prefill.h"
 
 namespace w8a8 {
