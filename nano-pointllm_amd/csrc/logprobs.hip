@@ -529,14 +529,15 @@ __global__ __launch_bounds__(64 * W, NV > 8 ? 4 : NV > 4 ? 6 : 8) void logprobs_
     for (int i = n + tid; i < p.top; i += N) write(i, 0);   // a short slice
     return;
   }
-  // Rare: the slice's logits are read again for each place.
+  // Rare (thousands of NaN): the slice's logits are read again for each place.  A NaN of
+  // token 0 has the largest rank that there is, so the first place takes any.
   uint64_t last = ~uint64_t{0};
   for (int place = 0; place < p.top; ++place) {
     uint64_t mine = 0;
     for (int i = first_token + tid; i < last_token + more; i += N) {
       const int token = nth_token(i);
       const uint64_t rank = rank_of(to_f32(x[token]), token);
-      if (rank < last && rank > mine) mine = rank;
+      if ((place == 0 || rank < last) && rank > mine) mine = rank;
     }
     mine = wave_max64(mine);
     if (lane == 0) best[wave] = mine;

@@ -179,3 +179,34 @@ def test_one_row_more_than_keep_a_workgroup_each(cuda, vocab, dtype, top):
             assert a is None or torch.equal(a, b[:few])
     if top:
         assert torch.equal(outs[512].top_tokens, outs[513].top_tokens[:512])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [40, 1000, 1025, 5003, 65537, 140003, 262147])
+@pytest.mark.parametrize("top", [1, 33])
+def test_rows_of_many_nan(cuda, top, vocab, dtype):
+    """More NaN than candidates are ranked, the first token's and the last one's
+    among them: they come first, by their number, then infinity."""
+    G.note(f"logprobs many nan {vocab} {top} {dtype}")
+    x = torch.zeros(8, vocab, dtype=dtype, device=cuda)
+    x[0] = math.nan
+    x[1, 1:] = math.nan
+    x[2, :-1] = math.nan
+    x[3, ::2] = math.nan
+    x[4, 1::2] = math.nan
+    x[4, 0] = math.inf
+    x[5] = math.inf
+    x[5, :12] = math.nan
+    x[6] = -math.inf
+    x[6, 0] = math.nan
+    x[7] = math.inf
+    x[7, vocab - 1] = math.nan
+    tokens = torch.zeros(8, dtype=torch.int64, device=cuda)
+    out = L.token_logprobs(x, tokens, top=top)
+    value = x.double().cpu()
+    key = torch.where(value.isnan(), 3.0, torch.where(value == math.inf, 2.0, torch.where(
+        value == 0, 1.0, 0.0)))
+    want = torch.sort(key, stable=True, dim=-1, descending=True).indices[:, :top]
+    assert torch.equal(out.top_tokens.cpu(), want)
+    assert out.logprobs.isnan().all() and out.entropy.isnan().all()
+    assert out.top_logprobs.isnan().all()
